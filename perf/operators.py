@@ -391,12 +391,13 @@ def _run_own(s):
         out, lse = dfattn.kv8_attention(s["cache"], s["q"], s["table"], s["query_start"], s["seq_lens"], s["heads"],
                                         s["max_q"], s["max_len"], s["scale"])
         return {"out": out, "lse": lse}
-    logprob, entropy, lse, ids, top = ops.token_logprobs_forward(s["logits"], s["tokens"], s["top"])
+    logprob, entropy, stats, ids, top = ops.token_logprobs_forward(s["logits"], s["tokens"], s["top"])
     out = {"logprob": logprob, "entropy": entropy}
     if s["top"]:
         out["top_ids"], out["top_logprobs"] = ids, top
     if s["grad"]:
-        out["grad"] = ops.token_logprobs_backward(s["logits"], s["tokens"], lse, entropy, s["g_logprob"], s["g_entropy"])
+        out["grad"] = ops.token_logprobs_backward(s["logits"], s["tokens"], stats, entropy, s["g_logprob"],
+                                                  s["g_entropy"])
     return out
 
 
