@@ -11,7 +11,9 @@ The library's C ABI is include/dfattn.h. This module loads the in-tree build
 * ``AttentionContext``, the mirror of the reference's per-layer context
   (darkforest-cuda/src/lib.rs:1949-2368), and the host-slice helpers
   ``fused_attention_forward`` / ``attention_backward_host`` (lib.rs:2371, 2421);
-* ``FusedCausalAttention``, a torch.autograd.Function over the fast path.
+* ``FusedCausalAttention``, a torch.autograd.Function over the fast path;
+* serving batches of requests from a paged 8-bit cache (``paged_plan``,
+  ``kv8_cache``, ``kv8_append``, ``kv8_read``, ``kv8_attention``: kv8.py).
 
 There is no CPU fallback: if the library is missing every call raises
 ``DfattnNotBuilt``.
@@ -34,6 +36,7 @@ STATUS_NAMES = {
     -5: "DFATTN_ERR_OVERFLOW",
     -6: "DFATTN_ERR_WORKSPACE",
     -7: "DFATTN_ERR_HIP",
+    -8: "DFATTN_ERR_FLAGS",
 }
 
 # Every symbol include/dfattn.h declares, with (restype, argtypes).
@@ -68,6 +71,12 @@ SYMBOLS = {
     "launch_paged_copy_row_f32_to_bf16": (None, [_P, _P, ctypes.c_int32, _U32, _U32, _U32]),
     "dfattn_decode_workspace_bytes": (ctypes.c_size_t, [_U32, _U32, _U32]),
     "dfattn_decode": (ctypes.c_int, [_P] * 4 + [_U32, _U32, _P, _P, _U32, _U32, _U32, _F, _P, ctypes.c_size_t, _P]),
+    "dfattn_paged_plan": (ctypes.c_int, [_P] * 9 + [_U32] * 6 + [_P]),
+    "dfattn_kv8_pool_bytes": (ctypes.c_size_t, [_U32] * 4),
+    "dfattn_kv8_append": (ctypes.c_int, [_P] * 7 + [_U32] * 8 + [_P]),
+    "dfattn_kv8_read": (ctypes.c_int, [_P] * 7 + [_U32] * 7 + [_P]),
+    "dfattn_kv8_attention_workspace_bytes": (ctypes.c_size_t, [_U32] * 7),
+    "dfattn_kv8_attention": (ctypes.c_int, [_P] * 10 + [_U32] * 13 + [_F, _U32, _P, ctypes.c_size_t, _P]),
     "dfattn_status_string": (ctypes.c_char_p, [ctypes.c_int]),
     "dfattn_last_error": (ctypes.c_int, []),
     "dfattn_last_error_message": (ctypes.c_char_p, []),
@@ -650,3 +659,8 @@ class FusedCausalAttention:
             cls._fn = _Fn
         d_head = q.shape[1] // n_heads
         return cls._fn.apply(q, k, v, n_heads, d_head ** -0.5 if scale is None else scale, causal)
+
+
+# ---------------------------------------------------------------- the paged 8-bit cache
+from .kv8 import (KV_E4M3, KV_I8, KV8Cache, kv8_append, kv8_attention,  # noqa: E402
+                  kv8_attention_workspace_bytes, kv8_cache, kv8_read, paged_plan)

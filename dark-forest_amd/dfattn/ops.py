@@ -5,6 +5,8 @@
   elementwise.cu:195, 217; matmul.cu:240) on fresh output tensors;
 * `logit_ce_chunk` / `sum_into`, `embedding_forward` / `embedding_backward`: the chunked fused
   cross-entropy (softmax.cu:396) and the token embedding and its gradient (elementwise.cu:268, 291);
+* `token_logprobs` (autograd), `token_logprobs_forward` / `token_logprobs_backward`: log probabilities of given
+  tokens with the rows' entropy and largest alternatives, and the logits' gradient;
 * `ParamArena` / `ArenaAdamW`: the engine's single allocation for its weights, gradients and AdamW
   moments (static_gpt2.rs:401-567) and its AdamW update (matmul.cu:341, lib.rs:1755-1788) as one
   launch over the whole arena, with the step count on the device.
@@ -57,6 +59,8 @@ SYMBOLS = {
     "dfgpt2_linear_forward": (_I, [_P] * 5 + [_U32, _U32, _U32, _P]),
     "dfgpt2_linear_backward_input": (_I, [_P] * 4 + [_U32, _U32, _U32, _P]),
     "dfgpt2_linear_backward_weight": (_I, [_P] * 3 + [_U32, _U32, _U32, _P]),
+    "dfgpt2_token_logprobs": (_I, [_P] * 7 + [_U32] * 5 + [_P]),
+    "dfgpt2_token_logprobs_backward": (_I, [_P] * 7 + [_U32] * 4 + [_P]),
     "dfgpt2_layernorm_backward_fused": (_I, [_P] * 11 + [_SZ, _U32, _U32, _P]),
 }
 
@@ -234,6 +238,94 @@ def embedding_backward(ids, grad_out, grad_table):
     rows_in_table, dim = _rows_cols(grad_table)
     _check(ops_lib().dfgpt2_embedding_backward(_ids_ptr(ids), _dev_ptr(grad_out), _dev_ptr(grad_table), ids.numel(),
                                                dim, rows_in_table, _stream_ptr()))
+
+
+def _logit_rows(t):
+    """(pointer, row stride, type code) of float32 or bfloat16 logits [rows, V] with contiguous rows."""
+    torch = _torch()
+    if not t.is_cuda or t.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("logits must be a float32 or bfloat16 device tensor")
+    rows, v = _rows_cols(t)
+    stride = t.stride(0) if rows > 1 else v
+    if (t.stride(1) != 1 and v > 1) or stride < v:
+        raise ValueError("logits must be [rows, V] with contiguous rows")
+    return t.data_ptr(), stride, 0 if t.dtype == torch.float32 else 1
+
+
+def _same_device(t, *others):
+    torch = _torch()
+    if t.device.index != torch._C._cuda_getDevice() or any(o is not None and o.device != t.device for o in others):
+        raise ValueError("the tensors must be on the current device")
+
+
+def token_logprobs_forward(logits, tokens, top_k=0):
+    """dfgpt2_token_logprobs over logits [rows, V] (float32 or bfloat16, rows may be a column block of a wider
+    tensor) and int32 tokens [rows]. Returns (logprob [rows], entropy [rows], stats [rows, 2], top_ids [rows, top_k] int32,
+    top_logprobs [rows, top_k]); stats holds each row's maximum and ln sum exp(x - maximum)."""
+    torch = _torch()
+    rows, v = _rows_cols(logits)
+    p, stride, dtype = _logit_rows(logits)
+    _same_device(logits, tokens)
+    if tokens.shape != (rows,):
+        raise ValueError("tokens must be [rows]")
+    dev = logits.device
+    logprob, entropy = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    _check(ops_lib().dfgpt2_token_logprobs(p, _ids_ptr(tokens), logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                                           ids.data_ptr(), top.data_ptr(), dtype, rows, v, stride, top_k,
+                                           _stream_ptr()))
+    return logprob, entropy, stats, ids, top
+
+
+def token_logprobs_backward(logits, tokens, stats, entropy, grad_logprob=None, grad_entropy=None, out=None):
+    """dfgpt2_token_logprobs_backward: the gradient of the logits [rows, V] in their type, from the forward's stats
+    and entropy; a gradient that is None is 0. out may be the logits themselves where they are contiguous."""
+    torch = _torch()
+    rows, v = _rows_cols(logits)
+    p, stride, dtype = _logit_rows(logits)
+    _same_device(logits, tokens, stats, entropy, grad_logprob, grad_entropy, out)
+    out = torch.empty((rows, v), dtype=logits.dtype, device=logits.device) if out is None else out
+    if out.shape != (rows, v) or out.dtype != logits.dtype or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor like the logits")
+    if any(t is not None and t.shape != (rows,) for t in (tokens, entropy, grad_logprob, grad_entropy)) or \
+            stats.shape != (rows, 2):
+        raise ValueError("tokens, entropy and the gradients must be [rows], stats [rows, 2]")
+    _check(ops_lib().dfgpt2_token_logprobs_backward(p, _ids_ptr(tokens), _dev_ptr(stats), _dev_ptr(entropy),
+                                                    _dev_ptr(grad_logprob), _dev_ptr(grad_entropy), out.data_ptr(),
+                                                    dtype, rows, v, stride, _stream_ptr()))
+    return out
+
+
+_token_logprobs_fn = None
+
+
+def token_logprobs(logits, tokens, top_k=0):
+    """(logprob, entropy, top_ids, top_logprobs) of token_logprobs_forward, differentiable in logits through
+    logprob and entropy (the alternatives carry no gradient)."""
+    global _token_logprobs_fn
+    if _token_logprobs_fn is None:
+        torch = _torch()
+
+        class _Fn(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, logits, tokens, top_k):
+                logprob, entropy, stats, ids, top = token_logprobs_forward(logits, tokens, top_k)
+                ctx.save_for_backward(logits, tokens, stats, entropy)
+                ctx.mark_non_differentiable(ids, top)
+                ctx.set_materialize_grads(False)
+                return logprob, entropy, ids, top
+
+            @staticmethod
+            def backward(ctx, g_logprob, g_entropy, _ids, _top):
+                if g_logprob is None and g_entropy is None:
+                    return None, None, None
+                c = lambda g: None if g is None else g.contiguous()
+                return token_logprobs_backward(*ctx.saved_tensors, c(g_logprob), c(g_entropy)), None, None
+
+        _token_logprobs_fn = _Fn
+    return _token_logprobs_fn.apply(logits, tokens, top_k)
 
 
 class ParamArena:

@@ -62,6 +62,12 @@ typedef enum dfattn_status {
 #define DFATTN_KV_F32 0u  /* fp32 rows                                        */
 #define DFATTN_KV_BF16 1u /* bf16 bit patterns in uint16 (the reference's      */
                           /* __nv_bfloat16 pools)                             */
+/* Element types of the 8-bit caches (dfattn_kv8_*), two's complement int8 and
+ * the OCP fp8 format e4m3 (largest value 448). */
+#define DFATTN_KV_I8 2u
+#define DFATTN_KV_E4M3 3u
+/* A slot that is none (dfattn_paged_plan's map behind the last token). */
+#define DFATTN_NO_SLOT 0xffffffffu
 
 /* ---- Group 1: the reference's launcher symbols ---------------------------
  * Same signatures as the reference. Launches go to the legacy default (null)
@@ -327,6 +333,112 @@ int dfattn_decode(const float *q, const void *k_cache, const void *v_cache,
                   uint32_t kv_dtype, float *out, float *lse, uint32_t n_heads,
                   uint32_t cur_seq_len, uint32_t d_head, float scale,
                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- Serving: batches of requests over a paged 8-bit cache ---------------
+ * No counterparts in the reference, whose paged cache holds fp32 or bf16 rows
+ * of one request (paged_kv.rs). All take device pointers and a stream, allocate
+ * nothing, read no device value on the host and may be captured into a graph.
+ * uint32 arrays hold ids and lengths (page ids and slots as the block tables
+ * above: int32 values of the same bits).
+ *
+ * A batch of requests. Request r owns the tokens query_start[r] ..
+ * query_start[r+1]-1 of this step, packed one after the other, and seq_lens[r]
+ * cached tokens including those, in pages block_table[r*max_pages + i]: its
+ * position t is slot page * page_size + t % page_size of page
+ * block_table[r*max_pages + t / page_size].
+ *
+ * dfattn_paged_plan makes that description on the device from the lengths:
+ * request r has cached_lens[r] tokens in its pages and gets new_lens[r] more.
+ * Pages are taken in order from free_pages[*free_start .. n_free-1]. Requests
+ * are admitted in order up to the first that does not fit (more than max_pages
+ * pages, no pages left, or more than token_capacity tokens in all); that one
+ * and those after it take no part: no tokens, seq_lens[r] = cached_lens[r],
+ * their table rows untouched. Writes the new entries of block_table (others are
+ * left as they are), seq_lens [R], query_start [R+1], slot_map
+ * [token_capacity] (the slot of each token; DFATTN_NO_SLOT behind the last, and
+ * where a page id is not below n_pages) and counts [3]: requests admitted,
+ * tokens, and the next call's free_start. Outputs must not overlap inputs
+ * (counts + 2 is not free_start: copy it between calls). n_requests <= 8192,
+ * page_size any, n_pages * page_size <= 2^31. Latency: 4-6 us.               */
+int dfattn_paged_plan(const uint32_t *cached_lens, const uint32_t *new_lens,
+                      const uint32_t *free_pages, const uint32_t *free_start,
+                      uint32_t *block_table, uint32_t *seq_lens,
+                      uint32_t *query_start, uint32_t *slot_map, uint32_t *counts,
+                      uint32_t n_free, uint32_t n_requests, uint32_t max_pages,
+                      uint32_t token_capacity, uint32_t page_size,
+                      uint32_t n_pages, void *stream);
+
+/* The 8-bit cache: codes of one byte and, for each page and kv head, one fp32
+ * scale; a value is code * scale. k_pool is [n_pages, n_kv_heads, page_size,
+ * Dp], v_pool [n_pages, n_kv_heads, Dp, page_size] (a page's values of one
+ * column lie together, as the attention's second product reads them), Dp =
+ * d_head rounded up to 16; k_scales and v_scales are [n_pages, n_kv_heads].
+ * page_size is a multiple of 16 up to 256, d_head 1..128, pools 16-byte
+ * aligned. dfattn_kv8_pool_bytes is the size of one pool (0 for invalid
+ * arguments); a pool needs no initial contents.                              */
+size_t dfattn_kv8_pool_bytes(uint32_t n_pages, uint32_t n_kv_heads, uint32_t page_size,
+                             uint32_t d_head);
+
+/* Append: row i of k and v [n_tokens, n_kv_heads*d_head] goes to slot
+ * slot_map[i] (rows whose slot is not in the pool are left out). The rows
+ * of one page must stand next to each other in the map with rising slots, as
+ * dfattn_paged_plan's maps have them; else the contents of that page are
+ * unspecified. A page's rows before the first one written are kept, those
+ * after the last are unspecified. Scales are powers of two: the smallest s
+ * >= 2^-126 with |x| <= 127 s (int8) or 448 s (e4m3) for every new value, and
+ * not below the page's scale where rows are kept. A new value is rounded once,
+ * to the nearest code (ties to even; the quotient by s is exact); kept rows
+ * are rounded again only when s grows. A page and head that is given an
+ * infinity or NaN gets the scale NaN: all its values are NaN until its first
+ * row is written again. (A number within half a step of 2^128 reads as
+ * infinity.) act_dtype: DFATTN_KV_F32 or DFATTN_KV_BF16, the
+ * type of k and v, whose rows start row_stride elements apart.               */
+int dfattn_kv8_append(const void *k, const void *v, const uint32_t *slot_map, void *k_pool,
+                      void *v_pool, float *k_scales, float *v_scales, uint32_t act_dtype,
+                      uint32_t kv_dtype, uint32_t n_tokens, uint32_t n_kv_heads,
+                      uint32_t d_head, uint32_t page_size, uint32_t n_pages,
+                      uint32_t row_stride, void *stream);
+
+/* Read back: rows k_out[i], v_out[i] [n_rows, n_kv_heads*d_head] := the values
+ * code * scale of slots[i], in act_dtype; zeros where the slot is not in the
+ * pool. Slots in any order, any number of times.                             */
+int dfattn_kv8_read(const void *k_pool, const void *v_pool, const float *k_scales,
+                    const float *v_scales, const uint32_t *slots, void *k_out, void *v_out,
+                    uint32_t act_dtype, uint32_t kv_dtype, uint32_t n_rows,
+                    uint32_t n_kv_heads, uint32_t d_head, uint32_t page_size,
+                    uint32_t n_pages, void *stream);
+
+/* Attention of a batch over its pages: q and out [n_tokens, n_heads*d_head] in
+ * act_dtype (rows q_row_stride elements apart in q, contiguous in out), head h
+ * reading kv head h / (n_heads / n_kv_heads). Query j of the n of request r
+ * stands at position seq_lens[r] - n + j and sees the cached positions up to
+ * its own (causal != 0) or all seq_lens[r]. out = softmax(scale q k) v; lse
+ * [n_heads, n_tokens] (may be NULL): natural log of the sum of exp(scale q k).
+ * A row that sees nothing gets zeros and -infinity. Rows from
+ * query_start[R] on are left as they are. Keys in a page whose id is not below
+ * n_pages are left out; a table entry past a request's length is not read.
+ * max_query_len and max_seq_len are bounds the caller knows of the lengths on
+ * the device; queries past max_query_len are not computed, a longer sequence
+ * only costs time. Softmax statistics and sums are fp32; with fp32 activations
+ * q and P enter the matrix products as two fp16 terms (22 bits), with bf16
+ * as one (12 bits at least). |scale q| must stay below fp32's range over 2^16.
+ * Workspace: dfattn_kv8_attention_workspace_bytes of the same sizes (0: none
+ * needed); NULL: no split over the keys, one workgroup walks each row's. Calls
+ * that may overlap need one each. Results are reproducible bit for bit.      */
+size_t dfattn_kv8_attention_workspace_bytes(uint32_t n_requests, uint32_t n_tokens,
+                                            uint32_t max_query_len, uint32_t max_seq_len,
+                                            uint32_t n_heads, uint32_t n_kv_heads,
+                                            uint32_t d_head);
+int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool,
+                         const float *k_scales, const float *v_scales,
+                         const uint32_t *block_table, const uint32_t *query_start,
+                         const uint32_t *seq_lens, void *out, float *lse,
+                         uint32_t act_dtype, uint32_t kv_dtype, uint32_t n_requests,
+                         uint32_t n_tokens, uint32_t max_query_len, uint32_t max_seq_len,
+                         uint32_t n_heads, uint32_t n_kv_heads, uint32_t d_head,
+                         uint32_t page_size, uint32_t n_pages, uint32_t max_pages,
+                         uint32_t q_row_stride, float scale, uint32_t causal,
+                         void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---- Group 3: the reference's per-layer attention context ---------------
  * Mirror of AttentionContext (darkforest-cuda/src/lib.rs:1949-2368), the

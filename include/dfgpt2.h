@@ -156,6 +156,27 @@ int dfgpt2_linear_backward_input(const float *grad_out, const float *w, const fl
 int dfgpt2_linear_backward_weight(const float *grad_out, const float *x, float *grad_w, uint32_t rows,
                                   uint32_t in_features, uint32_t out_features, hipStream_t stream);
 
+/* Log probabilities of given tokens (no reference counterpart; the chunked cross-entropy above gives
+ * a mean loss only). Per row of logits [rows, cols] (dtype DFATTN_KV_F32 or DFATTN_KV_BF16, rows
+ * row_stride elements apart), with p the row's softmax: logprob = ln p[token], entropy = -sum p ln p,
+ * stats [rows, 2] = the row's maximum m and ln sum exp(x - m), and the top_k (0..64, <= cols) largest
+ * logits' ids and ln p, largest first, equal logits in the order of their ids, NaN above all numbers
+ * (top_ids, top_logprobs [rows, top_k]; may be NULL when top_k is 0). entropy and stats may be NULL.
+ * Values of -infinity are masked out (p = 0); a row of nothing else has m, logprob and top_logprobs
+ * -infinity and entropy 0. A NaN or +infinity makes its row's results NaN (the ids stay). A token that
+ * is not below cols has logprob 0. Statistics are fp32, in one fixed order of sums. rows <= 2^21.
+ * backward: grad_logits [rows, cols] (the logits' type, contiguous, overwritten; may be logits itself
+ * when that is contiguous) = grad_logprob (1[j = token] - p_j) - grad_entropy p_j (ln p_j + entropy), from
+ * the forward's stats and entropy; either gradient may be NULL (0). A masked-out value and a row of
+ * nothing else get 0; a token that is not below cols gets nothing of grad_logprob.           */
+int dfgpt2_token_logprobs(const void *logits, const uint32_t *tokens, float *logprob, float *entropy, float *stats,
+                          uint32_t *top_ids, float *top_logprobs, uint32_t dtype, uint32_t rows, uint32_t cols,
+                          uint32_t row_stride, uint32_t top_k, hipStream_t stream);
+int dfgpt2_token_logprobs_backward(const void *logits, const uint32_t *tokens, const float *stats,
+                                   const float *entropy, const float *grad_logprob, const float *grad_entropy,
+                                   void *grad_logits, uint32_t dtype, uint32_t rows, uint32_t cols,
+                                   uint32_t row_stride, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -27,6 +27,11 @@ pub const DFATTN_BWD_QKV_SAVED: u32 = 1;
 /// `dfattn_decode` cache element types.
 pub const DFATTN_KV_F32: u32 = 0;
 pub const DFATTN_KV_BF16: u32 = 1;
+/// Element types of the 8-bit caches (`dfattn_kv8_*`).
+pub const DFATTN_KV_I8: u32 = 2;
+pub const DFATTN_KV_E4M3: u32 = 3;
+/// A slot that is none (`dfattn_paged_plan`).
+pub const DFATTN_NO_SLOT: u32 = 0xffffffff;
 /// Bytes of the static device array `dfattn_bwd_noalloc` uses as its workspace (per GPU).
 pub const DFATTN_NOALLOC_SCRATCH_BYTES: usize = 32 << 20;
 
@@ -143,6 +148,33 @@ extern "C" {
     pub fn dfattn_attention_backward(q: *const f32, k: *const f32, v: *const f32, d_out: *const f32,
                                      len: usize, seq_len: u32, d_head: u32, scale: f32, causal: u32,
                                      d_q: *mut f32, d_k: *mut f32, d_v: *mut f32) -> c_int;
+
+    // Serving from a paged 8-bit cache: tables and slot maps, append, read-back, attention.
+    pub fn dfattn_paged_plan(cached_lens: *const u32, new_lens: *const u32, free_pages: *const u32,
+                             free_start: *const u32, block_table: *mut u32, seq_lens: *mut u32,
+                             query_start: *mut u32, slot_map: *mut u32, counts: *mut u32, n_free: u32,
+                             n_requests: u32, max_pages: u32, token_capacity: u32, page_size: u32,
+                             n_pages: u32, stream: *mut c_void) -> c_int;
+    pub fn dfattn_kv8_pool_bytes(n_pages: u32, n_kv_heads: u32, page_size: u32, d_head: u32) -> usize;
+    pub fn dfattn_kv8_append(k: *const c_void, v: *const c_void, slot_map: *const u32, k_pool: *mut c_void,
+                             v_pool: *mut c_void, k_scales: *mut f32, v_scales: *mut f32, act_dtype: u32,
+                             kv_dtype: u32, n_tokens: u32, n_kv_heads: u32, d_head: u32, page_size: u32,
+                             n_pages: u32, row_stride: u32, stream: *mut c_void) -> c_int;
+    pub fn dfattn_kv8_read(k_pool: *const c_void, v_pool: *const c_void, k_scales: *const f32,
+                           v_scales: *const f32, slots: *const u32, k_out: *mut c_void, v_out: *mut c_void,
+                           act_dtype: u32, kv_dtype: u32, n_rows: u32, n_kv_heads: u32, d_head: u32,
+                           page_size: u32, n_pages: u32, stream: *mut c_void) -> c_int;
+    pub fn dfattn_kv8_attention_workspace_bytes(n_requests: u32, n_tokens: u32, max_query_len: u32,
+                                                max_seq_len: u32, n_heads: u32, n_kv_heads: u32,
+                                                d_head: u32) -> usize;
+    pub fn dfattn_kv8_attention(q: *const c_void, k_pool: *const c_void, v_pool: *const c_void,
+                                k_scales: *const f32, v_scales: *const f32, block_table: *const u32,
+                                query_start: *const u32, seq_lens: *const u32, out: *mut c_void, lse: *mut f32,
+                                act_dtype: u32, kv_dtype: u32, n_requests: u32, n_tokens: u32,
+                                max_query_len: u32, max_seq_len: u32, n_heads: u32, n_kv_heads: u32,
+                                d_head: u32, page_size: u32, n_pages: u32, max_pages: u32, q_row_stride: u32,
+                                scale: f32, causal: u32, workspace: *mut c_void, workspace_bytes: usize,
+                                stream: *mut c_void) -> c_int;
 
     // Status and version.
     pub fn dfattn_status_string(status: c_int) -> *const c_char;

@@ -80,4 +80,12 @@ extern "C" {
                                         stream: *mut c_void) -> c_int;
     pub fn dfgpt2_linear_backward_weight(grad_out: *const f32, x: *const f32, grad_w: *mut f32, rows: u32,
                                          in_features: u32, out_features: u32, stream: *mut c_void) -> c_int;
+    pub fn dfgpt2_token_logprobs(logits: *const c_void, tokens: *const u32, logprob: *mut f32,
+                                 entropy: *mut f32, stats: *mut f32, top_ids: *mut u32, top_logprobs: *mut f32,
+                                 dtype: u32, rows: u32, cols: u32, row_stride: u32, top_k: u32,
+                                 stream: *mut c_void) -> c_int;
+    pub fn dfgpt2_token_logprobs_backward(logits: *const c_void, tokens: *const u32, stats: *const f32,
+                                          entropy: *const f32, grad_logprob: *const f32,
+                                          grad_entropy: *const f32, grad_logits: *mut c_void, dtype: u32,
+                                          rows: u32, cols: u32, row_stride: u32, stream: *mut c_void) -> c_int;
 }
