@@ -87,7 +87,7 @@ def attention(ptrs=None, act=0, kv=2, r=3, n=3, max_q=1, max_len=5000, heads=4, 
     (dict(ptrs={9: ODD}), MIS), (dict(ptrs={1: ctypes.c_void_p(0x10008)}), MIS), (dict(ptrs={6: ODD}), MIS),
     (dict(heads=0), SHAPE), (dict(heads=3), SHAPE), (dict(width=0), SHAPE), (dict(stride=255), SHAPE),
     (dict(heads=65538, hk=2), OVER), (dict(r=65536), OVER), (dict(n=(1 << 30) + 1), OVER), (dict(width=1 << 28), OVER),
-    (dict(ws=ODD, ws_bytes=1 << 30), WORK),
+    (dict(r=60000, n=1 << 30, max_q=1 << 30), OVER), (dict(ws=P, ws_bytes=4), WORK), (dict(ws=ODD, ws_bytes=1 << 30), WORK),
     (dict(r=0), 0), (dict(n=0), 0), (dict(max_q=0), 0),
 ])
 def test_attention(kw, status):
@@ -102,6 +102,7 @@ def test_sizes():
         assert lib.dfattn_kv8_pool_bytes(*bad) == 0
     size = lib.dfattn_kv8_attention_workspace_bytes
     assert size(1, 1, 1, 64, 12, 12, 64) == 0            # one short row: nothing to split
+    assert size(1, 1, 1, 100000, 12, 12, 64) > 0
     assert size(0, 1, 1, 100000, 12, 12, 64) == 0 and size(1, 1, 1, 100000, 12, 5, 64) == 0
     with pytest.raises(ValueError):
         dfattn.kv8_cache(2, 2, 64, 17, device="cpu")
