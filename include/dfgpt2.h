@@ -164,7 +164,7 @@ int dfgpt2_linear_backward_weight(const float *grad_out, const float *x, float *
  * (top_ids, top_logprobs [rows, top_k]; may be NULL when top_k is 0). entropy and stats may be NULL.
  * Values of -infinity are masked out (p = 0); a row of nothing else has m, logprob and top_logprobs
  * -infinity and entropy 0. A NaN or +infinity makes its row's results NaN (the ids stay). A token that
- * is not below cols has logprob 0. Statistics are fp32, in one fixed order of sums. rows <= 2^21.
+ * is not below cols has logprob 0. Statistics are fp32, in one fixed order of sums. rows <= 2^21, cols <= 2^27.
  * backward: grad_logits [rows, cols] (the logits' type, contiguous, overwritten; may be logits itself
  * when that is contiguous) = grad_logprob (1[j = token] - p_j) - grad_entropy p_j (ln p_j + entropy), from
  * the forward's stats and entropy; either gradient may be NULL (0). A masked-out value and a row of
