@@ -17,7 +17,7 @@ namespace {
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr uint32_t kMaxTop = 64;
 constexpr uint32_t kMaxRows = 1u << 21;
-constexpr int kCandidates = 512;
+constexpr int kCandidates = 512, kSlots = 8;
 
 struct LogprobArgs {
   const void *logits;
@@ -82,159 +82,196 @@ __device__ __forceinline__ raw4 load_end(const void *row, int i0, int n) {
   return r;
 }
 
-// The row's groups of this thread: group j holds ids (j * kThreads + thread) *
-// kPer; the last, partial one of the workgroup is apart. Up to G whole ones stay
-// in registers; G = 0: read again by each pass.
-template <bool BF16, int G>
-struct Row {
-  const void *row;
-  int whole, first;
-  raw4 r[G > 0 ? G : 1], end;
-  static constexpr int kStep = kThreads * kPer<BF16>;
-  __device__ __forceinline__ Row(const void *p, int n, int tid) : row(p), whole(n / kStep), first(tid * kPer<BF16>) {
-    if constexpr (G > 0) {
-#pragma unroll
-      for (int j = 0; j < G; ++j)
-        if (j < whole) r[j] = load_group<BF16>(row, j * kStep + first);
-    }
-    end = load_end<BF16>(row, whole * kStep + first, n);
-  }
-  // f(logits of a group, its first id); ids from n on are -infinity.
-  template <typename F>
-  __device__ __forceinline__ void each(F f) {
-    if constexpr (G > 0) {
-#pragma unroll
-      for (int j = 0; j < G; ++j)
-        if (j < whole) {
-          // Not known to be the values of the pass before: the compiler would keep every widened one.
-          asm volatile("" : "+v"(r[j].x), "+v"(r[j].y), "+v"(r[j].z), "+v"(r[j].w));
-          f(r[j], j * kStep + first);
-        }
-    } else {
-#pragma unroll 4
-      for (int j = 0; j < whole; ++j) f(load_group<BF16>(row, j * kStep + first), j * kStep + first);
-    }
-    f(end, whole * kStep + first);
-  }
-};
-
 struct Shared {
-  float lane_max[kWaves][64], sum_s[kWaves], sum_t[kWaves], thr;
+  float lane_max[kWaves][64], sum_s[kWaves], sum_t[kWaves];
+  int above[64];
   unsigned n_cand, wave_equal[kWaves];
   unsigned long long cand[kCandidates], best[kWaves];
 };
 
-// One workgroup per row, in one pass over memory where the row fits the
-// registers: the threads' maxima, the sums of exponentials, then the
-// alternatives. For those, the k-th largest of the 64 lanes' maxima (a lane's
-// over all waves) bounds the k-th largest logit from below, so the few logits
-// at or above it are the candidates; each one's rank among them is its place.
-template <bool BF16, int G>
-__global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
-  constexpr int W = kPer<BF16>;
-  __shared__ Shared sh;
-  const size_t row = blockIdx.x, at = row * a.stride;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.cols, k = a.k;
-  const void *base = static_cast<const char *>(a.logits) + at * (BF16 ? 2 : 4);
-  Row<BF16, G> x(base, n, tid);
-  const uint32_t token = a.tokens[row];
-  const float chosen = token < (uint32_t)n ? load_logit<BF16>(base, token) : 0.f;
-  float mine = -INFINITY;
-  x.each([&](raw4 r, int) {
-#pragma unroll
-    for (int w = 0; w < W; ++w) mine = fmaxf(mine, logit_of<BF16>(r, w));
-  });
+// The next larger number; the smallest one after either zero.
+__device__ __forceinline__ float next_above(float x) {
+  const unsigned u = __float_as_uint(x);
+  return x == 0.f ? __uint_as_float(1u) : __uint_as_float(u & 0x80000000u ? u - 1u : u + 1u);
+}
+
+// S = sum e^(x - m) and T = sum e^(x - m) (x - m) log2 e about a maximum m.
+struct Sums {
+  float m, s, t;
+  // The same about m_new >= m. (2^-1000 is 0: sums about -infinity are 0.)
+  __device__ __forceinline__ void move(float m_new) {
+    const float d = fmaxf((m - (m_new == -INFINITY ? 0.f : m_new)) * kLog2e, -1000.f);
+    const float f = __builtin_amdgcn_exp2f(d);
+    t = f * fmaf(d, s, t);
+    s *= f;
+    m = m_new;
+  }
+};
+
+// The k-th largest of the 64 lanes' maxima (a lane's over all waves): a lower bound
+// of the k-th largest of the values so far. `strict`: eight or more lanes hold it,
+// a mask's value most likely, so that only what is above it makes a candidate.
+__device__ __forceinline__ float lane_bound(Shared &sh, float mine, int k, int lane, int wave, bool &strict) {
   sh.lane_max[wave][lane] = mine;
-  if (tid == 0) sh.n_cand = 0;
+  if (wave == 0) sh.above[lane] = 0;
   __syncthreads();
   float top = sh.lane_max[0][lane];
 #pragma unroll
   for (int v = 1; v < kWaves; ++v) top = fmaxf(top, sh.lane_max[v][lane]);
-  const float m = wave_max(top), m0 = m == -INFINITY ? 0.f : m;
-  if (k > 0 && wave == kWaves - 1) {
-    int above = 0;
+  int above = 0;
 #pragma unroll
-    for (int j = 0; j < 64; ++j) {
-      const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(top), j));
-      above += o > top || (o == top && j < lane);
-    }
-    if (above == k - 1) sh.thr = top;
+  for (int j = 0; j < 64 / kWaves; ++j) {
+    const int o_lane = wave * (64 / kWaves) + j;
+    const float o = __shfl(top, o_lane, 64);
+    above += o > top || (o == top && o_lane < lane);
   }
-  // S = sum e^(x - m) and T = sum e^(x - m) (x - m) log2 e. A masked-out logit
-  // adds 0 to T (0 times at least -200), a NaN makes both NaN.
-  float s = 0.f, t = 0.f;
-  x.each([&](raw4 r, int) {
+  atomicAdd(&sh.above[lane], above);
+  __syncthreads();
+  const int who = __ffsll(__ballot(sh.above[lane] == k - 1)) - 1;
+  const float thr = __shfl(top, who, 64);
+  strict = __popcll(__ballot(top == thr)) >= 8;
+  return thr;
+}
+
+// One workgroup per row, one pass over memory: kBatch groups a thread at a time,
+// the next ones on their way meanwhile; exponentials about the thread's maximum so
+// far. The alternatives: each thread's maxima by slots of batches wait in LDS until
+// lane_bound gives a bound that at least k logits reach. The few slots that reach it
+// (some 30 of 512 threads hold one) are read again for the candidates, and each
+// candidate's rank among them is its place.
+template <bool BF16, bool TOP>
+__global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
+  constexpr int W = kPer<BF16>, kBatch = BF16 ? 2 : 4, kStep = kThreads * W;
+  __shared__ Shared sh;
+  __shared__ float slot_max[TOP ? kSlots : 1][kThreads];
+  const size_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = a.cols, k = a.k;
+  const void *base = static_cast<const char *>(a.logits) + row * a.stride * (BF16 ? 2 : 4);
+  const uint32_t token = a.tokens[row];
+  const float chosen = token < (uint32_t)n ? load_logit<BF16>(base, token) : 0.f;
+  // Group j of a thread: ids (j * kThreads + tid) * W ..; `whole` of them are whole in the workgroup.
+  const int whole = n / kStep, first = tid * W;
+  const raw4 end = load_end<BF16>(base, whole * kStep + first, n);
+  const unsigned fill = BF16 ? 0xff80ff80u : 0xff800000u;
+  auto load = [&](int j) {
+    if (j < whole) return load_group<BF16>(base, j * kStep + first);
+    return j == whole ? end : raw4{fill, fill, fill, fill};
+  };
+  const int per_slot = ((whole + kBatch) / kBatch + kSlots - 1) / kSlots;  // batches
+  Sums x = {-INFINITY, 0.f, 0.f};
+  auto batch = [&](const raw4 *r) {
+    float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float y = (logit_of<BF16>(r, w) - m0) * kLog2e, e = __builtin_amdgcn_exp2f(y);
-      s += e;
-      t = fmaf(e, fmaxf(y, -200.f), t);
+    for (int q = 0; q < kBatch; ++q)
+#pragma unroll
+      for (int w = 0; w < W; ++w) top = fmaxf(top, logit_of<BF16>(r[q], w));
+    if (top > x.m) x.move(top);
+    const float m0 = x.m == -INFINITY ? 0.f : x.m;
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        // A masked-out logit adds 0 to T (0 times at least -200), a NaN makes both NaN.
+        const float y = (logit_of<BF16>(r[q], w) - m0) * kLog2e, e = __builtin_amdgcn_exp2f(y);
+        x.s += e;
+        x.t = fmaf(e, fmaxf(y, -200.f), x.t);
+      }
+    return top;
+  };
+  if (TOP && tid == 0) sh.n_cand = 0;
+  raw4 cur[kBatch], next[kBatch];
+#pragma unroll
+  for (int q = 0; q < kBatch; ++q) cur[q] = load(q);
+  int slot = 0, left = per_slot;
+  float slot_top = -INFINITY;
+  for (int j0 = 0; j0 <= whole; j0 += kBatch) {
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) next[q] = load(j0 + kBatch + q);
+    const float top = batch(cur);
+    if constexpr (TOP) {
+      slot_top = fmaxf(slot_top, top);
+      slot_max[slot][tid] = slot_top;
+      if (--left == 0) {
+        ++slot;
+        left = per_slot;
+        slot_top = -INFINITY;
+      }
     }
-  });
-  s = wave_sum(s);
-  t = wave_sum(t);
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) cur[q] = next[q];
+  }
+  const int slots = slot + (left < per_slot);
+  const float mine = x.m;
+  const float wave_top = wave_max(mine);
+  x.move(wave_top);
+  x.s = wave_sum(x.s);
+  x.t = wave_sum(x.t);
   if (lane == 0) {
-    sh.sum_s[wave] = s;
-    sh.sum_t[wave] = t;
+    sh.lane_max[0][wave] = wave_top;
+    sh.sum_s[wave] = x.s;
+    sh.sum_t[wave] = x.t;
   }
   __syncthreads();
-  s = sh.sum_s[0];
-  t = sh.sum_t[0];
+  float m = sh.lane_max[0][0];
 #pragma unroll
-  for (int v = 1; v < kWaves; ++v) {
-    s += sh.sum_s[v];
-    t += sh.sum_t[v];
+  for (int v = 1; v < kWaves; ++v) m = fmaxf(m, sh.lane_max[0][v]);
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int v = 0; v < kWaves; ++v) {
+    Sums y = {sh.lane_max[0][v], sh.sum_s[v], sh.sum_t[v]};
+    y.move(m);
+    s += y.s;
+    t += y.t;
   }
-  const bool nan = s != s;
-  const float ln_s = m == -INFINITY && !nan ? 0.f : logf(s);
+  const bool nan = s != s, none = m == -INFINITY && !nan;
+  const float m0 = none ? 0.f : m, ln_s = none ? 0.f : logf(s);
   auto logp = [&](float v) { return v == -INFINITY && !nan ? v : (v - m0) - ln_s; };
   if (tid == 0) {
     a.logprob[row] = token < (uint32_t)n ? logp(chosen) : 0.f;
-    if (a.entropy) a.entropy[row] = m == -INFINITY && !nan ? 0.f : ln_s - t * kLn2 / s;
+    if (a.entropy) a.entropy[row] = none ? 0.f : ln_s - t * kLn2 / s;
     if (a.stats) {
       a.stats[2 * row] = nan ? ln_s : m;
       a.stats[2 * row + 1] = ln_s;
     }
   }
-  if (k == 0) return;
+  if constexpr (!TOP) return;
 
-  const float thr = sh.thr;
   auto put = [&](unsigned long long key, int place) {
     a.top_ids[row * k + place] = 0xffffffffu - (uint32_t)key;
     a.top_logprobs[row * k + place] = logp(logit_of_rank((unsigned)(key >> 32)));
   };
-  // The candidates: what is at or above the bound, where there is room for it all; else
-  // what is above it. A group of a thread's is looked through where its largest is.
-  auto collect = [&](bool equal_too) {
-    x.each([&](raw4 r, int i0) {
-      float g = logit_of<BF16>(r, 0);
-#pragma unroll
-      for (int w = 1; w < W; ++w) g = fmaxf(g, logit_of<BF16>(r, w));
-      if (g >= thr) {
+  float thr = INFINITY;
+  bool strict = false;
+  unsigned c = kCandidates + 1;
+  for (int pass = 0; pass < 2 && c > kCandidates && !nan; ++pass) {
+    __syncthreads();
+    if (pass == 0)
+      thr = lane_bound(sh, mine, k, lane, wave, strict);
+    else  // too many equal the bound
+      strict = true;
+    if (pass > 0 && tid == 0) sh.n_cand = 0;
+    if (pass > 0) __syncthreads();
+    const float least = strict ? next_above(thr) : thr;
+    unsigned todo = 0;
+    if (mine >= least)
+      for (int i = 0; i < slots; ++i) todo |= slot_max[i][tid] >= least ? 1u << i : 0u;
+    for (; todo; todo &= todo - 1) {
+      const int j1 = (__ffs(todo) - 1) * per_slot * kBatch, j2 = min(j1 + per_slot * kBatch, whole + 1);
+#pragma unroll kBatch
+      for (int j = j1; j < j2; ++j) {
+        const raw4 r = j < whole ? load_group<BF16>(base, j * kStep + first) : end;
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           const float v = logit_of<BF16>(r, w);
-          if ((v > thr || (equal_too && v == thr)) && i0 + w < n) {
-            const unsigned c = atomicAdd(&sh.n_cand, 1u);
-            if (c < kCandidates) sh.cand[c] = key_of(v, i0 + w);
+          if (v >= least && j * kStep + first + w < n) {
+            const unsigned at = atomicAdd(&sh.n_cand, 1u);
+            if (at < kCandidates) sh.cand[at] = key_of(v, j * kStep + first + w);
           }
         }
       }
-    });
-    __syncthreads();
-    return sh.n_cand;
-  };
-  unsigned c = kCandidates + 1;
-  bool all = true;
-  if (!nan) {
-    c = collect(true);
-    if (c > kCandidates) {
-      all = false;
-      __syncthreads();
-      if (tid == 0) sh.n_cand = 0;
-      __syncthreads();
-      c = collect(false);
     }
+    __syncthreads();
+    c = sh.n_cand;
   }
   if (c <= kCandidates) {
     // Four lanes a candidate, each against a quarter of them.
@@ -246,8 +283,8 @@ __global__ __launch_bounds__(kThreads) void logprob_kernel(LogprobArgs a) {
       place += __shfl_xor(place, 2, 64);
       if ((tid & 3) == 0 && i < c && place < k) put(key, place);
     }
-    if (all || (int)c >= k) return;
-    // The rest equals the bound (a mask's value, say): the lowest ids of those.
+    if (!strict || (int)c >= k) return;
+    // The rest equals the bound: the lowest ids of those.
     int found = (int)c;
     for (int i0 = 0; i0 < n && found < k; i0 += kThreads) {
       const int i = i0 + tid;
@@ -357,20 +394,12 @@ __global__ __launch_bounds__(256) void logprob_grad_kernel(GradArgs a) {
   }
 }
 
-// Rows of up to 1, 6, 12 and 24 whole groups a thread (and the partial one) stay in registers.
 template <bool BF16>
 void launch_logprobs(const LogprobArgs &a, uint32_t rows, hipStream_t s) {
-  const int groups = a.cols / (kThreads * kPer<BF16>);
-  if (groups <= 1)
-    hipLaunchKernelGGL((logprob_kernel<BF16, 1>), dim3(rows), dim3(kThreads), 0, s, a);
-  else if (groups <= 6)
-    hipLaunchKernelGGL((logprob_kernel<BF16, 6>), dim3(rows), dim3(kThreads), 0, s, a);
-  else if (groups <= 12)
-    hipLaunchKernelGGL((logprob_kernel<BF16, 12>), dim3(rows), dim3(kThreads), 0, s, a);
-  else if (groups <= 24)
-    hipLaunchKernelGGL((logprob_kernel<BF16, 24>), dim3(rows), dim3(kThreads), 0, s, a);
+  if (a.k > 0)
+    hipLaunchKernelGGL((logprob_kernel<BF16, true>), dim3(rows), dim3(kThreads), 0, s, a);
   else
-    hipLaunchKernelGGL((logprob_kernel<BF16, 0>), dim3(rows), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((logprob_kernel<BF16, false>), dim3(rows), dim3(kThreads), 0, s, a);
 }
 
 int check(const char *fn, uint32_t dtype, uint32_t rows, uint32_t cols, uint32_t row_stride) {
