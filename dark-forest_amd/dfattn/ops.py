@@ -241,21 +241,29 @@ def embedding_backward(ids, grad_out, grad_table):
 
 
 def _logit_rows(t):
-    """(pointer, row stride, type code) of float32 or bfloat16 logits [rows, V] with contiguous rows."""
+    """(rows, V, pointer, row stride, type code) of float32 or bfloat16 logits [rows, V] with contiguous rows, on
+    the current device."""
     torch = _torch()
-    if not t.is_cuda or t.dtype not in (torch.float32, torch.bfloat16):
+    dtype = t.dtype
+    if not t.is_cuda or (dtype is not torch.float32 and dtype is not torch.bfloat16):
         raise ValueError("logits must be a float32 or bfloat16 device tensor")
-    rows, v = _rows_cols(t)
-    stride = t.stride(0) if rows > 1 else v
-    if (t.stride(1) != 1 and v > 1) or stride < v:
-        raise ValueError("logits must be [rows, V] with contiguous rows")
-    return t.data_ptr(), stride, 0 if t.dtype == torch.float32 else 1
-
-
-def _same_device(t, *others):
-    torch = _torch()
-    if t.device.index != torch._C._cuda_getDevice() or any(o is not None and o.device != t.device for o in others):
+    if t.get_device() != torch._C._cuda_getDevice():
         raise ValueError("the tensors must be on the current device")
+    rows, v = _rows_cols(t)
+    stride = v
+    if not t.is_contiguous():
+        if rows > 1:
+            stride = t.stride(0)
+        if (t.stride(1) != 1 and v > 1) or stride < v:
+            raise ValueError("logits must be [rows, V] with contiguous rows")
+    return rows, v, t.data_ptr(), stride, 0 if dtype is torch.float32 else 1
+
+
+def _beside(t, *others):
+    dev = t.get_device()
+    for o in others:
+        if o is not None and (not o.is_cuda or o.get_device() != dev):
+            raise ValueError("the tensors must be on the current device")
 
 
 def token_logprobs_forward(logits, tokens, top_k=0):
@@ -263,16 +271,16 @@ def token_logprobs_forward(logits, tokens, top_k=0):
     tensor) and int32 tokens [rows]. Returns (logprob [rows], entropy [rows], stats [rows, 2], top_ids [rows, top_k] int32,
     top_logprobs [rows, top_k]); stats holds each row's maximum and ln sum exp(x - maximum)."""
     torch = _torch()
-    rows, v = _rows_cols(logits)
-    p, stride, dtype = _logit_rows(logits)
-    _same_device(logits, tokens)
+    rows, v, p, stride, dtype = _logit_rows(logits)
+    _beside(logits, tokens)
     if tokens.shape != (rows,):
         raise ValueError("tokens must be [rows]")
-    dev = logits.device
-    logprob, entropy = (torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(2))
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
-    top = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    empty, f32, dev = torch.empty, torch.float32, logits.device
+    logprob = empty((rows,), dtype=f32, device=dev)
+    entropy = empty((rows,), dtype=f32, device=dev)
+    stats = empty((rows, 2), dtype=f32, device=dev)
+    ids = empty((rows, top_k), dtype=torch.int32, device=dev)
+    top = empty((rows, top_k), dtype=f32, device=dev)
     _check(ops_lib().dfgpt2_token_logprobs(p, _ids_ptr(tokens), logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
                                            ids.data_ptr(), top.data_ptr(), dtype, rows, v, stride, top_k,
                                            _stream_ptr()))
@@ -282,11 +290,10 @@ def token_logprobs_forward(logits, tokens, top_k=0):
 def token_logprobs_backward(logits, tokens, stats, entropy, grad_logprob=None, grad_entropy=None, out=None):
     """dfgpt2_token_logprobs_backward: the gradient of the logits [rows, V] in their type, from the forward's stats
     and entropy; a gradient that is None is 0. out may be the logits themselves where they are contiguous."""
-    torch = _torch()
-    rows, v = _rows_cols(logits)
-    p, stride, dtype = _logit_rows(logits)
-    _same_device(logits, tokens, stats, entropy, grad_logprob, grad_entropy, out)
-    out = torch.empty((rows, v), dtype=logits.dtype, device=logits.device) if out is None else out
+    rows, v, p, stride, dtype = _logit_rows(logits)
+    _beside(logits, tokens, stats, entropy, grad_logprob, grad_entropy, out)
+    if out is None:
+        out = _torch().empty((rows, v), dtype=logits.dtype, device=logits.device)
     if out.shape != (rows, v) or out.dtype != logits.dtype or not out.is_contiguous():
         raise ValueError("out must be a contiguous tensor like the logits")
     if any(t is not None and t.shape != (rows,) for t in (tokens, entropy, grad_logprob, grad_entropy)) or \
