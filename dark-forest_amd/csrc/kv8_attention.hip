@@ -6,6 +6,13 @@
 // the positions t it sees, k_t and v_t codes times the scale of their page and
 // head.
 #include "kv8.h"
+#ifndef KV8_MINSTEPS
+#define KV8_MINSTEPS 2
+#define KV8_SHAREFROM 1024
+#endif
+#ifndef KV8_OCC
+#define KV8_OCC (QT == 1 ? (NC == 1 ? 4 : 3) : 2)
+#endif
 
 #include <algorithm>
 
@@ -21,8 +28,11 @@ struct AttnArgs {
   const uint32_t *table, *query_start, *seq_lens;
   void *out;
   float *lse;
-  float *part_o, *part_ml;  // n_splits > 1: normalised outputs, and (m, l), of each (row, head, split)
-  uint32_t n_tokens, max_q, max_pages, n_pages, q_tiles, n_splits, chunk, total;
+  // Shared out (see Share): normalised outputs [parts * Hk][2][cols][D] and (m, l) [parts * Hk][2][cols][2]
+  // of the pieces, and the steps before each (request, tile) [R * q_tiles + 1].
+  float *part_o, *part_ml;
+  uint32_t *before;
+  uint32_t R, n_tokens, max_q, max_pages, n_pages, q_tiles, parts, cols;
   int H, Hk, D, P;
   size_t q_stride;
   float scale;
@@ -73,35 +83,58 @@ __device__ __forceinline__ f32x4 mfma(half8_t a, half8_t b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+constexpr int kWaves = 4, kStep = 64 * kWaves;  // keys of a workgroup's step
+
 // The rows a workgroup works on: request r, kv head hk, and the columns (query
-// token, head of the group) col0 .. col0+16*QT-1 of its nq * G.
+// token, head of the group) col0 .. of its nq * G.
 struct Where {
-  uint32_t r, split, tile;
-  int hk, nq, n_cols, active;
-  uint32_t q0;       // first token of the request
-  long long first;   // position of its first query
-  int length, k_end; // cached positions; those the last column sees
+  uint32_t r, tile, q0;  // q0: first token of the request
+  int hk, n_cols, col0;
+  int length, k_end, first;  // cached positions, those the last column sees, that of the first query
+  // The positions that query j sees.
+  __device__ __forceinline__ int end_of(const AttnArgs &a, int j) const {
+    return a.causal ? min(length, max(first + j + 1, 0)) : length;
+  }
 };
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+// UNIFORM: r and tile are the same in all lanes, and so is what is read for them.
+template <bool UNIFORM>
 __device__ __forceinline__ bool find_rows(const AttnArgs &a, Where &w, int cols_per_tile) {
   const int G = a.H / a.Hk;
-  const uint32_t q0 = min(a.query_start[w.r], a.n_tokens), q1 = min(a.query_start[w.r + 1], a.n_tokens);
-  const int nq = q1 > q0 ? (int)(q1 - q0) : 0;
+  uint32_t q0 = min(a.query_start[w.r], a.n_tokens), q1 = min(a.query_start[w.r + 1], a.n_tokens);
+  uint32_t L = min(a.seq_lens[w.r], a.max_pages * (uint32_t)a.P);
+  if constexpr (UNIFORM) {
+    q0 = uniform(q0);
+    q1 = uniform(q1);
+    L = uniform(L);
+  }
+  const uint32_t nq = q1 > q0 ? q1 - q0 : 0;
   w.q0 = q0;
-  w.nq = min((uint32_t)nq, a.max_q);
-  w.n_cols = w.nq * G;
-  const int col0 = (int)w.tile * cols_per_tile;
-  if (col0 >= w.n_cols) return false;
-  const uint32_t L = a.seq_lens[w.r];
-  w.length = (int)min((unsigned long long)L, (unsigned long long)a.max_pages * a.P);
-  w.first = (long long)L - nq;
-  const int last = (min(w.n_cols, col0 + cols_per_tile) - 1) / G;
-  w.k_end = a.causal ? (int)min((long long)w.length, max(w.first + last + 1, 0ll)) : w.length;
-  w.active = max(1, (int)min((long long)a.n_splits, ((long long)w.k_end + a.chunk - 1) / a.chunk));
-  return true;
+  w.n_cols = (int)min(nq, a.max_q) * G;
+  w.col0 = (int)w.tile * cols_per_tile;
+  w.length = (int)L;
+  w.first = (int)L - (int)nq;
+  const int last = (min(w.n_cols, w.col0 + cols_per_tile) - 1) / G;
+  w.k_end = w.end_of(a, last);
+  return w.col0 < w.n_cols;
 }
 
-constexpr int kWaves = 4;
-
+// How the work of a call is shared out: the steps (kStep keys of one tile) of one kv
+// head, request by request and tile by tile (a tile that sees nothing has one
+// step, which writes its zeros), are cut into equal parts of `per`, one to a
+// workgroup, and alike for each head. So every workgroup has the same work whatever
+// the lengths are, and the heads of a page, which lie together, are read at the
+// same time (by parts of one head after the other the call of 2 x 131072 keys took
+// 79 us, so 65). A tile cut between workgroups is merged by
+// attention_reduce_kernel; a workgroup has at most two such pieces, the tile that
+// its part begins in (slot 0) and the one that goes on behind it (slot 1).
+constexpr uint32_t kMinSteps = KV8_MINSTEPS;
+struct Share {
+  uint32_t total, per;
+  // before: the steps before each (request, tile)
+  __device__ __forceinline__ Share(const uint32_t *before, const AttnArgs &a)
+      : total(uniform(before[a.R * a.q_tiles])), per(max((total + a.parts - 1) / a.parts, kMinSteps)) {}
+};
 // One workgroup: 16*QT columns (queries of one kv head) against the keys of one
 // split, 64 keys a wave and step, the waves' results merged at the end.
 //
@@ -118,40 +151,102 @@ constexpr int kWaves = 4;
 // r), where 2^r (r whole) bounds the largest such product so far: m and r move
 // together, so weights keep 2^-39 of the largest one whatever the pages'
 // scales.
-template <bool E4M3, int NT, int NC, int QT>
-__global__ __launch_bounds__(64 * kWaves, QT == 1 ? 2 : 1) void attention_kernel(AttnArgs a) {
+template <bool E4M3, int NT, int NC, int QT, bool SHARED>
+__global__ __launch_bounds__(64 * kWaves, KV8_OCC) void attention_kernel(AttnArgs a) {
   constexpr bool BF16 = NT == 1;
   constexpr int NV = 4 * NC;
   constexpr int kCols = 16 * QT;
+  extern __shared__ uint32_t before[];  // SHARED: R * q_tiles + 1
   __shared__ float m_lds[kWaves][kCols], l_lds[kWaves][kCols];
   __shared__ __attribute__((aligned(16))) float o_lds[kWaves][kCols][20];
-  uint32_t id = linear_block();
-  if (id >= a.total) return;
-  Where w;
-  w.split = id % a.n_splits;
-  id /= a.n_splits;
-  w.hk = (int)(id % (uint32_t)a.Hk);
-  id /= (uint32_t)a.Hk;
-  w.tile = id % a.q_tiles;
-  w.r = id / a.q_tiles;
-  if (!find_rows(a, w, kCols)) return;
-  if ((int)w.split >= w.active) return;
+  __shared__ uint32_t wave_steps[kWaves];
+  __shared__ half8_t q_lds[QT][NC][2][NT][64];
+  __shared__ float scale_lds[kCols];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m16 = lane & 15, g = lane >> 4;
-  const int G = a.H / a.Hk, D = a.D, Dp = padded(D), P = a.P, col0 = (int)w.tile * kCols;
-  const int k0 = (int)w.split * (int)a.chunk;
-  const int k1 = (int)w.split + 1 == w.active ? w.k_end : k0 + (int)a.chunk;
+  const int G = a.H / a.Hk, D = a.D, Dp = padded(D), P = a.P;
+  uint32_t at = 0, end = 0, pair = 0;  // this workgroup's steps, and the (request, tile) they are at
+  Where w;
+  if constexpr (SHARED) {
+    const uint32_t n = a.R * a.q_tiles, each = (n + 64 * kWaves - 1) / (64 * kWaves);
+    const uint32_t i0 = min(n, tid * each), i1 = min(n, i0 + each);
+    auto steps_of = [&](uint32_t i) {
+      Where v;
+      v.r = i / a.q_tiles;
+      v.tile = i % a.q_tiles;
+      return find_rows<false>(a, v, kCols) ? max(1u, (uint32_t)(v.k_end + kStep - 1) / kStep) : 0u;
+    };
+    uint32_t mine = 0;
+    for (uint32_t i = i0; i < i1; ++i) {
+      const uint32_t x = steps_of(i);
+      before[i] = mine;
+      mine += x;
+    }
+    uint32_t sum = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const uint32_t o = __shfl_up(sum, off, 64);
+      if (lane >= off) sum += o;
+    }
+    if (lane == 63) wave_steps[wave] = sum;
+    __syncthreads();
+    uint32_t base = sum - mine;
+    for (int v = 0; v < wave; ++v) base += wave_steps[v];
+    for (uint32_t i = i0; i < i1; ++i) before[i] += base;
+    if (tid == 64 * kWaves - 1) before[n] = base + mine;
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (uint32_t i = tid; i <= n; i += 64 * kWaves) a.before[i] = before[i];
+    const Share sh(before, a);
+    const uint32_t part = blockIdx.x / (uint32_t)a.Hk;
+    w.hk = (int)(blockIdx.x % (uint32_t)a.Hk);
+    at = part * sh.per;
+    end = min(at + sh.per, sh.total);
+    if (at >= end) return;
+    pair = 0;  // the last (request, tile) with before[pair] <= at
+    for (uint32_t hi = n; hi - pair > 1;) {
+      const uint32_t mid = (pair + hi) / 2;
+      if (uniform(before[mid]) <= at)
+        pair = mid;
+      else
+        hi = mid;
+    }
+  } else {
+    uint32_t id = linear_block();
+    w.tile = id % a.q_tiles;
+    id /= a.q_tiles;
+    w.hk = (int)(id % (uint32_t)a.Hk);
+    w.r = id / (uint32_t)a.Hk;
+    if (w.r >= a.R || !find_rows<true>(a, w, kCols)) return;
+  }
+  bool begins = true;  // the first of this workgroup's tiles
+  while (true) {
+  int k0 = 0, k1;
+  bool direct = true;
+  if constexpr (SHARED) {
+    w.r = pair / a.q_tiles;
+    w.tile = pair % a.q_tiles;
+    find_rows<true>(a, w, kCols);
+    const uint32_t s0 = uniform(before[pair]), n = uniform(before[pair + 1]) - s0, s1 = min(s0 + n, end);
+    k0 = (int)(at - s0) * kStep;
+    k1 = min(w.k_end, (int)(s1 - s0) * kStep);
+    direct = at == s0 && s1 == s0 + n;
+    at = s1;
+  } else {
+    k1 = w.k_end;
+  }
+  const int col0 = w.col0;
   const uint32_t *table = a.table + (size_t)w.r * a.max_pages;
-  const size_t head_bytes = (size_t)P * Dp;
 
-  // Q, and where each column's keys end.
-  half8_t q[QT][NC][2][NT];
-  float col_scale[QT];
+  // Q as the products take it, in LDS for all waves (16 columns converted by one of
+  // them each), and where each column's keys end.
   int k_end[QT];
+  const int min_end = w.end_of(a, col0 / G);  // of the workgroup's columns: the first one's
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     const int c = min(col0 + 16 * t + m16, w.n_cols - 1), j = c / G;
+    k_end[t] = w.end_of(a, j);
+    if (t % kWaves != wave) continue;
     const size_t row = (size_t)(w.q0 + j) * a.q_stride + (size_t)(w.hk * G + c % G) * D;
-    k_end[t] = a.causal ? (int)min((long long)w.length, max(w.first + j + 1, 0ll)) : w.length;
     float x[NC][16];
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
@@ -186,21 +281,27 @@ __global__ __launch_bounds__(64 * kWaves, QT == 1 ? 2 : 1) void attention_kernel
       for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[n][i]));
     top = column_max(top);
     const int e = top > 0.f && top <= 3.4028234e38f ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
-    col_scale[t] = __builtin_amdgcn_ldexpf(a.scale * kLog2e, -e);
+    // (A negative scale's sign goes into q.)
+    if (g == 0) scale_lds[16 * t + m16] = __builtin_amdgcn_ldexpf(fabsf(a.scale) * kLog2e, -e);
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < 2; ++h) {
+        half8_t q[2];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float y = __builtin_amdgcn_ldexpf(x[n][8 * h + i], e);
-          const half_t hi = (half_t)y;
-          q[t][n][h][0][i] = hi;
-          if constexpr (NT == 2) q[t][n][h][1][i] = (half_t)(y - (float)hi);
+          const float y = __builtin_amdgcn_ldexpf(a.scale < 0.f ? -x[n][8 * h + i] : x[n][8 * h + i], e);
+          q[0][i] = (half_t)y;
+          q[1][i] = (half_t)(y - (float)q[0][i]);
         }
+#pragma unroll
+        for (int e2 = 0; e2 < NT; ++e2) q_lds[t][n][h][e2][lane] = q[e2];
+      }
   }
-  int min_end = k_end[0];  // of the workgroup's columns: the first one's
-  min_end = __builtin_amdgcn_readfirstlane(min_end);
+  __syncthreads();
+  float col_scale[QT];
+#pragma unroll
+  for (int t = 0; t < QT; ++t) col_scale[t] = scale_lds[16 * t + m16];
 
   float m[QT], l[QT], r[QT];
   f32x4 o[QT][NV];
@@ -213,91 +314,127 @@ __global__ __launch_bounds__(64 * kWaves, QT == 1 ? 2 : 1) void attention_kernel
     for (int n = 0; n < NV; ++n) o[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  struct Pages {
-    uint32_t k, v;
+  // The pages that this lane reads in a step: that of the K rows (group m16 / 4 of
+  // the step's four groups of 16 keys), and that of the V columns and of the scores
+  // it gets (group g). `at` counts groups of 16 keys, split into a page's index and
+  // the place within; a step moves all by 4 * kWaves groups.
+  struct Place {
+    uint32_t index, off, page;
   };
-  struct Tile {
-    u32x4 k[NC][4], v[NV];
+  struct KTile {
+    u32x4 c[NC][4];
+  };
+  struct VTile {
+    u32x4 c[NV];
     float ks, vs;
     bool ok;
   };
-  // The pages of the step at keys t0: of the K rows this lane reads, and of the
-  // V columns (and of the scores it gets). Steps past the end read its last page.
-  auto load_pages = [&](int t0) {
-    const int last = k1 - 1;
-    return Pages{table[(unsigned)min(t0 + 16 * (m16 >> 2), last) / (unsigned)P],
-                 table[(unsigned)min(t0 + 16 * g, last) / (unsigned)P]};
+  const uint32_t p16 = (uint32_t)P >> 4, move_i = 4 * kWaves / p16, move_o = 4 * kWaves % p16;
+  const uint32_t last_index = k1 > 0 ? (uint32_t)(k1 - 1) / (uint32_t)P : 0;
+  auto place_of = [&](int t0, int group) {
+    const uint32_t at = ((uint32_t)t0 >> 4) + group;
+    return Place{at / p16, at % p16, 0u};
   };
-  auto load_tile = [&](Tile &x, Pages p, int t0) {
-    const bool ok_k = p.k < a.n_pages, ok_v = p.v < a.n_pages;
-    x.ok = ok_v;
-    const size_t hk_at = (size_t)(ok_k ? p.k : 0u) * a.Hk + w.hk, hv_at = (size_t)(ok_v ? p.v : 0u) * a.Hk + w.hk;
-    x.ks = a.k_scales[hv_at];
-    x.vs = a.v_scales[hv_at];
-    const int kr = (int)((unsigned)(t0 + 16 * (m16 >> 2)) % (unsigned)P) + (m16 & 3);
-    const unsigned char *kp = a.k + hk_at * head_bytes + (size_t)kr * Dp + 16 * g;
+  // (Steps past the end look up its last page.)
+  auto look_up = [&](Place &p) { p.page = table[min(p.index, last_index)]; };
+  auto advance = [&](Place &p) {
+    p.index += move_i;
+    p.off += move_o;
+    if (p.off >= p16) {
+      p.off -= p16;
+      ++p.index;
+    }
+  };
+  const uint32_t page_bytes = (uint32_t)a.Hk * (uint32_t)(P * Dp);
+  // Lanes past a row's last 16 bytes read those again: Q is 0 there.
+  const unsigned char *k_lane = a.k + (size_t)w.hk * (P * Dp) + (m16 & 3) * Dp;
+  const unsigned char *v_lane = a.v + (size_t)w.hk * (P * Dp) + (size_t)m16 * P;
+  int k_col[NC];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) k_col[n] = min(64 * n + 16 * g, Dp - 16);
+  auto load_k = [&](KTile &x, const Place &p) {
+    const uint32_t page = p.page < a.n_pages ? p.page : 0u;
+    const unsigned char *kp = k_lane + ((uint64_t)page * page_bytes + __umul24(16 * p.off, Dp));
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        x.k[n][t] = 64 * n + 16 * g < Dp ? *reinterpret_cast<const u32x4 *>(kp + 64 * n + 4 * t * Dp) : u32x4{0, 0, 0, 0};
-    const unsigned char *vp = a.v + hv_at * head_bytes + (size_t)m16 * P + (unsigned)(t0 + 16 * g) % (unsigned)P;
+      for (int t = 0; t < 4; ++t) x.c[n][t] = *reinterpret_cast<const u32x4 *>(kp + (k_col[n] + 4 * t * Dp));
+  };
+  auto load_v = [&](VTile &x, const Place &p) {
+    x.ok = p.page < a.n_pages;
+    const uint32_t page = x.ok ? p.page : 0u;
+    const size_t head = (size_t)page * (uint32_t)a.Hk + w.hk;
+    x.ks = a.k_scales[head];
+    x.vs = a.v_scales[head];
+    const unsigned char *vp = v_lane + ((uint64_t)page * page_bytes + 16 * p.off);
 #pragma unroll
     for (int n = 0; n < NV; ++n)
-      x.v[n] = 16 * n < Dp ? *reinterpret_cast<const u32x4 *>(vp + (size_t)16 * n * P) : u32x4{0, 0, 0, 0};
+      if (16 * n < Dp) x.c[n] = *reinterpret_cast<const u32x4 *>(vp + 16 * n * P);
   };
-  auto compute = [&](const Tile &x, int t0) {
+  auto compute = [&](const KTile &kt, const VTile &vt, int t0) {
+    // (Q is read from LDS in every step: kept in registers it would cost a wave per SIMD.)
+    asm volatile("" ::: "memory");
     f32x4 s[QT][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int t = 0; t < QT; ++t) s[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int n = 0; n < NC; ++n)
+    for (int n = 0; n < NC; ++n)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const half8_t kh = widen8<E4M3>(x.k[n][j][2 * h], x.k[n][j][2 * h + 1]);
+      for (int h = 0; h < 2; ++h) {
+        half8_t q[QT][NT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int e = 0; e < NT; ++e) q[t][e] = q_lds[t][n][h][e][lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const half8_t kh = widen8<E4M3>(kt.c[n][j][2 * h], kt.c[n][j][2 * h + 1]);
 #pragma unroll
           for (int t = 0; t < QT; ++t)
 #pragma unroll
-            for (int e = 0; e < NT; ++e) s[t][j] = mfma(kh, q[t][n][h][e], s[t][j]);
+            for (int e = 0; e < NT; ++e) s[t][j] = mfma(kh, q[t][e], s[t][j]);
         }
-    }
-    // Whether every column sees all 64 keys.
-    const bool whole = t0 + 64 <= min(k1, min_end) && __all(x.ok);
+      }
+    // Whether every column sees all 64 keys. If not, what it does not see is -infinity here
+    // and a probability of 0 below, whatever the page's scales are.
+    const bool whole = t0 + 64 <= min(k1, min_end) && __all(vt.ok);
     half8_t p[QT][2][NT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      const float f = x.ks * col_scale[t];
-      float y[16], top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) y[i] = s[t][i >> 2][i & 3] * f;
+      const float f = vt.ks * col_scale[t];  // >= 0, or NaN
+      const int n = whole ? 16 : vt.ok ? min(k1, k_end[t]) - (t0 + 16 * g) : 0;  // of this lane's 16 keys
       if (!whole) {
-        const int n = x.ok ? min(k1, k_end[t]) - (t0 + 16 * g) : 0;  // of this lane's 16 keys
 #pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = i < n ? y[i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[t][i >> 2][i & 3] = i < n ? s[t][i >> 2][i & 3] : -INFINITY;
       }
+      float top = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, y[i]);
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i >> 2][i & 3]);
+      top = n > 0 ? top * f : -INFINITY;
       const float m_new = fmaxf(m[t], column_max(top));
       const float base = m_new == -INFINITY ? 0.f : m_new;
       const float dm = m[t] - base;  // <= 0, -inf at first
-      const float reach = column_max(top - base + __builtin_amdgcn_logf(x.vs));
+      const float reach = column_max(top - base + __builtin_amdgcn_logf(vt.vs));
       const float r_new = fmaxf(fmaxf(r[t] + __builtin_ceilf(fmaxf(dm, -1000.f)), __builtin_ceilf(reach)), -300.f);
       if (__any(m_new != m[t] || r_new != r[t])) {
         const float al = __builtin_amdgcn_exp2f(dm), ao = __builtin_amdgcn_ldexpf(al, (int)(r[t] - r_new));
         l[t] *= al;
 #pragma unroll
-        for (int n = 0; n < NV; ++n) o[t][n] *= ao;
+        for (int n2 = 0; n2 < NV; ++n2) o[t][n2] *= ao;
         m[t] = m_new;
         r[t] = r_new;
       }
-      const float pv = __builtin_amdgcn_ldexpf(x.vs, 14 - (int)r_new);
+      const float pv = __builtin_amdgcn_ldexpf(vt.vs, 14 - (int)r_new);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float e = __builtin_amdgcn_exp2f(y[i] - base);
+        float e = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], f, -base));
         float u = e * pv;
-        if (!whole) u = y[i] == -INFINITY ? 0.f : u;
+        if (!whole) {
+          e = i < n ? e : 0.f;
+          u = i < n ? u : 0.f;
+        }
         l[t] += e;
         const half_t hi = (half_t)u;
         p[t][i >> 3][0][i & 7] = hi;
@@ -307,9 +444,10 @@ __global__ __launch_bounds__(64 * kWaves, QT == 1 ? 2 : 1) void attention_kernel
     // V: the codes of keys past the end hold anything (e4m3: a NaN).
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
-      u32x4 c = x.v[n];
+      if (16 * n >= Dp) continue;
+      u32x4 c = vt.c[n];
       if (!whole) {
-        const int left = x.ok ? k1 - (t0 + 16 * g) : 0;
+        const int left = vt.ok ? k1 - (t0 + 16 * g) : 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int b = left - 4 * i;  // bytes of this dword to keep
@@ -327,29 +465,27 @@ __global__ __launch_bounds__(64 * kWaves, QT == 1 ? 2 : 1) void attention_kernel
     }
   };
 
-  constexpr int kStep = 64 * kWaves;
   int t0 = k0 + 64 * wave;
   if (t0 < k1) {
-    Tile x, y;
-    load_tile(x, load_pages(t0), t0);
-    Pages next = load_pages(t0 + kStep);
-    while (true) {
-      if (t0 + kStep < k1) load_tile(y, next, t0 + kStep);
-      next = load_pages(t0 + 2 * kStep);
-      compute(x, t0);
-      t0 += kStep;
-      if (t0 >= k1) break;
-      if (t0 + kStep < k1) load_tile(x, next, t0 + kStep);
-      next = load_pages(t0 + 2 * kStep);
-      compute(y, t0);
-      t0 += kStep;
-      if (t0 >= k1) break;
+    Place pk = place_of(t0, m16 >> 2), pv = place_of(t0, g);
+    look_up(pk);
+    look_up(pv);
+    KTile kt;
+    VTile vt;
+    for (; t0 < k1; t0 += kStep) {
+      load_k(kt, pk);
+      load_v(vt, pv);
+      advance(pk);
+      advance(pv);
+      look_up(pk);
+      look_up(pv);
+      compute(kt, vt, t0);
     }
   }
 
   // The waves' results, 16 columns of d at a time. A column's output is
   // normalised here, so that it stays in the values' range.
-  const bool direct = w.active == 1;
+  const size_t slot = SHARED ? (size_t)(2 * blockIdx.x + (begins ? 0 : 1)) * a.cols : 0;
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
     l[t] = column_sum(l[t]);
@@ -379,7 +515,7 @@ __global__ __launch_bounds__(64 * kWaves, QT == 1 ? 2 : 1) void attention_kernel
       if (direct) {
         if (a.lse) a.lse[(size_t)h * a.n_tokens + row] = (mm + __builtin_log2f(ll)) * kLn2;
       } else {
-        float *ml = a.part_ml + 2 * ((row * a.H + h) * a.n_splits + w.split);
+        float *ml = a.part_ml + 2 * (slot + c);
         ml[0] = mm;
         ml[1] = ll;
       }
@@ -408,102 +544,145 @@ __global__ __launch_bounds__(64 * kWaves, QT == 1 ? 2 : 1) void attention_kernel
       if (direct)
         store_act(a.out, (row * a.H + h) * D + 16 * n + d, x, BF16);
       else
-        a.part_o[((row * a.H + h) * a.n_splits + w.split) * D + 16 * n + d] = x;
+        a.part_o[(slot + c) * D + 16 * n + d] = x;
+    }
+  }
+  if constexpr (!SHARED) return;
+  if (at >= end) return;
+  // The next tile that has steps.
+  begins = false;
+  do ++pair;
+  while (uniform(before[pair + 1]) <= at);
+  __syncthreads();
+  }
+}
+
+// The tiles that were cut between workgroups: out = sum_i (l_i 2^(m_i - m) / l) o_i
+// over the parts. Four columns to a workgroup, one a wave; where there are many parts
+// the four waves take a column's together.
+constexpr int kReduceWaves = 4, kAlone = 16;
+__global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(AttnArgs a, int cols_per_tile, bool bf16) {
+  __shared__ float scratch[kReduceWaves], o_lds[kReduceWaves][128];
+  const uint32_t quads = (a.cols + 3) / 4;
+  uint32_t id = linear_block();
+  const int c0 = (int)(id % quads) * 4;
+  id /= quads;
+  Where w;
+  w.tile = id % a.q_tiles;
+  id /= a.q_tiles;
+  w.hk = (int)(id % (uint32_t)a.Hk);
+  w.r = id / (uint32_t)a.Hk;
+  if (w.r >= a.R) return;
+  const uint32_t i0 = w.r * a.q_tiles + w.tile, s0 = uniform(a.before[i0]), n = uniform(a.before[i0 + 1]) - s0;
+  if (n == 0) return;
+  const Share sh(a.before, a);
+  const uint32_t first = s0 / sh.per, parts = (s0 + n - 1) / sh.per - first + 1;
+  if (parts == 1) return;
+  find_rows<true>(a, w, cols_per_tile);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = a.H / a.Hk, D = a.D;
+  const bool second = s0 % sh.per != 0;  // the first part lies in slot 1 of its workgroup
+  auto slot_of = [&](uint32_t i) { return (size_t)(2 * ((first + i) * (uint32_t)a.Hk + w.hk) + (i == 0 && second ? 1 : 0)) * a.cols; };
+  const bool alone = parts <= kAlone;
+  for (int q = 0; q < 4; ++q) {
+    const int c = c0 + q;
+    if (w.col0 + c >= w.n_cols) return;
+    if (alone && q != wave) continue;
+    const uint32_t p0 = alone ? 0 : wave, step = alone ? 1 : kReduceWaves;
+    auto over_waves = [&](float v, bool is_max) {
+      v = is_max ? wave_max(v) : wave_sum(v);
+      if (alone) return v;
+      __syncthreads();
+      if (lane == 0) scratch[wave] = v;
+      __syncthreads();
+      float x = scratch[0];
+      for (int i = 1; i < kReduceWaves; ++i) x = is_max ? fmaxf(x, scratch[i]) : x + scratch[i];
+      return x;
+    };
+    // The largest m of all parts, then the weights' sum: lanes over this wave's parts.
+    float mm = -INFINITY;
+    for (uint32_t i = p0 + step * lane; i < parts; i += step * 64) mm = fmaxf(mm, a.part_ml[2 * (slot_of(i) + c)]);
+    mm = over_waves(mm, true);
+    const float base = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    for (uint32_t i = p0 + step * lane; i < parts; i += step * 64) {
+      const float *ml = a.part_ml + 2 * (slot_of(i) + c);
+      ll += ml[1] * __builtin_amdgcn_exp2f(ml[0] - base);
+    }
+    ll = over_waves(ll, false);
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+    float x0 = 0.f, x1 = 0.f;
+#pragma unroll 8
+    for (uint32_t i = p0; i < parts; i += step) {
+      const size_t at = slot_of(i) + c;
+      const float f = a.part_ml[2 * at + 1] * __builtin_amdgcn_exp2f(a.part_ml[2 * at] - base) * inv;
+      if (lane < D) x0 += f * a.part_o[at * D + lane];
+      if (lane + 64 < D) x1 += f * a.part_o[at * D + lane + 64];
+    }
+    const int h = w.hk * G + (w.col0 + c) % G;
+    const size_t row = w.q0 + (w.col0 + c) / G, out = (row * a.H + h) * D;
+    if (!alone) {
+      o_lds[wave][lane] = x0;
+      o_lds[wave][lane + 64] = x1;
+      __syncthreads();
+      x0 = x1 = 0.f;
+      for (int i = 0; i < kReduceWaves; ++i) {
+        x0 += o_lds[i][lane];
+        x1 += o_lds[i][lane + 64];
+      }
+    }
+    if (alone || wave == 0) {
+      if (lane < D) store_act(a.out, out + lane, x0, bf16);
+      if (lane + 64 < D) store_act(a.out, out + lane + 64, x1, bf16);
+      if (lane == 0 && a.lse) a.lse[(size_t)h * a.n_tokens + row] = (mm + __builtin_log2f(ll)) * kLn2;
     }
   }
 }
 
-// Rows whose keys were split: out = sum_s (l_s 2^(m_s - m) / l) o_s, one
-// workgroup per (query token, head).
-constexpr int kReduceThreads = 256;
-__global__ __launch_bounds__(kReduceThreads) void attention_reduce_kernel(AttnArgs a, int cols_per_tile, bool bf16) {
-  __shared__ float scratch[kReduceThreads / 64], w_lds[kReduceThreads], o_lds[kReduceThreads / 64][128];
-  uint32_t id = linear_block();
-  const int h = (int)(id % (uint32_t)a.H);
-  id /= (uint32_t)a.H;
-  const int j = (int)(id % a.max_q);
-  Where w;
-  w.r = id / a.max_q;
-  if (id / a.max_q >= a.total) return;  // (total: the requests here)
-  const int G = a.H / a.Hk;
-  w.tile = (uint32_t)((j * G + h % G) / cols_per_tile);
-  if (!find_rows(a, w, cols_per_tile) || j >= w.nq || w.active == 1) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n = w.active, D = a.D;
-  const size_t row = (size_t)(w.q0 + j) * a.H + h;
-  const float *ml = a.part_ml + 2 * row * a.n_splits, *po = a.part_o + row * a.n_splits * D;
-  auto reduce = [&](float v, bool is_max) {
-    v = is_max ? wave_max(v) : wave_sum(v);
-    __syncthreads();
-    if (lane == 0) scratch[wave] = v;
-    __syncthreads();
-    float x = scratch[0];
-    for (int i = 1; i < kReduceThreads / 64; ++i) x = is_max ? fmaxf(x, scratch[i]) : x + scratch[i];
-    return x;
-  };
-  // (n is at most kReduceThreads.)
-  const float ms = tid < n ? ml[2 * tid] : -INFINITY, ls = tid < n ? ml[2 * tid + 1] : 0.f;
-  const float mm = reduce(ms, true), base = mm == -INFINITY ? 0.f : mm;
-  const float ws = ls * __builtin_amdgcn_exp2f(ms - base);
-  w_lds[tid] = ws;
-  const float ll = reduce(ws, false), inv = ll == 0.f ? 0.f : 1.f / ll;
-  float x0 = 0.f, x1 = 0.f;
-#pragma unroll 8
-  for (int s = wave; s < n; s += kReduceThreads / 64) {
-    const float f = w_lds[s] * inv;
-    // A split that saw nothing of this row has weight 0 and zeros.
-    if (lane < D) x0 += f * po[(size_t)s * D + lane];
-    if (lane + 64 < D) x1 += f * po[(size_t)s * D + lane + 64];
-  }
-  o_lds[wave][lane] = x0;
-  o_lds[wave][lane + 64] = x1;
-  __syncthreads();
-  if (tid < D) {
-    float x = 0.f;
-    for (int i = 0; i < kReduceThreads / 64; ++i) x += o_lds[i][tid];
-    store_act(a.out, row * D + tid, x, bf16);
-  }
-  if (tid == 0 && a.lse) a.lse[(size_t)h * a.n_tokens + w.q0 + j] = (mm + __builtin_log2f(ll)) * kLn2;
-}
-
-// How a call is cut: columns (query tokens times heads of a kv head) by 16, 32
-// or 64, keys so that about kTargetGroups workgroups are there to share out.
-constexpr uint32_t kTargetGroups = 2048, kMinChunk = 256, kMaxSplits = kReduceThreads;
+// How a call is cut: columns (query tokens times heads of a kv head) by 16, 32 or
+// 64. The work is shared out where sequences may be longer than kShareFrom keys and
+// the (request, tile) pairs fit LDS; else one workgroup takes each tile.
+constexpr uint32_t kShareFrom = KV8_SHAREFROM, kMaxPairs = 4096, kCus = 256;
 struct Cut {
-  uint32_t qt, q_tiles, n_splits, chunk;
+  uint32_t qt, cols, q_tiles, parts;  // parts: 0, not shared out
+  size_t part_bytes, bytes;
 };
-Cut cut_of(uint32_t n_requests, uint32_t max_q, uint32_t max_len, uint32_t n_heads, uint32_t n_kv_heads, uint32_t d_head,
-           bool split) {
-  Cut c;
+Cut cut_of(uint32_t n_requests, uint32_t max_q, uint32_t max_len, uint32_t n_heads, uint32_t n_kv_heads, uint32_t d_head) {
+  Cut c{};
   const uint64_t cols = (uint64_t)max_q * (n_heads / n_kv_heads);
   c.qt = cols <= 16 ? 1 : cols <= 32 || d_head > 64 ? 2 : 4;
+  c.cols = (uint32_t)std::min<uint64_t>(cols, 16 * c.qt);
   c.q_tiles = (uint32_t)((cols + 16 * c.qt - 1) / (16 * c.qt));
-  c.n_splits = 1;
-  c.chunk = 1u << 30;
-  if (split && max_len > kMinChunk) {
-    const uint64_t groups = (uint64_t)n_requests * n_kv_heads * c.q_tiles;
-    const uint64_t want = std::min<uint64_t>(kMaxSplits, (kTargetGroups + groups - 1) / groups);
-    const uint32_t per = (uint32_t)((max_len + want - 1) / want);
-    c.chunk = std::max(kMinChunk, (per + kMinChunk - 1) / kMinChunk * kMinChunk);
-    c.n_splits = (max_len + c.chunk - 1) / c.chunk;
-  }
+  const uint64_t pairs = (uint64_t)n_requests * c.q_tiles;
+  if (max_len <= kShareFrom || pairs > kMaxPairs) return c;
+  // As many workgroups as run at a time.
+  c.parts = std::max(1u, kCus * (c.qt > 1 ? 2 : d_head > 64 ? 3 : 4) / n_kv_heads);
+  const uint64_t slots = 2ull * c.parts * n_kv_heads * c.cols;
+  c.part_bytes = slots * d_head * sizeof(float);
+  c.bytes = c.part_bytes + slots * 2 * sizeof(float) + (pairs + 1) * sizeof(uint32_t);
   return c;
 }
 
-template <bool E4M3, int NT, int NC>
-void launch_qt(const AttnArgs &a, uint32_t qt, dim3 grid, hipStream_t s) {
-  if (qt == 1)
-    hipLaunchKernelGGL((attention_kernel<E4M3, NT, NC, 1>), grid, dim3(64 * kWaves), 0, s, a);
-  else if (qt == 2)
-    hipLaunchKernelGGL((attention_kernel<E4M3, NT, NC, 2>), grid, dim3(64 * kWaves), 0, s, a);
-  else if constexpr (NC == 1)
-    hipLaunchKernelGGL((attention_kernel<E4M3, NT, NC, 4>), grid, dim3(64 * kWaves), 0, s, a);
+template <bool E4M3, int NT, int NC, int QT>
+void launch(const AttnArgs &a, hipStream_t s) {
+  if (a.parts > 0)
+    hipLaunchKernelGGL((attention_kernel<E4M3, NT, NC, QT, true>), dim3(a.parts * (uint32_t)a.Hk), dim3(64 * kWaves),
+                       ((size_t)a.R * a.q_tiles + 1) * sizeof(uint32_t), s, a);
+  else
+    hipLaunchKernelGGL((attention_kernel<E4M3, NT, NC, QT, false>), linear_grid((size_t)a.R * a.Hk * a.q_tiles),
+                       dim3(64 * kWaves), 0, s, a);
 }
 template <bool E4M3, int NT>
-void launch_nc(const AttnArgs &a, uint32_t qt, dim3 grid, hipStream_t s) {
-  if (a.D <= 64)
-    launch_qt<E4M3, NT, 1>(a, qt, grid, s);
+void launch_shape(const AttnArgs &a, uint32_t qt, hipStream_t s) {
+  if (a.D <= 64 && qt == 1)
+    launch<E4M3, NT, 1, 1>(a, s);
+  else if (a.D <= 64 && qt == 2)
+    launch<E4M3, NT, 1, 2>(a, s);
+  else if (a.D <= 64)
+    launch<E4M3, NT, 1, 4>(a, s);
+  else if (qt == 1)
+    launch<E4M3, NT, 2, 1>(a, s);
   else
-    launch_qt<E4M3, NT, 2>(a, qt, grid, s);
+    launch<E4M3, NT, 2, 2>(a, s);
 }
 
 }  // namespace
@@ -521,8 +700,7 @@ size_t dfattn_kv8_attention_workspace_bytes(uint32_t n_requests, uint32_t n_toke
       n_heads % n_kv_heads != 0 || n_heads > 65535u || n_requests > 65535u || n_tokens > (1u << 30) || d_head == 0 ||
       d_head > 128)
     return 0;
-  const Cut c = cut_of(n_requests, std::min(max_query_len, n_tokens), max_seq_len, n_heads, n_kv_heads, d_head, true);
-  return c.n_splits == 1 ? 0 : (size_t)n_tokens * n_heads * c.n_splits * (d_head + 2) * sizeof(float);
+  return cut_of(n_requests, std::min(max_query_len, n_tokens), max_seq_len, n_heads, n_kv_heads, d_head).bytes;
 }
 
 int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool, const float *k_scales,
@@ -555,7 +733,7 @@ int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool, 
   if (workspace != nullptr && (workspace_bytes < need || !aligned_to(workspace, 16)))
     return record_error(DFATTN_ERR_WORKSPACE, std::string(fn) + ": workspace too small or misaligned");
   max_query_len = std::min(max_query_len, n_tokens);
-  const Cut c = cut_of(n_requests, max_query_len, max_seq_len, n_heads, n_kv_heads, d_head, workspace != nullptr);
+  Cut c = cut_of(n_requests, max_query_len, max_seq_len, n_heads, n_kv_heads, d_head);
   const size_t item = act_dtype == DFATTN_KV_F32 ? 4 : 2;
   AttnArgs a{};
   a.q = q;
@@ -568,15 +746,22 @@ int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool, 
   a.seq_lens = seq_lens;
   a.out = out;
   a.lse = lse;
-  a.part_o = static_cast<float *>(workspace);
-  a.part_ml = a.part_o + (size_t)n_tokens * n_heads * c.n_splits * d_head;
+  // The steps are counted in 32 bits.
+  const uint64_t most = (uint64_t)n_requests * c.q_tiles * (((uint64_t)max_pages * page_size + kStep - 1) / kStep);
+  if (workspace == nullptr || most >= (1ull << 31)) c.parts = 0;
+  a.parts = c.parts;
+  if (c.parts > 0) {
+    a.part_o = static_cast<float *>(workspace);
+    a.part_ml = a.part_o + c.part_bytes / sizeof(float);
+    a.before = reinterpret_cast<uint32_t *>(a.part_ml + 2ull * 2 * c.parts * n_kv_heads * c.cols);
+  }
+  a.R = n_requests;
   a.n_tokens = n_tokens;
   a.max_q = max_query_len;
   a.max_pages = max_pages;
   a.n_pages = n_pages;
   a.q_tiles = c.q_tiles;
-  a.n_splits = c.n_splits;
-  a.chunk = c.chunk;
+  a.cols = c.cols;
   a.H = (int)n_heads;
   a.Hk = (int)n_kv_heads;
   a.D = (int)d_head;
@@ -585,26 +770,23 @@ int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool, 
   a.scale = scale;
   a.causal = causal != 0;
   a.q_vec = d_head % 4 == 0 && q_row_stride % 4 == 0 && aligned_to(q, 4 * item);
-  const uint64_t total = (uint64_t)n_requests * n_kv_heads * c.q_tiles * c.n_splits;
-  const uint64_t rows = (uint64_t)n_requests * max_query_len * n_heads;
-  if (total >= (1ull << 31) || (c.n_splits > 1 && rows >= (1ull << 31)))
+  const uint64_t tiles = (uint64_t)n_requests * n_kv_heads * c.q_tiles;
+  if (tiles * ((c.cols + 3) / 4) >= (1ull << 31))
     return record_error(DFATTN_ERR_OVERFLOW, std::string(fn) + ": shape is too large");
-  a.total = (uint32_t)total;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const dim3 grid = linear_grid(total);
   const bool e4m3 = kv_dtype == DFATTN_KV_E4M3, bf16 = act_dtype == DFATTN_KV_BF16;
   if (e4m3 && bf16)
-    launch_nc<true, 1>(a, c.qt, grid, s);
+    launch_shape<true, 1>(a, c.qt, s);
   else if (e4m3)
-    launch_nc<true, 2>(a, c.qt, grid, s);
+    launch_shape<true, 2>(a, c.qt, s);
   else if (bf16)
-    launch_nc<false, 1>(a, c.qt, grid, s);
+    launch_shape<false, 1>(a, c.qt, s);
   else
-    launch_nc<false, 2>(a, c.qt, grid, s);
+    launch_shape<false, 2>(a, c.qt, s);
   st = launched(fn);
-  if (st != DFATTN_OK || c.n_splits == 1) return st;
-  a.total = n_requests;
-  hipLaunchKernelGGL(attention_reduce_kernel, linear_grid(rows), dim3(kReduceThreads), 0, s, a, (int)(16 * c.qt), bf16);
+  if (st != DFATTN_OK || c.parts == 0) return st;
+  hipLaunchKernelGGL(attention_reduce_kernel, linear_grid(tiles * ((c.cols + 3) / 4)), dim3(64 * kReduceWaves), 0, s, a,
+                     (int)(16 * c.qt), bf16);
   return launched(fn);
 }
 
