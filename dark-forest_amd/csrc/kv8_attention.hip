@@ -6,13 +6,6 @@
 // the positions t it sees, k_t and v_t codes times the scale of their page and
 // head.
 #include "kv8.h"
-#ifndef KV8_MINSTEPS
-#define KV8_MINSTEPS 2
-#define KV8_SHAREFROM 1024
-#endif
-#ifndef KV8_OCC
-#define KV8_OCC (QT == 1 ? (NC == 1 ? 4 : 3) : 2)
-#endif
 
 #include <algorithm>
 
@@ -84,6 +77,7 @@ __device__ __forceinline__ f32x4 mfma(half8_t a, half8_t b, f32x4 c) {
 }
 
 constexpr int kWaves = 4, kStep = 64 * kWaves;  // keys of a workgroup's step
+constexpr int kResident = 2;                     // workgroups on a CU (256 registers a wave)
 
 // The rows a workgroup works on: request r, kv head hk, and the columns (query
 // token, head of the group) col0 .. of its nq * G.
@@ -128,7 +122,7 @@ __device__ __forceinline__ bool find_rows(const AttnArgs &a, Where &w, int cols_
 // 79 us, so 65). A tile cut between workgroups is merged by
 // attention_reduce_kernel; a workgroup has at most two such pieces, the tile that
 // its part begins in (slot 0) and the one that goes on behind it (slot 1).
-constexpr uint32_t kMinSteps = KV8_MINSTEPS;
+constexpr uint32_t kMinSteps = 2;
 struct Share {
   uint32_t total, per;
   // before: the steps before each (request, tile)
@@ -152,7 +146,7 @@ struct Share {
 // together, so weights keep 2^-39 of the largest one whatever the pages'
 // scales.
 template <bool E4M3, int NT, int NC, int QT, bool SHARED>
-__global__ __launch_bounds__(64 * kWaves, KV8_OCC) void attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnArgs a) {
   constexpr bool BF16 = NT == 1;
   constexpr int NV = 4 * NC;
   constexpr int kCols = 16 * QT;
@@ -368,13 +362,11 @@ __global__ __launch_bounds__(64 * kWaves, KV8_OCC) void attention_kernel(AttnArg
     x.vs = a.v_scales[head];
     const unsigned char *vp = v_lane + ((uint64_t)page * page_bytes + 16 * p.off);
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
-      if (16 * n < Dp) x.c[n] = *reinterpret_cast<const u32x4 *>(vp + 16 * n * P);
+    for (int n = 0; n < NV; ++n) x.c[n] = *reinterpret_cast<const u32x4 *>(vp + min(16 * n, Dp - 16) * P);
   };
-  auto compute = [&](const KTile &kt, const VTile &vt, int t0) {
+  auto score = [&](const KTile &kt, f32x4 (&s)[QT][4]) {
     // (Q is read from LDS in every step: kept in registers it would cost a wave per SIMD.)
     asm volatile("" ::: "memory");
-    f32x4 s[QT][4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -395,73 +387,83 @@ __global__ __launch_bounds__(64 * kWaves, KV8_OCC) void attention_kernel(AttnArg
           for (int t = 0; t < QT; ++t)
 #pragma unroll
             for (int e = 0; e < NT; ++e) s[t][j] = mfma(kh, q[t][e], s[t][j]);
+          if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
-    // Whether every column sees all 64 keys. If not, what it does not see is -infinity here
-    // and a probability of 0 below, whatever the page's scales are.
-    const bool whole = t0 + 64 <= min(k1, min_end) && __all(vt.ok);
+  };
+  auto absorb = [&](f32x4 (&s)[QT][4], VTile &vt, int t0) {
+    float f[QT], vs[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      // >= 0, or NaN. (A scale of 0 is as good as 1e-36, and -infinity times that is no NaN.)
+      f[t] = vt.ks * col_scale[t];
+      f[t] = f[t] < 1e-36f ? 1e-36f : f[t];
+      vs[t] = vt.vs;
+    }
+    // Where not every column sees all 64 keys: what it does not see gets the score -infinity,
+    // whose probability is 0; where it sees none of the lane's 16 keys, the page's scales are
+    // left out too (they may be NaN). The codes of keys past the end hold anything (e4m3: a NaN).
+    if (!(t0 + 64 <= min(k1, min_end) && __all(vt.ok))) {
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const int n = vt.ok ? min(k1, k_end[t]) - (t0 + 16 * g) : 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i >> 2][i & 3] = i < n ? s[t][i >> 2][i & 3] : -INFINITY;
+        f[t] = n > 0 ? f[t] : 1.f;
+        vs[t] = n > 0 ? vs[t] : 0.f;
+      }
+      const int left = vt.ok ? k1 - (t0 + 16 * g) : 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int b = left - 4 * i;  // bytes of this dword to keep
+        const unsigned keep = b >= 4 ? 0xffffffffu : b <= 0 ? 0u : (1u << (8 * b)) - 1u;
+#pragma unroll
+        for (int n = 0; n < NV; ++n) vt.c[n][i] &= keep;
+      }
+    }
     half8_t p[QT][2][NT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      const float f = vt.ks * col_scale[t];  // >= 0, or NaN
-      const int n = whole ? 16 : vt.ok ? min(k1, k_end[t]) - (t0 + 16 * g) : 0;  // of this lane's 16 keys
-      if (!whole) {
+      float top = s[t][0][0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[t][i >> 2][i & 3] = i < n ? s[t][i >> 2][i & 3] : -INFINITY;
-      }
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i >> 2][i & 3]);
-      top = n > 0 ? top * f : -INFINITY;
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[t][i >> 2][i & 3]);
+      top *= f[t];
       const float m_new = fmaxf(m[t], column_max(top));
       const float base = m_new == -INFINITY ? 0.f : m_new;
       const float dm = m[t] - base;  // <= 0, -inf at first
-      const float reach = column_max(top - base + __builtin_amdgcn_logf(vt.vs));
+      const float reach = column_max(top - base + __builtin_amdgcn_logf(vs[t]));
       const float r_new = fmaxf(fmaxf(r[t] + __builtin_ceilf(fmaxf(dm, -1000.f)), __builtin_ceilf(reach)), -300.f);
       if (__any(m_new != m[t] || r_new != r[t])) {
         const float al = __builtin_amdgcn_exp2f(dm), ao = __builtin_amdgcn_ldexpf(al, (int)(r[t] - r_new));
         l[t] *= al;
 #pragma unroll
-        for (int n2 = 0; n2 < NV; ++n2) o[t][n2] *= ao;
+        for (int n = 0; n < NV; ++n) o[t][n] *= ao;
         m[t] = m_new;
         r[t] = r_new;
       }
-      const float pv = __builtin_amdgcn_ldexpf(vt.vs, 14 - (int)r_new);
+      const float pv = __builtin_amdgcn_ldexpf(vs[t], 14 - (int)r_new);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float e = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], f, -base));
-        float u = e * pv;
-        if (!whole) {
-          e = i < n ? e : 0.f;
-          u = i < n ? u : 0.f;
-        }
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], f[t], -base));
         l[t] += e;
+        const float u = e * pv;
         const half_t hi = (half_t)u;
         p[t][i >> 3][0][i & 7] = hi;
         if constexpr (NT == 2) p[t][i >> 3][1][i & 7] = (half_t)(u - (float)hi);
       }
     }
-    // V: the codes of keys past the end hold anything (e4m3: a NaN).
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       if (16 * n >= Dp) continue;
-      u32x4 c = vt.c[n];
-      if (!whole) {
-        const int left = vt.ok ? k1 - (t0 + 16 * g) : 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int b = left - 4 * i;  // bytes of this dword to keep
-          c[i] &= b >= 4 ? 0xffffffffu : b <= 0 ? 0u : (1u << (8 * b)) - 1u;
-        }
-      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const half8_t vh = widen8<E4M3>(c[2 * h], c[2 * h + 1]);
+        const half8_t vh = widen8<E4M3>(vt.c[n][2 * h], vt.c[n][2 * h + 1]);
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
           for (int e = 0; e < NT; ++e) o[t][n] = mfma(vh, p[t][h][e], o[t][n]);
       }
+      if (n % 2 == 1) __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -470,16 +472,27 @@ __global__ __launch_bounds__(64 * kWaves, KV8_OCC) void attention_kernel(AttnArg
     Place pk = place_of(t0, m16 >> 2), pv = place_of(t0, g);
     look_up(pk);
     look_up(pv);
+    // V of this step and K of the next are on their way while the other is used: K's
+    // registers are free again after the scores, V's after the products.
     KTile kt;
     VTile vt;
+    load_k(kt, pk);
+    advance(pk);
+    look_up(pk);
     for (; t0 < k1; t0 += kStep) {
-      load_k(kt, pk);
       load_v(vt, pv);
-      advance(pk);
       advance(pv);
-      look_up(pk);
       look_up(pv);
-      compute(kt, vt, t0);
+      __builtin_amdgcn_sched_barrier(0);
+      f32x4 s[QT][4];
+      score(kt, s);
+      __builtin_amdgcn_sched_barrier(0);
+      if (t0 + kStep < k1) load_k(kt, pk);
+      advance(pk);
+      look_up(pk);
+      __builtin_amdgcn_sched_barrier(0);
+      absorb(s, vt, t0);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -641,7 +654,7 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
 // How a call is cut: columns (query tokens times heads of a kv head) by 16, 32 or
 // 64. The work is shared out where sequences may be longer than kShareFrom keys and
 // the (request, tile) pairs fit LDS; else one workgroup takes each tile.
-constexpr uint32_t kShareFrom = KV8_SHAREFROM, kMaxPairs = 4096, kCus = 256;
+constexpr uint32_t kShareFrom = 1024, kMaxPairs = 4096, kCus = 256;
 struct Cut {
   uint32_t qt, cols, q_tiles, parts;  // parts: 0, not shared out
   size_t part_bytes, bytes;
@@ -655,7 +668,7 @@ Cut cut_of(uint32_t n_requests, uint32_t max_q, uint32_t max_len, uint32_t n_hea
   const uint64_t pairs = (uint64_t)n_requests * c.q_tiles;
   if (max_len <= kShareFrom || pairs > kMaxPairs) return c;
   // As many workgroups as run at a time.
-  c.parts = std::max(1u, kCus * (c.qt > 1 ? 2 : d_head > 64 ? 3 : 4) / n_kv_heads);
+  c.parts = std::max(1u, kCus * kResident / n_kv_heads);
   const uint64_t slots = 2ull * c.parts * n_kv_heads * c.cols;
   c.part_bytes = slots * d_head * sizeof(float);
   c.bytes = c.part_bytes + slots * 2 * sizeof(float) + (pairs + 1) * sizeof(uint32_t);
