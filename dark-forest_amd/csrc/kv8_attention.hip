@@ -77,7 +77,7 @@ __device__ __forceinline__ f32x4 mfma(half8_t a, half8_t b, f32x4 c) {
 }
 
 constexpr int kWaves = 4, kStep = 64 * kWaves;  // keys of a workgroup's step
-constexpr int kResident = 2;                     // workgroups on a CU (256 registers a wave)
+constexpr int kResident = 2, kCus = 256;  // workgroups on a CU (256 registers a wave)
 
 // The rows a workgroup works on: request r, kv head hk, and the columns (query
 // token, head of the group) col0 .. of its nq * G.
@@ -571,36 +571,62 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
 }
 
 // The tiles that were cut between workgroups: out = sum_i (l_i 2^(m_i - m) / l) o_i
-// over the parts. Four columns to a workgroup, one a wave; where there are many parts
-// the four waves take a column's together.
-constexpr int kReduceWaves = 4, kAlone = 16;
+// over the pieces. Four columns to a workgroup, 16 where there are that many, a
+// wave to a column; where there are many pieces the four waves take a column's together. Bound by the latency of two
+// dependent reads: what says where the pieces are, then all of (m, l) and the first
+// kAhead outputs at once.
+constexpr int kReduceWaves = 4, kAhead = 8, kChunks = kCus * kResident / (64 * kReduceWaves);
+__host__ __device__ inline uint32_t reduce_cols(uint32_t cols) { return cols >= 16 ? 16 : 4; }
 __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(AttnArgs a, int cols_per_tile, bool bf16) {
   __shared__ float scratch[kReduceWaves], o_lds[kReduceWaves][128];
-  const uint32_t quads = (a.cols + 3) / 4;
+  const uint32_t per_group = reduce_cols(a.cols), col_groups = (a.cols + per_group - 1) / per_group;
   uint32_t id = linear_block();
-  const int c0 = (int)(id % quads) * 4;
-  id /= quads;
+  const int c0 = (int)(id % col_groups * per_group);
+  id /= col_groups;
   Where w;
   w.tile = id % a.q_tiles;
   id /= a.q_tiles;
   w.hk = (int)(id % (uint32_t)a.Hk);
   w.r = id / (uint32_t)a.Hk;
   if (w.r >= a.R) return;
-  const uint32_t i0 = w.r * a.q_tiles + w.tile, s0 = uniform(a.before[i0]), n = uniform(a.before[i0 + 1]) - s0;
-  if (n == 0) return;
+  const uint32_t i0 = w.r * a.q_tiles + w.tile;
+  const uint32_t b0 = a.before[i0], b1 = a.before[i0 + 1];
   const Share sh(a.before, a);
-  const uint32_t first = s0 / sh.per, parts = (s0 + n - 1) / sh.per - first + 1;
-  if (parts == 1) return;
-  find_rows<true>(a, w, cols_per_tile);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = a.H / a.Hk, D = a.D;
-  const bool second = s0 % sh.per != 0;  // the first part lies in slot 1 of its workgroup
-  auto slot_of = [&](uint32_t i) { return (size_t)(2 * ((first + i) * (uint32_t)a.Hk + w.hk) + (i == 0 && second ? 1 : 0)) * a.cols; };
-  const bool alone = parts <= kAlone;
-  for (int q = 0; q < 4; ++q) {
+  const bool any = find_rows<true>(a, w, cols_per_tile);
+  const uint32_t s0 = uniform(b0), n = uniform(b1) - s0;
+  const uint32_t first = s0 / sh.per, parts = n == 0 ? 0 : (s0 + n - 1) / sh.per - first + 1;
+  if (!any || parts <= 1) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = (int)uniform(tid >> 6), G = a.H / a.Hk, D = a.D;
+  const bool second = s0 % sh.per != 0;  // the first piece lies in slot 1 of its workgroup
+  auto slot_of = [&](uint32_t i) {
+    return (size_t)(2 * ((first + i) * (uint32_t)a.Hk + w.hk) + (i == 0 && second ? 1 : 0)) * a.cols;
+  };
+  const bool alone = parts <= kAhead;
+  const uint32_t p0 = alone ? 0 : wave, step = alone ? 1 : kReduceWaves;
+  const uint32_t mine = parts > p0 ? (parts - p0 + step - 1) / step : 0;  // this wave's pieces: p0 + step * j
+  for (int q = alone ? wave : 0; q < (int)per_group; q += alone ? kReduceWaves : 1) {
     const int c = c0 + q;
-    if (w.col0 + c >= w.n_cols) return;
-    if (alone && q != wave) continue;
-    const uint32_t p0 = alone ? 0 : wave, step = alone ? 1 : kReduceWaves;
+    if (c >= (int)a.cols || w.col0 + c >= w.n_cols) return;
+    float ms[kChunks], ls[kChunks], o0[kAhead], o1[kAhead];
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+      const uint32_t j = 64 * k + lane;
+      ms[k] = -INFINITY;
+      ls[k] = 0.f;
+      if (j < mine) {
+        const float *ml = a.part_ml + 2 * (slot_of(p0 + step * j) + c);
+        ms[k] = ml[0];
+        ls[k] = ml[1];
+      }
+    }
+    auto load = [&](uint32_t j, float &x, float &y) {
+      const float *po = a.part_o + (slot_of(p0 + step * j) + c) * D;
+      x = lane < D ? po[lane] : 0.f;
+      y = lane + 64 < D ? po[lane + 64] : 0.f;
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j)
+      if (j < mine) load(j, o0[j], o1[j]);
     auto over_waves = [&](float v, bool is_max) {
       v = is_max ? wave_max(v) : wave_sum(v);
       if (alone) return v;
@@ -611,29 +637,40 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
       for (int i = 1; i < kReduceWaves; ++i) x = is_max ? fmaxf(x, scratch[i]) : x + scratch[i];
       return x;
     };
-    // The largest m of all parts, then the weights' sum: lanes over this wave's parts.
-    float mm = -INFINITY;
-    for (uint32_t i = p0 + step * lane; i < parts; i += step * 64) mm = fmaxf(mm, a.part_ml[2 * (slot_of(i) + c)]);
+    float mm = ms[0];
+#pragma unroll
+    for (int k = 1; k < kChunks; ++k) mm = fmaxf(mm, ms[k]);
     mm = over_waves(mm, true);
     const float base = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f;
-    for (uint32_t i = p0 + step * lane; i < parts; i += step * 64) {
-      const float *ml = a.part_ml + 2 * (slot_of(i) + c);
-      ll += ml[1] * __builtin_amdgcn_exp2f(ml[0] - base);
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+      ls[k] *= __builtin_amdgcn_exp2f(ms[k] - base);
+      ll += ls[k];
     }
     ll = over_waves(ll, false);
     const float inv = ll == 0.f ? 0.f : 1.f / ll;
     float x0 = 0.f, x1 = 0.f;
-#pragma unroll 8
-    for (uint32_t i = p0; i < parts; i += step) {
-      const size_t at = slot_of(i) + c;
-      const float f = a.part_ml[2 * at + 1] * __builtin_amdgcn_exp2f(a.part_ml[2 * at] - base) * inv;
-      if (lane < D) x0 += f * a.part_o[at * D + lane];
-      if (lane + 64 < D) x1 += f * a.part_o[at * D + lane + 64];
-    }
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k)
+      for (uint32_t j = 64 * k; j < min(mine, 64u * (k + 1)); j += kAhead) {
+        if (j > 0) {
+#pragma unroll
+          for (uint32_t i = 0; i < kAhead; ++i)
+            if (j + i < mine) load(j + i, o0[i], o1[i]);
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+          if (j + i >= mine) break;
+          const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ls[k]), (j + i) % 64)) * inv;
+          x0 += f * o0[i];
+          x1 += f * o1[i];
+        }
+      }
     const int h = w.hk * G + (w.col0 + c) % G;
     const size_t row = w.q0 + (w.col0 + c) / G, out = (row * a.H + h) * D;
     if (!alone) {
+      if (q > 0) __syncthreads();
       o_lds[wave][lane] = x0;
       o_lds[wave][lane + 64] = x1;
       __syncthreads();
@@ -654,7 +691,7 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
 // How a call is cut: columns (query tokens times heads of a kv head) by 16, 32 or
 // 64. The work is shared out where sequences may be longer than kShareFrom keys and
 // the (request, tile) pairs fit LDS; else one workgroup takes each tile.
-constexpr uint32_t kShareFrom = 1024, kMaxPairs = 4096, kCus = 256;
+constexpr uint32_t kShareFrom = 1024, kMaxPairs = 4096;
 struct Cut {
   uint32_t qt, cols, q_tiles, parts;  // parts: 0, not shared out
   size_t part_bytes, bytes;
@@ -784,7 +821,8 @@ int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool, 
   a.causal = causal != 0;
   a.q_vec = d_head % 4 == 0 && q_row_stride % 4 == 0 && aligned_to(q, 4 * item);
   const uint64_t tiles = (uint64_t)n_requests * n_kv_heads * c.q_tiles;
-  if (tiles * ((c.cols + 3) / 4) >= (1ull << 31))
+  const uint64_t reductions = tiles * ((c.cols + reduce_cols(c.cols) - 1) / reduce_cols(c.cols));
+  if (reductions >= (1ull << 31))
     return record_error(DFATTN_ERR_OVERFLOW, std::string(fn) + ": shape is too large");
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool e4m3 = kv_dtype == DFATTN_KV_E4M3, bf16 = act_dtype == DFATTN_KV_BF16;
@@ -798,7 +836,7 @@ int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool, 
     launch_shape<false, 2>(a, c.qt, s);
   st = launched(fn);
   if (st != DFATTN_OK || c.parts == 0) return st;
-  hipLaunchKernelGGL(attention_reduce_kernel, linear_grid(tiles * ((c.cols + 3) / 4)), dim3(64 * kReduceWaves), 0, s, a,
+  hipLaunchKernelGGL(attention_reduce_kernel, linear_grid(reductions), dim3(64 * kReduceWaves), 0, s, a,
                      (int)(16 * c.qt), bf16);
   return launched(fn);
 }
