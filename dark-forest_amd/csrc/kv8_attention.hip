@@ -601,7 +601,7 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
   auto slot_of = [&](uint32_t i) {
     return (size_t)(2 * ((first + i) * (uint32_t)a.Hk + w.hk) + (i == 0 && second ? 1 : 0)) * a.cols;
   };
-  const bool alone = parts <= kAhead;
+  const bool alone = parts <= (per_group == 16 ? 4 * kAhead : kAhead);
   const uint32_t p0 = alone ? 0 : wave, step = alone ? 1 : kReduceWaves;
   const uint32_t mine = parts > p0 ? (parts - p0 + step - 1) / step : 0;  // this wave's pieces: p0 + step * j
   for (int q = alone ? wave : 0; q < (int)per_group; q += alone ? kReduceWaves : 1) {
@@ -688,8 +688,8 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
   }
 }
 
-// How a call is cut: columns (query tokens times heads of a kv head) by 16, 32 or
-// 64. The work is shared out where sequences may be longer than kShareFrom keys and
+// How a call is cut: columns (query tokens times heads of a kv head) by 16 or 32 (64
+// spill registers: 3 x 500 queries of 4096 keys 111 us, so 100). The work is shared out where sequences may be longer than kShareFrom keys and
 // the (request, tile) pairs fit LDS; else one workgroup takes each tile.
 constexpr uint32_t kShareFrom = 1024, kMaxPairs = 4096;
 struct Cut {
@@ -699,7 +699,7 @@ struct Cut {
 Cut cut_of(uint32_t n_requests, uint32_t max_q, uint32_t max_len, uint32_t n_heads, uint32_t n_kv_heads, uint32_t d_head) {
   Cut c{};
   const uint64_t cols = (uint64_t)max_q * (n_heads / n_kv_heads);
-  c.qt = cols <= 16 ? 1 : cols <= 32 || d_head > 64 ? 2 : 4;
+  c.qt = cols <= 16 ? 1 : 2;
   c.cols = (uint32_t)std::min<uint64_t>(cols, 16 * c.qt);
   c.q_tiles = (uint32_t)((cols + 16 * c.qt - 1) / (16 * c.qt));
   const uint64_t pairs = (uint64_t)n_requests * c.q_tiles;
@@ -725,10 +725,8 @@ template <bool E4M3, int NT>
 void launch_shape(const AttnArgs &a, uint32_t qt, hipStream_t s) {
   if (a.D <= 64 && qt == 1)
     launch<E4M3, NT, 1, 1>(a, s);
-  else if (a.D <= 64 && qt == 2)
-    launch<E4M3, NT, 1, 2>(a, s);
   else if (a.D <= 64)
-    launch<E4M3, NT, 1, 4>(a, s);
+    launch<E4M3, NT, 1, 2>(a, s);
   else if (qt == 1)
     launch<E4M3, NT, 2, 1>(a, s);
   else
