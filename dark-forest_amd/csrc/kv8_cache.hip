@@ -2,6 +2,9 @@
 // maps from lengths, the quantising append and the read-back (gfx950).
 #include "kv8.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace dfattn {
 namespace {
 
@@ -127,89 +130,365 @@ struct CacheArgs {
   size_t stride;
   uint32_t n;
   int H, D, P, n_pages;
+  bool vec;  // rows of activations may be read, or written, four values at a time
 };
 
-constexpr int kAppendThreads = 256;
+// Four values of activations as they lie in memory, columns d .. of a head of one
+// row: zero from D (left = D - d) on.
+// VEC: all rows may be read four values at a time.
+template <bool BF16, bool VEC>
+struct Quad {
+  std::conditional_t<BF16, uint2, float4> r;
+  // From element `at` of src, which is the same in all lanes.
+  __device__ __forceinline__ void load(const char *src, uint32_t at, int left) {
+    const char *p = src + at * (BF16 ? 2u : 4u);
+    if constexpr (VEC) {  // (left is 4 or more)
+      r = *reinterpret_cast<const decltype(r) *>(p);
+      return;
+    }
+    unsigned x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      x[j] = left <= j ? 0u : BF16 ? reinterpret_cast<const unsigned short *>(p)[j] : reinterpret_cast<const unsigned *>(p)[j];
+    if constexpr (BF16)
+      r = make_uint2(x[0] | x[1] << 16, x[2] | x[3] << 16);
+    else
+      r = make_float4(__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3]));
+  }
+  __device__ __forceinline__ void clear() { r = {}; }
+  __device__ __forceinline__ float4 value() const {
+    if constexpr (BF16)
+      return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16),
+                         __uint_as_float(r.y & 0xffff0000u));
+    else
+      return r;
+  }
+};
 
-// One wave takes one run (the consecutive rows of one page), one kv head and K
-// or V. It finds the largest magnitude, then the scale, then the codes; the
-// rows already there are coded again where the scale grew.
-template <bool E4M3, bool BF16>
-__global__ __launch_bounds__(kAppendThreads) void append_kernel(CacheArgs a) {
-  const uint32_t i = linear_block();
-  if (i >= a.n) return;
-  const int lane = threadIdx.x & 63;
-  const uint32_t n_slots = (uint32_t)a.n_pages * (uint32_t)a.P;
-  const uint32_t slot = a.slots[i];
-  if (slot >= n_slots) return;
-  const int off = (int)(slot % (uint32_t)a.P);
-  if (i > 0 && off != 0 && a.slots[i - 1] == slot - 1) return;  // not the first of its run
-  int len = 1;
-  while (len < a.P - off && i + len < a.n && a.slots[i + len] == slot + len) ++len;
-  const size_t page = slot / (uint32_t)a.P;
-  const int D = a.D, Dp = padded(D), P = a.P;
-  for (int task = (int)(blockIdx.z * 4 + (threadIdx.x >> 6)); task < 2 * a.H; task += 4 * gridDim.z) {
-    const int h = task >> 1;
-    const bool is_v = task & 1;
-    const void *src = is_v ? a.v : a.k;
-    auto value = [&](int row, int d) { return load_act(src, (size_t)(i + row) * a.stride + h * D + d, BF16); };
-    float amax = 0.f;
-    bool bad = false;
-    for (int e = lane; e < len * D; e += 64) {
-      const float x = fabsf(value(e / D, e % D));
-      bad |= !(x <= 3.4028234e38f);
-      amax = fmaxf(amax, x);
+// Lanes 4 i + j, j = 0..3, hold four bytes each: byte k of lane j moves to byte j of
+// lane k.
+__device__ __forceinline__ unsigned transpose4(unsigned x, int lane) {
+  const unsigned x0 = __builtin_amdgcn_mov_dpp(x, 0x00, 0xf, 0xf, false), x1 = __builtin_amdgcn_mov_dpp(x, 0x55, 0xf, 0xf, false);
+  const unsigned x2 = __builtin_amdgcn_mov_dpp(x, 0xaa, 0xf, 0xf, false), x3 = __builtin_amdgcn_mov_dpp(x, 0xff, 0xf, 0xf, false);
+  const unsigned pick = 0x0400u + 0x0101u * (lane & 3);  // this lane's byte of the first and of the second
+  const unsigned lo = __builtin_amdgcn_perm(x1, x0, pick), hi = __builtin_amdgcn_perm(x3, x2, pick);
+  return __builtin_amdgcn_perm(hi, lo, 0x05040100u);
+}
+
+constexpr int kAppendWaves = 4, kWindow = 48;
+constexpr uint32_t kAppendGroups = 2048, kFewTokens = 1024;
+
+// One side (K or V) of one page and head: its scale, and its codes.
+template <bool E4M3>
+struct Side {
+  unsigned char *codes;
+  float s, inv, ratio;
+  bool dead;  // poisoned: zeros, times NaN
+  // From the largest magnitude of the new rows, whether they hold an infinity or a
+  // NaN, and the scale of the rows that are kept (0: none).
+  __device__ __forceinline__ void scale(float amax, bool odd, float old) {
+    s = fmaxf(old, pow2_scale<E4M3>(amax));
+    dead = odd || old != old;
+    if (dead) s = __builtin_nanf("");
+    inv = dead ? 0.f : 1.f / s;
+    ratio = dead ? 0.f : old * inv;
+  }
+  __device__ __forceinline__ unsigned encode(float4 v) const {
+    if (dead) v = make_float4(0.f, 0.f, 0.f, 0.f);
+    return encode4<E4M3>(make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+  }
+  // The rows before `off`, to the new scale, by `lanes` lanes of which this is `lane`: row
+  // by row of K, column by column of V (whose last four bytes may hold newer rows).
+  __device__ __forceinline__ void recode(bool is_v, int off, int P, int D, int lane, int lanes) const {
+    const int Dp = padded(D), per_line = is_v ? (off + 3) >> 2 : Dp >> 2, lines = is_v ? D : off;
+    for (int e = lane; e < per_line * lines; e += lanes) {
+      const int line = e / per_line, q = e % per_line;
+      unsigned *at = reinterpret_cast<unsigned *>(codes + line * (is_v ? P : Dp)) + q;
+      const unsigned c = *at, keep = is_v && 4 * q + 4 > off ? ~0u << (8 * (off - 4 * q)) : 0u;
+      const float4 v = decode4<E4M3>(c);
+      *at = (encode4<E4M3>(make_float4(v.x * ratio, v.y * ratio, v.z * ratio, v.w * ratio)) & ~keep) | (c & keep);
     }
-    amax = wave_max(amax);
-    const size_t head = page * a.H + h;
-    float *scale = (is_v ? a.v_scales : a.k_scales) + head;
-    const float old = off > 0 ? *scale : 0.f;
-    float s = fmaxf(old, pow2_scale<E4M3>(amax));
-    if (__any(bad) || old != old) s = __builtin_nanf("");
-    if (lane == 0) *scale = s;
-    // A poisoned page and head holds zeros (times NaN).
-    const bool dead = s != s;
-    const float inv = dead ? 0.f : 1.f / s, ratio = dead ? 0.f : old * inv;
-    auto code = [&](float x) { return encode4<E4M3>(make_float4(dead ? 0.f : x * inv, 0.f, 0.f, 0.f)) & 0xffu; };
-    auto recode = [&](unsigned c) { return encode4<E4M3>(make_float4(decode4<E4M3>(c).x * ratio, 0.f, 0.f, 0.f)) & 0xffu; };
-    unsigned char *dst = (is_v ? a.v_pool : a.k_pool) + head * (size_t)(P * Dp);
-    const bool grew = off > 0 && ratio != 1.f;
-    for (int e = lane; e < len * Dp; e += 64) {
-      const int row = is_v ? e % len : e / Dp, d = is_v ? e / len : e % Dp;
-      if (is_v && d >= D) continue;
-      dst[is_v ? d * P + off + row : (off + row) * Dp + d] = (unsigned char)(d < D ? code(value(row, d)) : 0u);
-    }
-    if (grew)
-      for (int e = lane; e < off * Dp; e += 64) {
-        unsigned char *c = dst + (is_v ? e / off * P + e % off : e);
-        *c = (unsigned char)recode(*c);
+  }
+};
+
+struct Look {
+  float amax = 0.f, odd = 0.f;
+  __device__ __forceinline__ void at(float4 v) {
+    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+    odd += (v.x - v.x) + (v.y - v.y) + (v.z - v.z) + (v.w - v.w);  // 0, or NaN
+  }
+};
+
+// The append goes by runs, the consecutive rows of one page. A workgroup finds those
+// that start among kWindow tokens (their slots and the next ones are one load) and
+// takes every `phases`-th of them. A run's rows are taken per kv head and side (K or
+// V): the largest magnitude, the scale, the codes; rows already there are coded
+// again where the scale grew.
+// A run of one row (a generated token): 16 lanes to a head's row, or 32 (WIDE: more
+// than 64 columns), four or two of them a wave.
+// A longer one: a wave to a head and side (SPLIT, pages of 64 rows and more: all four
+// share it), 16 rows of the page and 64 columns at a time: lane 4 i + j holds columns
+// 4 i .. of rows j, 4 + j, 8 + j and 12 + j. V's codes are transposed within four
+// lanes, so that each has 16 rows of one column, which lie together. The rows are read
+// twice, the second time from the caches (with two groups' loads on their way at a time,
+// 130 to 250 registers, 8000 tokens took 31 us for 22).
+// Measured: 40 single rows (12 heads of 64, fp32) 5.5 us, a launch's latency; 8197
+// tokens of four prompts (8 heads of 128, bf16) 28-32 us for 50 MB, where a wave's two
+// passes, one behind the other, are what it waits for; 8000 tokens (12 of 64, fp32) 22 us
+// for 61 MB.
+template <bool E4M3, bool BF16, bool WIDE, bool SPLIT, bool VEC>
+__global__ __launch_bounds__(64 * kAppendWaves) void append_kernel(CacheArgs a, uint32_t phases) {
+  constexpr int kHalves = WIDE ? 2 : 1;
+  __shared__ float amax_lds[kAppendWaves], odd_lds[kAppendWaves];
+  const size_t i0 = (size_t)linear_block() * kWindow;
+  if (i0 >= a.n) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & 3, P = a.P, D = a.D, Dp = padded(D);
+  const uint32_t n_slots = (uint32_t)a.n_pages * (uint32_t)P;
+  const size_t row_bytes = a.stride * (BF16 ? 2 : 4);
+  const uint32_t phase = blockIdx.z % phases, z = blockIdx.z / phases, nz = gridDim.z / phases;
+  // Lane l holds the slot of token i0 - 1 + l.
+  const size_t token = i0 + lane;  // (one more than the lane's)
+  const uint32_t slots = token > 0 && token <= a.n ? a.slots[token - 1] : DFATTN_NO_SLOT;
+  const uint32_t before = __shfl_up(slots, 1, 64);
+  const bool valid = lane > 0 && slots < n_slots;
+  const bool follows = valid && slots % (uint32_t)P != 0 && slots == before + 1;
+  const unsigned long long links = __ballot(follows);
+  unsigned long long starts = __ballot(valid && !follows && lane <= kWindow);
+  for (uint32_t nth = 0; starts; starts &= starts - 1, ++nth) {
+    if (nth % phases != phase) continue;
+    const int first = __builtin_ctzll(starts);
+    const size_t i = i0 + first - 1;
+    const uint32_t slot = __builtin_amdgcn_readlane(slots, first);
+    const size_t page = slot / (uint32_t)P;
+    const int off = (int)(slot % (uint32_t)P);
+    const unsigned long long rest = ~(links >> first >> 1);
+    int len = 1 + (rest ? __builtin_ctzll(rest) : 64);  // rows of the run
+    if (first + len >= 64) {  // (zeros were shifted in: the run may go on behind the lanes)
+      len = 64 - first;
+      while (true) {
+        const size_t t = i + len + lane;
+        const unsigned long long gone =
+            ~__ballot(len + lane < P - off && t < a.n && a.slots[t] == slot + (uint32_t)(len + lane));
+        len += gone ? __builtin_ctzll(gone) : 64;
+        if (gone) break;
       }
+    }
+
+    if (len == 1) {
+      constexpr int kLanes = 16 * kHalves;
+      const int task = (int)(z * kAppendWaves + wave) * (64 / kLanes) + lane / kLanes;
+      for (int k = 0; k * (int)(nz * kAppendWaves) * (64 / kLanes) < 2 * a.H; ++k) {
+        const int t = task + k * (int)(nz * kAppendWaves) * (64 / kLanes), head_no = t >> 1, d = 4 * (lane % kLanes);
+        const bool is_v = t & 1, on = t < 2 * a.H;
+        const size_t head = page * a.H + (on ? head_no : 0);
+        float *scale = (is_v ? a.v_scales : a.k_scales) + head;
+        const float old = on && off > 0 ? *scale : 0.f;
+        Quad<BF16, VEC> x;
+        x.clear();
+        if (on && d < D)
+          x.load(static_cast<const char *>(is_v ? a.v : a.k) + i * row_bytes, (uint32_t)(head_no * D + d), D - d);
+        Look look;
+        look.at(x.value());
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) {
+          look.amax = fmaxf(look.amax, __shfl_xor(look.amax, o, 64));
+          look.odd += __shfl_xor(look.odd, o, 64);
+        }
+        Side<E4M3> side;
+        side.codes = (is_v ? a.v_pool : a.k_pool) + head * (size_t)(P * Dp);
+        side.scale(look.amax, look.odd != 0.f, old);
+        if (!on) continue;
+        if (d == 0) *scale = side.s;
+        if (off > 0 && side.ratio != 1.f) side.recode(is_v, off, P, D, lane % kLanes, kLanes);
+        const unsigned c = side.encode(x.value());
+        if (d >= Dp) continue;
+        if (!is_v) {
+          *reinterpret_cast<unsigned *>(side.codes + off * Dp + d) = c;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) side.codes[(d + r) * P + off] = (unsigned char)(c >> (8 * r));
+        }
+      }
+      continue;
+    }
+
+    const int last = off + len - 1, m0 = (off >> 4) + (SPLIT ? wave : 0), m1 = last >> 4, step = SPLIT ? kAppendWaves : 1;
+    const int n_tasks = 2 * a.H;
+    for (int task = SPLIT ? (int)z : (int)(z * kAppendWaves) + wave; task < n_tasks;
+         task += SPLIT ? (int)nz : (int)nz * kAppendWaves) {
+      const int h = task >> 1;
+      const bool is_v = task & 1;
+      const char *src = static_cast<const char *>(is_v ? a.v : a.k) + i * row_bytes + (size_t)(h * D) * (BF16 ? 2 : 4);
+      const size_t head = page * a.H + h;
+      float *scale = (is_v ? a.v_scales : a.k_scales) + head;
+      const float old = off > 0 ? *scale : 0.f;
+      // Rows 16 m + 4 j + sub of the page; what is outside the run is zero.
+      auto load = [&](int m, Quad<BF16, VEC> (&x)[4][kHalves]) {
+        const uint32_t at = (uint32_t)(16 * m + sub - off) * (uint32_t)a.stride + 4 * (lane >> 2);
+        if (16 * m >= off && 16 * m + 15 <= last) {
+#pragma unroll
+          for (int half = 0; half < kHalves; ++half) {
+            const int d = 64 * half + 4 * (lane >> 2);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j][half].clear();
+            if (d < D) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[j][half].load(src, at + 4 * j * (uint32_t)a.stride + 64 * half, D - d);
+            }
+          }
+          return;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int top = 16 * m + 4 * j, row = top + sub;
+          const bool any = top <= last && top + 3 >= off;
+#pragma unroll
+          for (int half = 0; half < kHalves; ++half) {
+            const int d = 64 * half + 4 * (lane >> 2);
+            x[j][half].clear();
+            if (any && row >= off && row <= last && d < D) x[j][half].load(src, at + 4 * j * (uint32_t)a.stride + 64 * half, D - d);
+          }
+        }
+      };
+      Look look;
+      auto look_at = [&](const Quad<BF16, VEC> (&x)[4][kHalves]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int half = 0; half < kHalves; ++half) look.at(x[j][half].value());
+      };
+      for (int m = m0; m <= m1; m += step) {
+        Quad<BF16, VEC> x[4][kHalves];
+        load(m, x);
+        look_at(x);
+      }
+      float amax = wave_max(look.amax);
+      bool odd = __any(look.odd != 0.f);
+      if constexpr (SPLIT) {
+        __syncthreads();  // (the task before has been read)
+        if (lane == 0) {
+          amax_lds[wave] = amax;
+          odd_lds[wave] = odd ? 1.f : 0.f;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < kAppendWaves; ++v) {
+          amax = fmaxf(amax, amax_lds[v]);
+          odd |= odd_lds[v] != 0.f;
+        }
+      }
+      Side<E4M3> side;
+      side.codes = (is_v ? a.v_pool : a.k_pool) + head * (size_t)(P * Dp);
+      side.scale(amax, odd, old);
+      const bool writes = !SPLIT || wave == 0;
+      if (writes && lane == 0) *scale = side.s;
+      // (V's bytes of the run's first rows may share four with kept ones: the wave that has the
+      // run's first group codes them again, before it writes its own.)
+      if (writes && off > 0 && side.ratio != 1.f) side.recode(is_v, off, P, D, lane, 64);
+      auto put = [&](int m, const Quad<BF16, VEC> (&x)[4][kHalves]) {
+        const bool whole = 16 * m >= off && 16 * m + 15 <= last;
+#pragma unroll
+        for (int half = 0; half < kHalves; ++half) {
+          const int d = 64 * half + 4 * (lane >> 2), column = d + sub;
+          if (!is_v) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int row = 16 * m + 4 * j + sub;
+              const unsigned c = side.encode(x[j][half].value());
+              if (row >= off && row <= last && d < Dp) *reinterpret_cast<unsigned *>(side.codes + row * Dp + d) = c;
+            }
+          } else {
+            u32x4 t;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = transpose4(side.encode(x[j][half].value()), lane);
+            if (column >= Dp) continue;
+            unsigned char *at = side.codes + column * P + 16 * m;
+            if (whole) {
+              *reinterpret_cast<u32x4 *>(at) = t;
+            } else {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int top = 16 * m + 4 * j;
+                if (top > last || top + 3 < off) continue;
+                if (top >= off && top + 3 <= last) {
+                  *reinterpret_cast<unsigned *>(at + 4 * j) = t[j];
+                } else {
+#pragma unroll
+                  for (int r = 0; r < 4; ++r)
+                    if (top + r >= off && top + r <= last) at[4 * j + r] = (unsigned char)(t[j] >> (8 * r));
+                }
+              }
+            }
+          }
+        }
+      };
+      for (int m = m0; m <= m1; m += step) {
+        Quad<BF16, VEC> x[4][kHalves];
+        load(m, x);
+        put(m, x);
+      }
+    }
   }
 }
 
 // ---------------------------------------------------------------- read
+// A wave takes four rows of the list and 64 columns of a head at a time, lane 4 i +
+// j columns 4 i .. of row j. V's codes of four consecutive rows of a page are read
+// as the append writes them; other rows byte by byte.
+constexpr int kReadWaves = 4;
+constexpr uint32_t kReadGroups = 4096;
 template <bool E4M3, bool BF16>
-__global__ __launch_bounds__(256) void read_kernel(CacheArgs a) {
-  const uint32_t i = linear_block();
-  if (i >= a.n) return;
-  const uint32_t slot = a.slots[i];
-  const bool in = slot < (uint32_t)a.n_pages * (uint32_t)a.P;
-  const size_t page = in ? slot / (uint32_t)a.P : 0;
-  const int off = in ? (int)(slot % (uint32_t)a.P) : 0, Dp = padded(a.D), dm = a.H * a.D;
-  for (int e = (int)threadIdx.x; e < 2 * dm; e += 256) {
-    const bool is_v = e >= dm;
-    const int x = is_v ? e - dm : e, h = x / a.D, d = x % a.D;
+__global__ __launch_bounds__(64 * kReadWaves) void read_kernel(CacheArgs a) {
+  const size_t i0 = ((size_t)linear_block() * kReadWaves + (threadIdx.x >> 6)) * 4;
+  if (i0 >= a.n) return;
+  const int lane = threadIdx.x & 63, sub = lane & 3, P = a.P, D = a.D, Dp = padded(D), shift = Dp > 64 ? 1 : 0;
+  const size_t i = i0 + sub, dm = (size_t)a.H * D;
+  const uint32_t slot = i < a.n ? a.slots[i] : DFATTN_NO_SLOT;
+  const bool in = slot < (uint32_t)a.n_pages * (uint32_t)P;
+  const size_t page = in ? slot / (uint32_t)P : 0;
+  const int off = in ? (int)(slot % (uint32_t)P) : 0;
+  const uint32_t slot0 = __builtin_amdgcn_mov_dpp(slot, 0x00, 0xf, 0xf, false);
+  const bool together = __all(in && slot0 % 4 == 0 && slot == slot0 + sub);
+  const int tasks = (2 * a.H) << shift;
+  for (int task = blockIdx.z; task < tasks; task += gridDim.z) {
+    const int x = task >> shift, h = x >> 1, d = 64 * (task & shift) + 4 * (lane >> 2);
+    const bool is_v = x & 1;
+    if (!(is_v && together) && d >= D) continue;
     const size_t head = page * a.H + h;
-    float val = 0.f;
-    if (in) {
-      const unsigned char *base = (is_v ? a.v_pool : a.k_pool) + head * (size_t)(a.P * Dp);
-      val = decode4<E4M3>(base[is_v ? d * a.P + off : off * Dp + d]).x * (is_v ? a.v_scales : a.k_scales)[head];
+    const unsigned char *base = (is_v ? a.v_pool : a.k_pool) + head * (size_t)(P * Dp);
+    unsigned c = 0;
+    if (!is_v) {
+      c = *reinterpret_cast<const unsigned *>(base + off * Dp + d);
+    } else if (together) {
+      const unsigned t = d + sub < Dp ? *reinterpret_cast<const unsigned *>(base + (d + sub) * P + (off & ~3)) : 0u;
+      c = transpose4(t, lane);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) c |= (unsigned)base[(d + r) * P + off] << (8 * r);
     }
+    if (i >= a.n || d >= D) continue;
+    const float s = (is_v ? a.v_scales : a.k_scales)[head];
+    float4 v = decode4<E4M3>(c);
+    v = in ? make_float4(v.x * s, v.y * s, v.z * s, v.w * s) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const size_t at = i * dm + (size_t)(h * D + d);
     void *out = is_v ? a.v_out : a.k_out;
-    if (BF16)
-      static_cast<unsigned short *>(out)[(size_t)i * dm + x] = (unsigned short)bf16_bits(val);
-    else
-      static_cast<float *>(out)[(size_t)i * dm + x] = val;
+    if (a.vec) {
+      if constexpr (BF16)
+        *reinterpret_cast<uint2 *>(static_cast<unsigned short *>(out) + at) =
+            make_uint2(bf16_bits(v.x) | bf16_bits(v.y) << 16, bf16_bits(v.z) | bf16_bits(v.w) << 16);
+      else
+        *reinterpret_cast<float4 *>(static_cast<float *>(out) + at) = v;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float y = (&v.x)[r];
+        if (d + r >= D) break;
+        if constexpr (BF16)
+          static_cast<unsigned short *>(out)[at + r] = (unsigned short)bf16_bits(y);
+        else
+          static_cast<float *>(out)[at + r] = y;
+      }
+    }
   }
 }
 
@@ -278,7 +557,8 @@ int dfattn_kv8_append(const void *k, const void *v, const uint32_t *slot_map, vo
   if (st != DFATTN_OK) return st;
   if (row_stride < (uint64_t)n_kv_heads * d_head)
     return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": row_stride must be at least n_kv_heads * d_head");
-  if (n_tokens > (1u << 31)) return record_error(DFATTN_ERR_OVERFLOW, std::string(fn) + ": too many tokens");
+  if (n_tokens > (1u << 31) || row_stride > (1u << 21))
+    return record_error(DFATTN_ERR_OVERFLOW, std::string(fn) + ": too many tokens, or a row_stride above 2^21");
   if (n_tokens == 0) return DFATTN_OK;
   st = check_all(fn, {k, v}, act_dtype == DFATTN_KV_F32 ? 4 : 2);
   if (st == DFATTN_OK) st = check_all(fn, {slot_map, k_scales, v_scales}, 4);
@@ -298,11 +578,41 @@ int dfattn_kv8_append(const void *k, const void *v, const uint32_t *slot_map, vo
   a.D = (int)d_head;
   a.P = (int)page_size;
   a.n_pages = (int)n_pages;
-  dim3 grid = linear_grid(n_tokens);
-  grid.z = (2 * n_kv_heads + 3) / 4;
+  const size_t four = act_dtype == DFATTN_KV_F32 ? 16 : 8;
+  a.vec = d_head % 4 == 0 && row_stride % 4 == 0 && aligned_to(k, four) && aligned_to(v, four);
+  // About kAppendGroups workgroups (250 to 300 a us start, empty or not: 8000 for a
+  // prompt of 8197 tokens took 30 us for that alone): a window's runs are dealt to several
+  // while there are fewer.
+  const bool wide = d_head > 64, split = page_size >= 64;
+  const uint32_t windows = (n_tokens + kWindow - 1) / kWindow;
+  // The heads' sides that a workgroup takes at once: few tokens are taken to be runs of one
+  // row, which need fewer workgroups (256 rows of 12 heads: 10 us for 15); for many that
+  // leaves waves without work where the runs are longer (8000 tokens: 25 us for 22).
+  const uint32_t per_group = split ? 1 : n_tokens <= kFewTokens ? kAppendWaves * (wide ? 2 : 4) : kAppendWaves;
+  const uint32_t tasks = std::min((2 * n_kv_heads + per_group - 1) / per_group, 1024u);
+  const uint32_t phases = std::min<uint32_t>(kWindow, std::max<uint64_t>(1, kAppendGroups / ((uint64_t)windows * tasks)));
+  dim3 grid = linear_grid(windows);
+  grid.z = phases * tasks;
   by_types(act_dtype, kv_dtype, [&](auto e4m3, auto bf16) {
-    hipLaunchKernelGGL((append_kernel<decltype(e4m3)::value, decltype(bf16)::value>), grid, dim3(kAppendThreads), 0,
-                       static_cast<hipStream_t>(stream), a);
+    constexpr bool E = decltype(e4m3)::value, B = decltype(bf16)::value;
+    auto go = [&](auto wide_, auto split_, auto vec_) {
+      hipLaunchKernelGGL((append_kernel<E, B, decltype(wide_)::value, decltype(split_)::value, decltype(vec_)::value>), grid,
+                         dim3(64 * kAppendWaves), 0, static_cast<hipStream_t>(stream), a, phases);
+    };
+    auto go_vec = [&](auto wide_, auto split_) {
+      if (a.vec)
+        go(wide_, split_, std::true_type{});
+      else
+        go(wide_, split_, std::false_type{});
+    };
+    if (wide && split)
+      go_vec(std::true_type{}, std::true_type{});
+    else if (wide)
+      go_vec(std::true_type{}, std::false_type{});
+    else if (split)
+      go_vec(std::false_type{}, std::true_type{});
+    else
+      go_vec(std::false_type{}, std::false_type{});
   });
   return launched(fn);
 }
@@ -334,8 +644,14 @@ int dfattn_kv8_read(const void *k_pool, const void *v_pool, const float *k_scale
   a.D = (int)d_head;
   a.P = (int)page_size;
   a.n_pages = (int)n_pages;
+  const size_t four = act_dtype == DFATTN_KV_F32 ? 16 : 8;
+  a.vec = d_head % 4 == 0 && aligned_to(k_out, four) && aligned_to(v_out, four);
+  // Heads to workgroups of their own as long as there are few waves.
+  const uint32_t groups = (n_rows + 4 * kReadWaves - 1) / (4 * kReadWaves), tasks = 2 * n_kv_heads * (d_head > 64 ? 2 : 1);
+  dim3 grid = linear_grid(groups);
+  grid.z = std::min(tasks, std::max(1u, kReadGroups / groups));
   by_types(act_dtype, kv_dtype, [&](auto e4m3, auto bf16) {
-    hipLaunchKernelGGL((read_kernel<decltype(e4m3)::value, decltype(bf16)::value>), linear_grid(n_rows), dim3(256), 0,
+    hipLaunchKernelGGL((read_kernel<decltype(e4m3)::value, decltype(bf16)::value>), grid, dim3(64 * kReadWaves), 0,
                        static_cast<hipStream_t>(stream), a);
   });
   return launched(fn);

@@ -392,7 +392,7 @@ size_t dfattn_kv8_pool_bytes(uint32_t n_pages, uint32_t n_kv_heads, uint32_t pag
  * infinity or NaN gets the scale NaN: all its values are NaN until its first
  * row is written again. (A number within half a step of 2^128 reads as
  * infinity.) act_dtype: DFATTN_KV_F32 or DFATTN_KV_BF16, the
- * type of k and v, whose rows start row_stride elements apart.               */
+ * type of k and v, whose rows start row_stride (at most 2^21) elements apart. */
 int dfattn_kv8_append(const void *k, const void *v, const uint32_t *slot_map, void *k_pool,
                       void *v_pool, float *k_scales, float *v_scales, uint32_t act_dtype,
                       uint32_t kv_dtype, uint32_t n_tokens, uint32_t n_kv_heads,

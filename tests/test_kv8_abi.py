@@ -52,7 +52,7 @@ CACHE = [(dict(act=2), FLAGS), (dict(kv=0), FLAGS), (dict(kv=4), FLAGS), (dict(h
 @pytest.mark.parametrize("kw,status", CACHE + [
     *[(dict(ptrs={i: None}), NULL) for i in range(7)], (dict(ptrs={0: ODD}), MIS), (dict(ptrs={1: ODD2}, act=1), MIS),
     (dict(ptrs={2: ODD}), MIS), (dict(ptrs={3: ctypes.c_void_p(0x10008)}), MIS), (dict(ptrs={6: ODD}), MIS),
-    (dict(stride=127), SHAPE), (dict(n=(1 << 31) + 1), OVER), (dict(n=0), 0),
+    (dict(stride=127), SHAPE), (dict(stride=(1 << 21) + 1), OVER), (dict(n=(1 << 31) + 1), OVER), (dict(n=0), 0),
 ])
 def test_append(kw, status):
     expect(status, "dfattn_kv8_append", append(**kw))
