@@ -528,8 +528,17 @@ int dfattn_paged_plan(const uint32_t *cached_lens, const uint32_t *new_lens, con
   if (st == DFATTN_OK && n_free > 0) st = check_all(fn, {free_pages}, 4);
   if (st == DFATTN_OK && token_capacity > 0) st = check_all(fn, {slot_map}, 4);
   if (st != DFATTN_OK) return st;
-  if (counts <= free_start && free_start < counts + 3)
-    return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": free_start must not lie in counts");
+  // Every workgroup reads all lengths while others write: nothing may be written in place.
+  const struct {
+    const uint32_t *p;
+    size_t n;
+  } spans[] = {{block_table, (size_t)n_requests * max_pages}, {seq_lens, n_requests}, {query_start, n_requests + 1u},
+               {slot_map, token_capacity}, {counts, 3}, {cached_lens, n_requests}, {new_lens, n_requests},
+               {free_pages, n_free}, {free_start, 1}};
+  for (int i = 0; i < 5; ++i)
+    for (int j = i + 1; j < 9; ++j)
+      if (spans[i].n > 0 && spans[j].n > 0 && spans[i].p < spans[j].p + spans[j].n && spans[j].p < spans[i].p + spans[i].n)
+        return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": outputs must not overlap inputs or each other");
   PlanArgs a{cached_lens, new_lens, free_pages, free_start, block_table, seq_lens, query_start, slot_map, counts,
              n_free, n_requests, max_pages, token_capacity, page_size, n_pages};
   // Four tokens a thread, up to two workgroups a CU.

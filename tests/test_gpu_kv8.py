@@ -204,6 +204,52 @@ def test_append_from_a_fused_projection(device):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+def check_calls(device, heads, d, page, pages, fmt, act, calls, shift=0, extra=0, spreads=(0.5, 3.0)):
+    """Appends `calls` (lists of slots) and compares every written value and scale bit for bit; rows of k and v
+    start heads * d + extra elements apart, the first at element `shift`."""
+    rng = np.random.RandomState(heads * 1000 + d + page)
+    cache = dfattn.kv8_cache(pages, heads, d, page, ref.DTYPE[fmt], device)
+    refs = [ref.Cache(pages, heads, page, d, fmt) for _ in range(2)]
+    top = {}
+    for n, slots in enumerate(calls):
+        wide = [as_act(random_rows(rng, len(slots), 1, heads * d + extra, spreads[n % len(spreads)])[:, 0], act, device)
+                for _ in range(2)]
+        kv = [w[:, shift:shift + heads * d] for w in wide]
+        for r, x in zip(refs, kv):
+            r.append(x.double().cpu().numpy().reshape(len(slots), heads, d), slots)
+        dfattn.kv8_append(cache, *kv, i32(slots, device))
+        for s_ in slots:
+            if 0 <= s_ < pages * page:
+                top[s_ // page] = s_ % page
+        at = [p_ * page + o for p_ in sorted(top) for o in range(top[p_] + 1)]
+        for name, g, w in zip("kv", dfattn.kv8_read(cache, i32(at, device), d), refs):
+            assert np.array_equal(g.double().cpu().numpy(), w.read(at)), (name, n)
+        for t, w in zip(cache[2:], refs):
+            assert np.array_equal(t.double().cpu().numpy(), w.scale), n
+
+
+@pytest.mark.parametrize("fmt,act", [("i8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("heads,d,page,extra,shift", [
+    (2, 64, 16, 0, 0), (3, 128, 16, 4, 0), (1, 20, 48, 1, 1), (2, 64, 64, 0, 0), (1, 100, 64, 8, 4), (2, 33, 128, 0, 0),
+    (1, 128, 256, 3, 2), (9, 16, 256, 0, 0)])
+def test_append_long_runs(device, heads, d, page, extra, shift, fmt, act):
+    """Prompts of many pages with partial first and last ones, rows behind kept rows whose scale grows, runs that
+    begin and end anywhere among the tokens, and a thousand requests of one token between them."""
+    say("long runs", heads, d, page, fmt, act)
+    pages = 1700 if page == 16 else 400 if page <= 64 else 130
+    order = np.random.RandomState(page).permutation(pages)
+    pos = lambda first, a, b: [int(order[first + t // page]) * page + t % page for t in range(a, b)]
+    few = 5 + page // 3
+    calls = [
+        pos(0, 0, 5) + pos(20, 0, few),                                     # small values
+        pos(0, 5, 5 * page + 3) + [-1, -1] + pos(20, few, 3 * page),        # larger ones behind them
+        pos(0, 5 * page + 3, 5 * page + 4) + pos(20, 3 * page, 3 * page + 2) +
+        [s for i in range(30, pages) for s in pos(i, 0, 1)] + pos(10, 0, 6 * page + 1),
+        [s for i in range(30, pages) for s in pos(i, 1, 2 + i % 2)] + pos(10, 6 * page + 1, 6 * page + 2),
+    ]
+    check_calls(device, heads, d, page, pages, fmt, act, calls, shift, extra)
+
+
 # ---------------------------------------------------------------- attention
 def build(device, lens, heads, d, page, fmt, seed, junk=True):
     """A cache holding lens[r] tokens of each request through the append, in scattered pages, the rest of the
@@ -302,6 +348,71 @@ def test_attention(device, case, fmt, act):
     say("attention", case, ATTENTION[case], fmt, act)
     lens, qlens, heads, kv_heads, d, page = ATTENTION[case]
     check_attention(device, lens, qlens, heads, kv_heads, d, page, fmt, act, seed=case)
+
+
+# Tiles cut between workgroups into two to seventy pieces, of one query to more than a tile's.
+CUT = [
+    ([2300], [1], 2, 2, 64, 16),
+    ([7000, 1], [1, 1], 4, 2, 32, 16),
+    ([20000], [1], 1, 1, 64, 32),
+    ([36000, 300], [1, 1], 1, 1, 16, 16),
+    ([5000, 2300, 130], [9, 1, 100], 4, 2, 128, 64),
+    ([9000], [20], 2, 1, 64, 16),
+    ([20000], [20], 2, 1, 32, 16),
+    ([1300], [1], 600, 600, 16, 16),                             # more heads than workgroups run at a time
+    ([1025, 1024, 0, 513], [3, 0, 2, 513], 1, 1, 80, 48),
+]
+
+
+@pytest.mark.parametrize("fmt,act", [("i8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("case", range(len(CUT)))
+def test_attention_cut_between_workgroups(device, case, fmt, act):
+    say("cut", case, CUT[case], fmt, act)
+    lens, qlens, heads, kv_heads, d, page = CUT[case]
+    check_attention(device, lens, qlens, heads, kv_heads, d, page, fmt, act, seed=100 + case)
+
+
+@pytest.mark.parametrize("r", [4096, 4097])
+def test_attention_of_many_requests(device, r):
+    """The most requests whose work is shared out, and one more, with one long sequence among them."""
+    say("requests", r)
+    lens, qlens = [1 + i % 3 for i in range(r)], [1 - (i % 7 == 3) for i in range(r)]
+    lens[r // 2] = 1500
+    check_attention(device, lens, qlens, 1, 1, 16, 16, "i8", "f32", seed=r)
+
+
+def test_requests_that_share_pages(device):
+    """Two requests with a common prefix in the same pages, each with a last page of its own."""
+    heads, d, page, n = 2, 64, 16, 200
+    cache, table, seq, vals = build(device, [n, n], heads, d, page, "i8", 31)
+    common = table.clone()
+    common[1, :n // page] = table[0, :n // page]
+    q = torch.randn(1, heads * d, device=device)
+    out, _ = dfattn.kv8_attention(cache, q.repeat(2, 1), common, i32([0, 1, 2], device), seq, heads, 1, n)
+    ok = np.ones(n, bool)
+    k, v = (np.concatenate([vals[0][i][:n // page * page], vals[1][i][n // page * page:]]) for i in range(2))
+    for r, (kr, vr) in enumerate((vals[0], (k, v))):
+        want, _, tol, _ = ref.attention(q.double().cpu().numpy(), lambda _: (kr, ok), lambda _: (vr, ok), [0, 1], [n], heads,
+                                        heads, d, d ** -0.5, True, 1, 2.0 ** -22, 0.0, page)
+        assert (np.abs(out[r].double().cpu().numpy() - want[0]) <= tol[0]).all()
+
+
+def test_two_streams_at_once(device):
+    """Calls that overlap, each with its own cache and workspace."""
+    sets = []
+    for i in range(2):
+        cache, table, seq, _ = build(device, [3000 + 100 * i, 700], 4, 64, 16, "i8", 40 + i)
+        q = torch.randn(2, 4 * 64, device=device)
+        start = i32([0, 1, 2], device)
+        sets.append((cache, q, table, start, seq, dfattn.kv8_attention(cache, q, table, start, seq, 4, 1, 3100)))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(10):
+        for s, (cache, q, table, start, seq, want) in zip(streams, sets):
+            got.append((dfattn.kv8_attention(cache, q, table, start, seq, 4, 1, 3100, stream=s), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for g, w in got for x, y in zip(g, w))
 
 
 @pytest.mark.parametrize("act", ["f32", "bf16"])

@@ -32,6 +32,9 @@ def plan(ptrs=None, n_free=9, r=4, width=8, cap=64, page=16, pages=100):
     (dict(r=0), SHAPE), (dict(width=0), SHAPE), (dict(page=0), SHAPE), (dict(pages=0), SHAPE), (dict(r=8193), OVER),
     (dict(pages=1 << 28), OVER), (dict(width=1 << 28), OVER), (dict(cap=(1 << 31) + 1), OVER),
     (dict(ptrs={3: ctypes.c_void_p(0x10000 + 0x8000 + 8)}), SHAPE),  # free_start inside counts
+    (dict(ptrs={5: ctypes.c_void_p(0x10000)}), SHAPE),               # seq_lens in place of cached_lens
+    (dict(ptrs={7: ctypes.c_void_p(0x10000 + 0x8000 - 4 * 63)}), SHAPE),  # the slot map's end in counts
+    (dict(ptrs={4: ctypes.c_void_p(0x10000 + 0x2000 + 32)}), SHAPE),      # the table in the free pages' last entry
 ])
 def test_plan(kw, status):
     expect(status, "dfattn_paged_plan", plan(**kw))
