@@ -21,7 +21,7 @@ struct AttnArgs {
   const uint32_t *table, *query_start, *seq_lens;
   void *out;
   float *lse;
-  // Shared out (see Share): normalised outputs [parts * Hk][2][cols][D] and (m, l) [parts * Hk][2][cols][2]
+  // Shared out (see Share): normalised outputs [parts * Hk][2][cols][Dp] and (m, l) [parts * Hk][2][cols][2]
   // of the pieces, and the steps before each (request, tile) [R * q_tiles + 1].
   float *part_o, *part_ml;
   uint32_t *before;
@@ -29,14 +29,29 @@ struct AttnArgs {
   int H, Hk, D, P;
   size_t q_stride;
   float scale;
-  bool causal, q_vec;
+  bool causal, q_vec, out_vec;  // q, out: four values at a time
 };
 
-__device__ __forceinline__ void store_act(void *p, size_t i, float x, bool bf16) {
-  if (bf16)
-    static_cast<unsigned short *>(p)[i] = (unsigned short)bf16_bits(x);
-  else
-    static_cast<float *>(p)[i] = x;
+// The first `left` of four values, to element i of the output.
+__device__ __forceinline__ void store_out(const AttnArgs &a, size_t i, int left, f32x4 x, bool bf16) {
+  unsigned short *const p16 = static_cast<unsigned short *>(a.out) + i;
+  float *const p32 = static_cast<float *>(a.out) + i;
+  if (a.out_vec) {
+    if (bf16)
+      *reinterpret_cast<uint2 *>(p16) =
+          make_uint2(bf16_bits(x[0]) | bf16_bits(x[1]) << 16, bf16_bits(x[2]) | bf16_bits(x[3]) << 16);
+    else
+      *reinterpret_cast<f32x4 *>(p32) = x;
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j >= left) break;
+    if (bf16)
+      p16[j] = (unsigned short)bf16_bits(x[j]);
+    else
+      p32[j] = x[j];
+  }
 }
 
 // Maximum and sum over the four lanes l, l ^ 16, l ^ 32, l ^ 48 (one column of
@@ -152,9 +167,11 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
   constexpr int kCols = 16 * QT;
   extern __shared__ uint32_t before[];  // SHARED: R * q_tiles + 1
   __shared__ float m_lds[kWaves][kCols], l_lds[kWaves][kCols];
-  __shared__ __attribute__((aligned(16))) float o_lds[kWaves][kCols][20];
   __shared__ uint32_t wave_steps[kWaves];
-  __shared__ half8_t q_lds[QT][NC][2][NT][64];
+  __shared__ union {
+    half8_t q[QT][NC][2][NT][64];
+    float o[kWaves][kCols][68];  // (once Q has been used)
+  } lds;
   __shared__ float scale_lds[kCols];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m16 = lane & 15, g = lane >> 4;
   const int G = a.H / a.Hk, D = a.D, Dp = padded(D), P = a.P;
@@ -289,7 +306,7 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
           q[1][i] = (half_t)(y - (float)q[0][i]);
         }
 #pragma unroll
-        for (int e2 = 0; e2 < NT; ++e2) q_lds[t][n][h][e2][lane] = q[e2];
+        for (int e2 = 0; e2 < NT; ++e2) lds.q[t][n][h][e2][lane] = q[e2];
       }
   }
   __syncthreads();
@@ -379,7 +396,7 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
-          for (int e = 0; e < NT; ++e) q[t][e] = q_lds[t][n][h][e][lane];
+          for (int e = 0; e < NT; ++e) q[t][e] = lds.q[t][n][h][e][lane];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const half8_t kh = widen8<E4M3>(kt.c[n][j][2 * h], kt.c[n][j][2 * h + 1]);
@@ -535,29 +552,32 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
     }
   }
 #pragma unroll
-  for (int n = 0; n < NV; ++n) {
-    if (16 * n >= D) break;
-    if (n > 0) __syncthreads();
+  for (int half = 0; half < NC; ++half) {
+    if (half > 0) __syncthreads();
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      f32x4 x = o[t][n] * weight[t];
+    for (int n = 4 * half; n < 4 * half + 4; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], shift[t]);
-      *reinterpret_cast<f32x4 *>(&o_lds[wave][16 * t + m16][4 * g]) = x;
-    }
+      for (int t = 0; t < QT; ++t) {
+        f32x4 x = o[t][n] * weight[t];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], shift[t]);
+        *reinterpret_cast<f32x4 *>(&lds.o[wave][16 * t + m16][16 * (n - 4 * half) + 4 * g]) = x;
+      }
     __syncthreads();
-    for (int e = tid; e < 16 * kCols; e += 64 * kWaves) {
-      const int c = e >> 4, d = e & 15;
-      if (col0 + c >= w.n_cols || 16 * n + d >= D) continue;
-      float x = o_lds[0][c][d];
 #pragma unroll
-      for (int v = 1; v < kWaves; ++v) x += o_lds[v][c][d];
-      const int h = w.hk * G + (col0 + c) % G;
-      const size_t row = w.q0 + (col0 + c) / G;
-      if (direct)
-        store_act(a.out, (row * a.H + h) * D + 16 * n + d, x, BF16);
-      else
-        a.part_o[(slot + c) * D + 16 * n + d] = x;
+    for (int e = tid; e < 16 * kCols; e += 64 * kWaves) {
+      const int c = e >> 4, d = 64 * half + 4 * (e & 15);
+      if (col0 + c >= w.n_cols || d >= D) continue;
+      f32x4 x = *reinterpret_cast<const f32x4 *>(&lds.o[0][c][4 * (e & 15)]);
+#pragma unroll
+      for (int v = 1; v < kWaves; ++v) x += *reinterpret_cast<const f32x4 *>(&lds.o[v][c][4 * (e & 15)]);
+      if (direct) {
+        const int h = w.hk * G + (col0 + c) % G;
+        const size_t row = w.q0 + (col0 + c) / G;
+        store_out(a, (row * a.H + h) * D + d, D - d, x, BF16);
+      } else {
+        *reinterpret_cast<f32x4 *>(a.part_o + (slot + c) * Dp + d) = x;
+      }
     }
   }
   if constexpr (!SHARED) return;
@@ -571,14 +591,17 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
 }
 
 // The tiles that were cut between workgroups: out = sum_i (l_i 2^(m_i - m) / l) o_i
-// over the pieces. Four columns to a workgroup, 16 where there are that many, a
-// wave to a column; where there are many pieces the four waves take a column's together. Bound by the latency of two
-// dependent reads: what says where the pieces are, then all of (m, l) and the first
-// kAhead outputs at once.
-constexpr int kReduceWaves = 4, kAhead = 8, kChunks = kCus * kResident / (64 * kReduceWaves);
-__host__ __device__ inline uint32_t reduce_cols(uint32_t cols) { return cols >= 16 ? 16 : 4; }
+// over the pieces i. A quarter of a wave takes a column, a lane four or eight of its
+// values, 16 pieces' (m, l) at a time. Few columns (a generated token) are shared by the
+// workgroup's four waves where there are more than kAhead pieces, so that all
+// are read at once. Bound by the latency of two dependent reads: what says where the pieces
+// are, then (m, l) and the first kAhead outputs together.
+constexpr int kReduceWaves = 4, kAhead = 8;
+__host__ __device__ inline uint32_t reduce_cols(uint32_t cols) { return cols > 16 ? 16 : 4; }
+template <int NC>
 __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(AttnArgs a, int cols_per_tile, bool bf16) {
-  __shared__ float scratch[kReduceWaves], o_lds[kReduceWaves][128];
+  __shared__ float ml_lds[kReduceWaves][4][2];
+  __shared__ f32x4 o_lds[kReduceWaves][NC][64];
   const uint32_t per_group = reduce_cols(a.cols), col_groups = (a.cols + per_group - 1) / per_group;
   uint32_t id = linear_block();
   const int c0 = (int)(id % col_groups * per_group);
@@ -596,96 +619,113 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
   const uint32_t s0 = uniform(b0), n = uniform(b1) - s0;
   const uint32_t first = s0 / sh.per, parts = n == 0 ? 0 : (s0 + n - 1) / sh.per - first + 1;
   if (!any || parts <= 1) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = (int)uniform(tid >> 6), G = a.H / a.Hk, D = a.D;
+  const int tid = threadIdx.x, lane = tid & 63, wave = (int)uniform(tid >> 6), l16 = lane & 15, G = a.H / a.Hk, D = a.D,
+            Dp = padded(D);
   const bool second = s0 % sh.per != 0;  // the first piece lies in slot 1 of its workgroup
   auto slot_of = [&](uint32_t i) {
     return (size_t)(2 * ((first + i) * (uint32_t)a.Hk + w.hk) + (i == 0 && second ? 1 : 0)) * a.cols;
   };
-  const bool alone = parts <= (per_group == 16 ? 4 * kAhead : kAhead);
-  const uint32_t p0 = alone ? 0 : wave, step = alone ? 1 : kReduceWaves;
+  // shared: wave v takes the pieces v, v + 4, ... of all four columns; else all of its own four.
+  const bool shared = per_group == 4;
+  if (shared && parts <= kAhead && wave > 0) return;
+  const bool split = shared && parts > kAhead;
+  const int c = c0 + (shared ? 0 : 4 * wave) + (lane >> 4);
+  const bool on = c < (int)a.cols && w.col0 + c < w.n_cols;
+  const uint32_t p0 = split ? wave : 0, step = split ? kReduceWaves : 1;
   const uint32_t mine = parts > p0 ? (parts - p0 + step - 1) / step : 0;  // this wave's pieces: p0 + step * j
-  for (int q = alone ? wave : 0; q < (int)per_group; q += alone ? kReduceWaves : 1) {
-    const int c = c0 + q;
-    if (c >= (int)a.cols || w.col0 + c >= w.n_cols) return;
-    float ms[kChunks], ls[kChunks], o0[kAhead], o1[kAhead];
+  // Running over 16 pieces at a time: m, l and the output, always normalised, so that it stays in the
+  // values' range.
+  float m = -INFINITY, l = 0.f;
+  f32x4 x[NC];
 #pragma unroll
-    for (int k = 0; k < kChunks; ++k) {
-      const uint32_t j = 64 * k + lane;
-      ms[k] = -INFINITY;
-      ls[k] = 0.f;
-      if (j < mine) {
-        const float *ml = a.part_ml + 2 * (slot_of(p0 + step * j) + c);
-        ms[k] = ml[0];
-        ls[k] = ml[1];
-      }
+  for (int k = 0; k < NC; ++k) x[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t j0 = 0; j0 < mine; j0 += 16) {
+    float mp = -INFINITY, lp = 0.f;
+    if (on && j0 + l16 < mine) {
+      const float *ml = a.part_ml + 2 * (slot_of(p0 + step * (j0 + l16)) + c);
+      mp = ml[0];
+      lp = ml[1];
     }
-    auto load = [&](uint32_t j, float &x, float &y) {
-      const float *po = a.part_o + (slot_of(p0 + step * j) + c) * D;
-      x = lane < D ? po[lane] : 0.f;
-      y = lane + 64 < D ? po[lane + 64] : 0.f;
-    };
+    f32x4 y[kAhead][NC];
+    auto load = [&](uint32_t j) {
 #pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j)
-      if (j < mine) load(j, o0[j], o1[j]);
-    auto over_waves = [&](float v, bool is_max) {
-      v = is_max ? wave_max(v) : wave_sum(v);
-      if (alone) return v;
-      __syncthreads();
-      if (lane == 0) scratch[wave] = v;
-      __syncthreads();
-      float x = scratch[0];
-      for (int i = 1; i < kReduceWaves; ++i) x = is_max ? fmaxf(x, scratch[i]) : x + scratch[i];
-      return x;
-    };
-    float mm = ms[0];
+      for (uint32_t i = 0; i < kAhead; ++i)
 #pragma unroll
-    for (int k = 1; k < kChunks; ++k) mm = fmaxf(mm, ms[k]);
-    mm = over_waves(mm, true);
-    const float base = mm == -INFINITY ? 0.f : mm;
-    float ll = 0.f;
-#pragma unroll
-    for (int k = 0; k < kChunks; ++k) {
-      ls[k] *= __builtin_amdgcn_exp2f(ms[k] - base);
-      ll += ls[k];
-    }
-    ll = over_waves(ll, false);
-    const float inv = ll == 0.f ? 0.f : 1.f / ll;
-    float x0 = 0.f, x1 = 0.f;
-#pragma unroll
-    for (int k = 0; k < kChunks; ++k)
-      for (uint32_t j = 64 * k; j < min(mine, 64u * (k + 1)); j += kAhead) {
-        if (j > 0) {
-#pragma unroll
-          for (uint32_t i = 0; i < kAhead; ++i)
-            if (j + i < mine) load(j + i, o0[i], o1[i]);
+        for (int k = 0; k < NC; ++k) {
+          const int d = 64 * k + 4 * l16;
+          y[i][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (on && j + i < mine && d < Dp)
+            y[i][k] = *reinterpret_cast<const f32x4 *>(a.part_o + (slot_of(p0 + step * (j + i)) + c) * Dp + d);
         }
+    };
+    load(j0);
+    float top = mp;
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-          if (j + i >= mine) break;
-          const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ls[k]), (j + i) % 64)) * inv;
-          x0 += f * o0[i];
-          x1 += f * o1[i];
-        }
+    for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new;
+    const float old = __builtin_amdgcn_exp2f(m - base);
+    m = m_new;
+    // (l of a piece, and so its weight, is 0 where it saw nothing, and NaN where that is its sum.)
+    lp *= __builtin_amdgcn_exp2f(mp - base);
+    float sum = lp;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    const float before = l * old;
+    l = before + sum;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    lp *= inv;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) x[k] *= before * inv;
+#pragma unroll
+    for (uint32_t half = 0; half < 2; ++half) {
+      if (half == 1) {
+        if (j0 + kAhead >= mine) break;
+        load(j0 + kAhead);
       }
-    const int h = w.hk * G + (w.col0 + c) % G;
-    const size_t row = w.q0 + (w.col0 + c) / G, out = (row * a.H + h) * D;
-    if (!alone) {
-      if (q > 0) __syncthreads();
-      o_lds[wave][lane] = x0;
-      o_lds[wave][lane + 64] = x1;
-      __syncthreads();
-      x0 = x1 = 0.f;
-      for (int i = 0; i < kReduceWaves; ++i) {
-        x0 += o_lds[i][lane];
-        x1 += o_lds[i][lane + 64];
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; ++i) {
+        const float f = __shfl(lp, (lane & 48) + (int)(half * kAhead + i), 64);
+#pragma unroll
+        for (int k = 0; k < NC; ++k) x[k] += f * y[i][k];
       }
-    }
-    if (alone || wave == 0) {
-      if (lane < D) store_act(a.out, out + lane, x0, bf16);
-      if (lane + 64 < D) store_act(a.out, out + lane + 64, x1, bf16);
-      if (lane == 0 && a.lse) a.lse[(size_t)h * a.n_tokens + row] = (mm + __builtin_log2f(ll)) * kLn2;
     }
   }
+  if (split) {
+    if (l16 == 0) {
+      ml_lds[wave][lane >> 4][0] = m;
+      ml_lds[wave][lane >> 4][1] = l;
+    }
+#pragma unroll
+    for (int k = 0; k < NC; ++k) o_lds[wave][k][lane] = x[k];
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int v = 1; v < kReduceWaves; ++v) m = fmaxf(m, ml_lds[v][lane >> 4][0]);
+    const float base = m == -INFINITY ? 0.f : m;
+    float f[kReduceWaves];
+    l = 0.f;
+#pragma unroll
+    for (int v = 0; v < kReduceWaves; ++v) {
+      f[v] = ml_lds[v][lane >> 4][1] * __builtin_amdgcn_exp2f(ml_lds[v][lane >> 4][0] - base);
+      l += f[v];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      x[k] *= f[0] * inv;  // (wave 0's own)
+#pragma unroll
+      for (int v = 1; v < kReduceWaves; ++v) x[k] += o_lds[v][k][lane] * (f[v] * inv);
+    }
+  }
+  if (!on) return;
+  const int h = w.hk * G + (w.col0 + c) % G;
+  const size_t row = w.q0 + (w.col0 + c) / G, out = (row * a.H + h) * D;
+#pragma unroll
+  for (int k = 0; k < NC; ++k) {
+    const int d = 64 * k + 4 * l16;
+    if (d < D) store_out(a, out + d, D - d, x[k], bf16);
+  }
+  if (l16 == 0 && a.lse) a.lse[(size_t)h * a.n_tokens + row] = (m + __builtin_log2f(l)) * kLn2;
 }
 
 // How a call is cut: columns (query tokens times heads of a kv head) by 16 or 32 (64
@@ -707,7 +747,7 @@ Cut cut_of(uint32_t n_requests, uint32_t max_q, uint32_t max_len, uint32_t n_hea
   // As many workgroups as run at a time.
   c.parts = std::max(1u, kCus * kResident / n_kv_heads);
   const uint64_t slots = 2ull * c.parts * n_kv_heads * c.cols;
-  c.part_bytes = slots * d_head * sizeof(float);
+  c.part_bytes = slots * padded((int)d_head) * sizeof(float);
   c.bytes = c.part_bytes + slots * 2 * sizeof(float) + (pairs + 1) * sizeof(uint32_t);
   return c;
 }
@@ -818,6 +858,7 @@ int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool, 
   a.scale = scale;
   a.causal = causal != 0;
   a.q_vec = d_head % 4 == 0 && q_row_stride % 4 == 0 && aligned_to(q, 4 * item);
+  a.out_vec = d_head % 4 == 0 && aligned_to(out, 4 * item);
   const uint64_t tiles = (uint64_t)n_requests * n_kv_heads * c.q_tiles;
   const uint64_t reductions = tiles * ((c.cols + reduce_cols(c.cols) - 1) / reduce_cols(c.cols));
   if (reductions >= (1ull << 31))
@@ -834,8 +875,12 @@ int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool, 
     launch_shape<false, 2>(a, c.qt, s);
   st = launched(fn);
   if (st != DFATTN_OK || c.parts == 0) return st;
-  hipLaunchKernelGGL(attention_reduce_kernel, linear_grid(reductions), dim3(64 * kReduceWaves), 0, s, a,
-                     (int)(16 * c.qt), bf16);
+  if (d_head <= 64)
+    hipLaunchKernelGGL(attention_reduce_kernel<1>, linear_grid(reductions), dim3(64 * kReduceWaves), 0, s, a,
+                       (int)(16 * c.qt), bf16);
+  else
+    hipLaunchKernelGGL(attention_reduce_kernel<2>, linear_grid(reductions), dim3(64 * kReduceWaves), 0, s, a,
+                       (int)(16 * c.qt), bf16);
   return launched(fn);
 }
 
