@@ -230,14 +230,15 @@ struct Look {
 // share it), 16 rows of the page and 64 columns at a time: lane 4 i + j holds columns
 // 4 i .. of rows j, 4 + j, 8 + j and 12 + j. V's codes are transposed within four
 // lanes, so that each has 16 rows of one column, which lie together. The rows are read
-// twice, the second time from the caches (with two groups' loads on their way at a time,
-// 130 to 250 registers, 8000 tokens took 31 us for 22).
-// Measured: 40 single rows (12 heads of 64, fp32) 5.5 us, a launch's latency; 8197
-// tokens of four prompts (8 heads of 128, bf16) 28-32 us for 50 MB, where a wave's two
-// passes, one behind the other, are what it waits for; 8000 tokens (12 of 64, fp32) 22 us
-// for 61 MB.
+// once to look and, but for the last 16, once more from the caches to write (two
+// groups' loads on their way at a time need 130 to 250 registers: 8000 tokens 31 us for 22).
+// Measured: 40 single rows (12 heads of 64, fp32) 5.6 us, a launch's latency; 8197
+// tokens of four prompts (8 heads of 128, bf16) 27 us for 50 MB, where each wave waits
+// for its slots, its rows and its stores one after the other; 8000 tokens (12 of 64, fp32)
+// 19 us for 61 MB. (128 registers at most for 64 columns: 19 us for 22; for 128 columns
+// they spill, 38 us for 27.)
 template <bool E4M3, bool BF16, bool WIDE, bool SPLIT, bool VEC>
-__global__ __launch_bounds__(64 * kAppendWaves) void append_kernel(CacheArgs a, uint32_t phases) {
+__global__ __launch_bounds__(64 * kAppendWaves, WIDE ? 3 : 4) void append_kernel(CacheArgs a, uint32_t phases) {
   constexpr int kHalves = WIDE ? 2 : 1;
   __shared__ float amax_lds[kAppendWaves], odd_lds[kAppendWaves];
   const size_t i0 = (size_t)linear_block() * kWindow;
@@ -357,8 +358,10 @@ __global__ __launch_bounds__(64 * kAppendWaves) void append_kernel(CacheArgs a, 
 #pragma unroll
           for (int half = 0; half < kHalves; ++half) look.at(x[j][half].value());
       };
-      for (int m = m0; m <= m1; m += step) {
-        Quad<BF16, VEC> x[4][kHalves];
+      Quad<BF16, VEC> x[4][kHalves];
+      int m = m0 - step;
+      while (m + step <= m1) {
+        m += step;
         load(m, x);
         look_at(x);
       }
@@ -422,10 +425,10 @@ __global__ __launch_bounds__(64 * kAppendWaves) void append_kernel(CacheArgs a, 
           }
         }
       };
-      for (int m = m0; m <= m1; m += step) {
-        Quad<BF16, VEC> x[4][kHalves];
-        load(m, x);
+      while (m >= m0) {
         put(m, x);
+        m -= step;
+        if (m >= m0) load(m, x);
       }
     }
   }
