@@ -475,8 +475,11 @@ int dfgpt2_token_logprobs_backward(const void *logits, const uint32_t *tokens, c
   if (st == DFATTN_OK) st = need(fn, {tokens, stats, entropy}, 4);
   if (st == DFATTN_OK) st = optional(fn, {grad_logprob, grad_entropy});
   if (st != DFATTN_OK) return st;
-  if (logits == grad_logits && row_stride != cols)
-    return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": grad_logits may be logits only where row_stride is cols");
+  const size_t item = dtype == DFATTN_KV_F32 ? 4 : 2;
+  const char *x = static_cast<const char *>(logits), *g = static_cast<const char *>(grad_logits);
+  const bool overlap = x < g + (size_t)rows * cols * item && g < x + ((size_t)(rows - 1) * row_stride + cols) * item;
+  if (overlap && (x != g || row_stride != cols))
+    return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": grad_logits may overlap logits only as the same rows");
   GradArgs a{logits, tokens, stats, entropy, grad_logprob, grad_entropy, grad_logits, row_stride, (int)cols};
   const bool bf16 = dtype == DFATTN_KV_BF16;
   const uint32_t part = 256 * kGradSteps * (bf16 ? kPer<true> : kPer<false>);

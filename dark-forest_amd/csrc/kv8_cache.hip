@@ -544,9 +544,9 @@ int dfattn_paged_plan(const uint32_t *cached_lens, const uint32_t *new_lens, con
         return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": outputs must not overlap inputs or each other");
   PlanArgs a{cached_lens, new_lens, free_pages, free_start, block_table, seq_lens, query_start, slot_map, counts,
              n_free, n_requests, max_pages, token_capacity, page_size, n_pages};
-  // Four tokens a thread, up to two workgroups a CU.
+  // A token a thread, up to two workgroups a CU.
   const uint32_t work = std::max(token_capacity, n_requests + 1);
-  const uint32_t grid = std::min(512u, (work + 4 * kPlanThreads - 1) / (4 * kPlanThreads));
+  const uint32_t grid = std::min(512u, (work + kPlanThreads - 1) / kPlanThreads);
   const size_t lds = 2 * (size_t)(n_requests + 1) * sizeof(uint32_t);
   hipLaunchKernelGGL(plan_kernel, dim3(grid), dim3(kPlanThreads), lds, static_cast<hipStream_t>(stream), a);
   return launched(fn);

@@ -140,7 +140,8 @@ def backward(ptrs=None, dtype=0, rows=4, cols=100, stride=None):
 @pytest.mark.parametrize("kw,status", [
     (dict(dtype=2), FLAGS), (dict(cols=0), SHAPE), (dict(stride=99), SHAPE), (dict(rows=(1 << 21) + 1), OVER),
     *[(dict(ptrs={i: None}), NULL) for i in (0, 1, 2, 3, 6)], *[(dict(ptrs={i: ODD}), MIS) for i in range(7)],
-    (dict(ptrs={6: P}, stride=104), SHAPE), (dict(rows=0), 0),
+    (dict(ptrs={6: P}, stride=104), SHAPE), (dict(rows=0), 0), (dict(ptrs={6: ctypes.c_void_p(0x10004)}), SHAPE),
+    (dict(ptrs={6: ctypes.c_void_p(0x10000 + 4 * (4 * 100 - 1))}), SHAPE),
 ])
 def test_token_logprobs_backward(kw, status):
     expect(status, "dfgpt2_token_logprobs_backward", backward(**kw))
