@@ -325,6 +325,7 @@ def token_logprobs(logits, tokens, top_k=0):
                 return logprob, entropy, ids, top
 
             @staticmethod
+            @torch.autograd.function.once_differentiable
             def backward(ctx, g_logprob, g_entropy, _ids, _top):
                 if g_logprob is None and g_entropy is None:
                     return None, None, None

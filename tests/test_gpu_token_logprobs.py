@@ -267,6 +267,39 @@ def test_autograd_against_differences(device):
     assert b.grad.dtype == torch.bfloat16
 
 
+def test_a_second_derivative_is_refused(device):
+    x = torch.randn(2, 30, device=device, requires_grad=True)
+    lp = ops.token_logprobs(x, torch.zeros(2, dtype=torch.int32, device=device))[0]
+    (g,) = torch.autograd.grad(lp.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.square().sum(), x)
+
+
+@pytest.mark.parametrize("n", [16384, 16385])
+def test_many_rows_at_once(device, n):
+    """More rows than run at a time, of both sides of the size where a row gets more threads."""
+    g = torch.Generator().manual_seed(n)
+    x = (torch.randn(16, n, generator=g) * 2).bfloat16()
+    tokens = torch.randint(0, n, (16,), generator=g)
+    _, got, _ = check(x, tokens, 20, device)
+    many = ops.token_logprobs_forward(x.to(device).repeat(160, 1), tokens.int().to(device).repeat(160), 20)
+    for a, b in zip(many, got):
+        assert torch.equal(a, b.repeat(160, *[1] * (b.dim() - 1)))
+
+
+def test_two_streams_at_once(device):
+    sets = [(torch.randn(300, 5001, device=device), torch.randint(0, 5001, (300,), device=device).int()) for _ in range(2)]
+    want = [ops.token_logprobs_forward(x, t, 7) for x, t in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], []
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((ops.token_logprobs_forward(*sets[i], 7), want[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g, w in got for a, b in zip(g, w))
+
+
 def test_replayed_from_a_graph(device):
     x = torch.randn(40, 3001, device=device)
     t = torch.randint(0, 3001, (40,), device=device).int()
