@@ -176,7 +176,7 @@ __device__ __forceinline__ unsigned transpose4(unsigned x, int lane) {
 }
 
 constexpr int kAppendWaves = 4, kWindow = 48;
-constexpr uint32_t kAppendGroups = 2048, kFewTokens = 1024;
+constexpr uint32_t kAppendGroups = 1024, kFewTokens = 1024;
 
 // One side (K or V) of one page and head: its scale, and its codes.
 template <bool E4M3>
@@ -233,10 +233,10 @@ struct Look {
 // once to look and, but for the last 16, once more from the caches to write (two
 // groups' loads on their way at a time need 130 to 250 registers: 8000 tokens 31 us for 22).
 // Measured: 40 single rows (12 heads of 64, fp32) 5.6 us, a launch's latency; 8197
-// tokens of four prompts (8 heads of 128, bf16) 27 us for 50 MB, where each wave waits
+// tokens of four prompts (8 heads of 128, bf16) 26 us for 50 MB, where each wave waits
 // for its slots, its rows and its stores one after the other; 8000 tokens (12 of 64, fp32)
-// 19 us for 61 MB. (128 registers at most for 64 columns: 19 us for 22; for 128 columns
-// they spill, 38 us for 27.)
+// 18 us for 61 MB. (128 registers at most for 64 columns: 19 us for 22, 96 spill, 36 us; for
+// 128 columns 128 spill, 38 us for 27.)
 template <bool E4M3, bool BF16, bool WIDE, bool SPLIT, bool VEC>
 __global__ __launch_bounds__(64 * kAppendWaves, WIDE ? 3 : 4) void append_kernel(CacheArgs a, uint32_t phases) {
   constexpr int kHalves = WIDE ? 2 : 1;
@@ -592,9 +592,9 @@ int dfattn_kv8_append(const void *k, const void *v, const uint32_t *slot_map, vo
   a.n_pages = (int)n_pages;
   const size_t four = act_dtype == DFATTN_KV_F32 ? 16 : 8;
   a.vec = d_head % 4 == 0 && row_stride % 4 == 0 && aligned_to(k, four) && aligned_to(v, four);
-  // About kAppendGroups workgroups (250 to 300 a us start, empty or not: 8000 for a
-  // prompt of 8197 tokens took 30 us for that alone): a window's runs are dealt to several
-  // while there are fewer.
+  // About kAppendGroups workgroups: 250 to 300 a us start, empty or not (8000 of them for a
+  // prompt of 8197 tokens took 30 us for that alone; 2048 took 19 us for 1000 single rows, 1024 take
+  // 13.5). A window's runs are dealt to several while there are fewer.
   const bool wide = d_head > 64, split = page_size >= 64;
   const uint32_t windows = (n_tokens + kWindow - 1) / kWindow;
   // The heads' sides that a workgroup takes at once: few tokens are taken to be runs of one
