@@ -402,7 +402,8 @@ int dfattn_kv8_append(const void *k, const void *v, const uint32_t *slot_map, vo
 
 /* Read back: rows k_out[i], v_out[i] [n_rows, n_kv_heads*d_head] := the values
  * code * scale of slots[i], in act_dtype; zeros where the slot is not in the
- * pool. Slots in any order, any number of times.                             */
+ * pool. Slots in any order, any number of times. Outputs must not overlap what
+ * is read.                                                                   */
 int dfattn_kv8_read(const void *k_pool, const void *v_pool, const float *k_scales,
                     const float *v_scales, const uint32_t *slots, void *k_out, void *v_out,
                     uint32_t act_dtype, uint32_t kv_dtype, uint32_t n_rows,
@@ -417,10 +418,12 @@ int dfattn_kv8_read(const void *k_pool, const void *v_pool, const float *k_scale
  * [n_heads, n_tokens] (may be NULL): natural log of the sum of exp(scale q k).
  * A row that sees nothing gets zeros and -infinity. Rows from
  * query_start[R] on are left as they are. Keys in a page whose id is not below
- * n_pages are left out; a table entry past a request's length is not read.
- * max_query_len and max_seq_len are bounds the caller knows of the lengths on
- * the device; queries past max_query_len are not computed, a longer sequence
- * only costs time. Softmax statistics and sums are fp32; with fp32 activations
+ * n_pages are left out; a table entry past a request's length is not read, and
+ * a length past the table's row counts as its end. max_query_len and
+ * max_seq_len are bounds the caller knows of the lengths on the device; queries
+ * past max_query_len are not computed, a longer sequence only costs time.
+ * n_requests <= 65535, max_pages * page_size <= 2^30, n_tokens <= 2^30; out and
+ * lse must not overlap what is read. Softmax statistics and sums are fp32; with fp32 activations
  * q and P enter the matrix products as two fp16 terms (22 bits), with bf16
  * as one (12 bits at least). |scale q| must stay below fp32's range over 2^16.
  * Workspace: dfattn_kv8_attention_workspace_bytes of the same sizes (0: none
