@@ -781,12 +781,17 @@ using namespace dfattn::kv8;
 
 extern "C" {
 
+// A request's columns (queries times heads of a kv head) are counted in 32 bits.
+static bool too_many_columns(uint32_t n_tokens, uint32_t max_query_len, uint32_t group) {
+  return (uint64_t)std::min(max_query_len, n_tokens) * group > (1ull << 30);
+}
+
 size_t dfattn_kv8_attention_workspace_bytes(uint32_t n_requests, uint32_t n_tokens, uint32_t max_query_len,
                                             uint32_t max_seq_len, uint32_t n_heads, uint32_t n_kv_heads,
                                             uint32_t d_head) {
   if (n_requests == 0 || n_tokens == 0 || max_query_len == 0 || n_kv_heads == 0 || n_heads == 0 ||
       n_heads % n_kv_heads != 0 || n_heads > 65535u || n_requests > 65535u || n_tokens > (1u << 30) || d_head == 0 ||
-      d_head > 128)
+      d_head > 128 || too_many_columns(n_tokens, max_query_len, n_heads / n_kv_heads))
     return 0;
   return cut_of(n_requests, std::min(max_query_len, n_tokens), max_seq_len, n_heads, n_kv_heads, d_head).bytes;
 }
@@ -807,7 +812,8 @@ int dfattn_kv8_attention(const void *q, const void *k_pool, const void *v_pool, 
   if (max_pages == 0) return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": max_pages must be >= 1");
   if (q_row_stride < (uint64_t)n_heads * d_head)
     return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": q_row_stride must be at least n_heads * d_head");
-  if (n_heads > 65535u || n_requests > 65535u || n_tokens > (1u << 30) || (uint64_t)max_pages * page_size > (1ull << 30))
+  if (n_heads > 65535u || n_requests > 65535u || n_tokens > (1u << 30) ||
+      (uint64_t)max_pages * page_size > (1ull << 30) || too_many_columns(n_tokens, max_query_len, n_heads / n_kv_heads))
     return record_error(DFATTN_ERR_OVERFLOW, std::string(fn) + ": shape is too large");
   if (n_requests == 0 || n_tokens == 0 || max_query_len == 0) return DFATTN_OK;
   st = check_all(fn, {q, out}, act_dtype == DFATTN_KV_F32 ? 4 : 2);

@@ -108,10 +108,16 @@ def _cache(cache, d_head, n):
              _ptr(vs, "v scales", n[2], dev)), KV_I8 if dtype is n[4] else KV_E4M3, heads, page, pages)
 
 
+def _check_stream(stream, dev):
+    if stream is not None and stream.device_index != dev:
+        raise ValueError("the stream is not on the current device")
+
+
 class _On:
     """Allocations under `stream` where one is given (memory then belongs to it)."""
 
-    def __init__(self, stream):
+    def __init__(self, stream, dev):
+        _check_stream(stream, dev)
         self.c = None if stream is None else _torch().cuda.stream(stream)
 
     def __enter__(self):
@@ -138,7 +144,7 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, free_start, page_
     r = cached_lens.numel()
     if block_table.dim() != 2 or block_table.shape[0] != r or new_lens.numel() != r or free_start.numel() != 1:
         raise ValueError("cached_lens and new_lens are [R], block_table [R, max_pages], free_start [1]")
-    with _On(stream):
+    with _On(stream, dev):
         on = cached_lens.device
         if seq_lens is None and query_start is None and slot_map is None and counts is None:
             # One allocation in four parts (4.5 us instead of 6.5).
@@ -170,6 +176,7 @@ def kv8_append(cache, k, v, slot_map, stream=None):
     """dfattn_kv8_append: rows k, v [n, kv heads * d_head] (float32 or bfloat16; one row stride, so column blocks
     of a fused projection will do) into the slots slot_map [n] of `cache`."""
     names = _names()
+    _check_stream(stream, names[6])
     n, dm = k.shape
     if dm % cache[0].shape[1]:
         raise ValueError("k and v must be [n, kv heads * d_head]")
@@ -194,7 +201,7 @@ def kv8_read(cache, slots, d_head, dtype=None, k_out=None, v_out=None, stream=No
         dtype = names[2] if k_out is None else k_out.dtype
     if dtype is not names[2] and dtype is not names[3]:
         raise ValueError("values are read as float32 or bfloat16")
-    with _On(stream):
+    with _On(stream, dev):
         if k_out is None:
             k_out = names[0].empty(shape, dtype=dtype, device=slots.device)
         if v_out is None:
@@ -230,7 +237,7 @@ def kv8_attention(cache, q, block_table, query_start, seq_lens, n_heads, max_que
     if block_table.dim() != 2 or block_table.shape[0] != r or query_start.numel() != r + 1:
         raise ValueError("seq_lens is [R], query_start [R+1], block_table [R, max_pages]")
     pq, sq, act = _rows(q, "q", dm, names)
-    with _On(stream):
+    with _On(stream, dev):
         if out is None:
             out = empty((n, dm), dtype=q.dtype, device=q.device)
         if lse is None:

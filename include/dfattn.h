@@ -422,8 +422,8 @@ int dfattn_kv8_read(const void *k_pool, const void *v_pool, const float *k_scale
  * a length past the table's row counts as its end. max_query_len and
  * max_seq_len are bounds the caller knows of the lengths on the device; queries
  * past max_query_len are not computed, a longer sequence only costs time.
- * n_requests <= 65535, max_pages * page_size <= 2^30, n_tokens <= 2^30; out and
- * lse must not overlap what is read. Softmax statistics and sums are fp32; with fp32 activations
+ * n_requests <= 65535; max_pages * page_size, n_tokens and max_query_len *
+ * (n_heads / n_kv_heads) <= 2^30; out and lse must not overlap what is read. Softmax statistics and sums are fp32; with fp32 activations
  * q and P enter the matrix products as two fp16 terms (22 bits), with bf16
  * as one (12 bits at least). |scale q| must stay below fp32's range over 2^16.
  * Workspace: dfattn_kv8_attention_workspace_bytes of the same sizes (0: none

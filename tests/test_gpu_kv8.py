@@ -724,3 +724,18 @@ def test_wrapper_refusals(device):
     with pytest.raises(dfattn.DfattnError):
         dfattn.kv8_attention(cache, torch.zeros(3, 3 * 64, device=device), i32([[0]], device), i32([0, 3], device),
                              i32([3], device), 3, 3, 3)
+
+
+def test_a_stream_of_another_device_is_refused(device):
+    class Elsewhere:
+        device_index, cuda_stream = torch.cuda.current_device() + 1, 0
+
+    cache = dfattn.kv8_cache(2, 2, 64, 16, device=device)
+    x, slots, start = torch.zeros(1, 128, device=device), i32([0], device), i32([0, 1], device)
+    table, one = i32([[0, 1]], device), i32([1], device)
+    for call in (lambda: dfattn.kv8_append(cache, x, x, slots, stream=Elsewhere),
+                 lambda: dfattn.kv8_read(cache, slots, 64, stream=Elsewhere),
+                 lambda: dfattn.kv8_attention(cache, x, table, start, one, 2, 1, 1, stream=Elsewhere),
+                 lambda: dfattn.paged_plan(one, one, table, slots, slots, 16, 2, 4, stream=Elsewhere)):
+        with pytest.raises(ValueError):
+            call()

@@ -91,6 +91,7 @@ def attention(ptrs=None, act=0, kv=2, r=3, n=3, max_q=1, max_len=5000, heads=4, 
     (dict(heads=0), SHAPE), (dict(heads=3), SHAPE), (dict(width=0), SHAPE), (dict(stride=255), SHAPE),
     (dict(heads=65538, hk=2), OVER), (dict(r=65536), OVER), (dict(n=(1 << 30) + 1), OVER), (dict(width=1 << 28), OVER),
     (dict(r=60000, n=1 << 30, max_q=1 << 30), OVER), (dict(ws=P, ws_bytes=4), WORK), (dict(ws=ODD, ws_bytes=1 << 30), WORK),
+    (dict(n=1 << 26, max_q=1 << 26, heads=34), OVER),  # 17 * 2^26 columns
     (dict(r=0), 0), (dict(n=0), 0), (dict(max_q=0), 0),
 ])
 def test_attention(kw, status):
@@ -107,6 +108,7 @@ def test_sizes():
     assert size(1, 1, 1, 64, 12, 12, 64) == 0            # one short row: nothing to split
     assert size(1, 1, 1, 100000, 12, 12, 64) > 0
     assert size(0, 1, 1, 100000, 12, 12, 64) == 0 and size(1, 1, 1, 100000, 12, 5, 64) == 0
+    assert size(1, 1 << 26, 1 << 26, 100000, 34, 2, 64) == 0
     with pytest.raises(ValueError):
         dfattn.kv8_cache(2, 2, 64, 17, device="cpu")
     with pytest.raises(ValueError):
