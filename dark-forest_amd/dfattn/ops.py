@@ -266,25 +266,36 @@ def _beside(t, *others):
             raise ValueError("the tensors must be on the current device")
 
 
-def token_logprobs_forward(logits, tokens, top_k=0):
+def _logprob_outputs(logits, rows, top_k, together):
+    """(logprob, entropy, stats, ids, top) to be written; `together`: in one allocation (5.5 us instead of 8), which
+    autograd, counting the changes of a whole allocation, must not keep parts of."""
+    torch = _torch()
+    empty, f32, i32, dev = torch.empty, torch.float32, torch.int32, logits.device
+    if together:
+        n = rows * top_k
+        whole = empty((4 * rows + 2 * n,), dtype=f32, device=dev)
+        logprob, entropy, stats, ids, top = whole.split_with_sizes([rows, rows, 2 * rows, n, n])
+        return logprob, entropy, stats.view(rows, 2), ids.view(i32).view(rows, top_k), top.view(rows, top_k)
+    return (empty((rows,), dtype=f32, device=dev), empty((rows,), dtype=f32, device=dev),
+            empty((rows, 2), dtype=f32, device=dev), empty((rows, top_k), dtype=i32, device=dev),
+            empty((rows, top_k), dtype=f32, device=dev))
+
+
+def token_logprobs_forward(logits, tokens, top_k=0, _together=True):
     """dfgpt2_token_logprobs over logits [rows, V] (float32 or bfloat16, rows may be a column block of a wider
     tensor) and int32 tokens [rows]. Returns (logprob [rows], entropy [rows], stats [rows, 2], top_ids [rows, top_k] int32,
-    top_logprobs [rows, top_k]); stats holds each row's maximum and ln sum exp(x - maximum)."""
-    torch = _torch()
+    top_logprobs [rows, top_k]), parts of one allocation; stats holds each row's maximum and ln sum exp(x - maximum)."""
     rows, v, p, stride, dtype = _logit_rows(logits)
     _beside(logits, tokens)
     if tokens.shape != (rows,):
         raise ValueError("tokens must be [rows]")
-    empty, f32, dev = torch.empty, torch.float32, logits.device
-    logprob = empty((rows,), dtype=f32, device=dev)
-    entropy = empty((rows,), dtype=f32, device=dev)
-    stats = empty((rows, 2), dtype=f32, device=dev)
-    ids = empty((rows, top_k), dtype=torch.int32, device=dev)
-    top = empty((rows, top_k), dtype=f32, device=dev)
+    if top_k < 0:
+        raise ValueError("top_k must be at least 0")
+    out = logprob, entropy, stats, ids, top = _logprob_outputs(logits, rows, top_k, _together)
     _check(ops_lib().dfgpt2_token_logprobs(p, _ids_ptr(tokens), logprob.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
                                            ids.data_ptr(), top.data_ptr(), dtype, rows, v, stride, top_k,
                                            _stream_ptr()))
-    return logprob, entropy, stats, ids, top
+    return out
 
 
 def token_logprobs_backward(logits, tokens, stats, entropy, grad_logprob=None, grad_entropy=None, out=None):
@@ -318,7 +329,7 @@ def token_logprobs(logits, tokens, top_k=0):
         class _Fn(torch.autograd.Function):
             @staticmethod
             def forward(ctx, logits, tokens, top_k):
-                logprob, entropy, stats, ids, top = token_logprobs_forward(logits, tokens, top_k)
+                logprob, entropy, stats, ids, top = token_logprobs_forward(logits, tokens, top_k, _together=False)
                 ctx.save_for_backward(logits, tokens, stats, entropy)
                 ctx.mark_non_differentiable(ids, top)
                 ctx.set_materialize_grads(False)
