@@ -183,18 +183,17 @@ template <bool E4M3>
 struct Side {
   unsigned char *codes;
   float s, inv, ratio;
-  bool dead;  // poisoned: zeros, times NaN
-  // From the largest magnitude of the new rows, whether they hold an infinity or a
-  // NaN, and the scale of the rows that are kept (0: none).
-  __device__ __forceinline__ void scale(float amax, bool odd, float old) {
-    s = fmaxf(old, pow2_scale<E4M3>(amax));
-    dead = odd || old != old;
+  // From the bits of the new rows' largest magnitude (an infinity or a NaN is above all
+  // numbers) and the scale of the rows that are kept (0: none). With such a row, or after
+  // one, the scale is NaN, and with it every value, whatever its code.
+  __device__ __forceinline__ void scale(unsigned top, float old) {
+    s = fmaxf(old, pow2_scale<E4M3>(__uint_as_float(top)));
+    const bool dead = top >= 0x7f800000u || old != old;
     if (dead) s = __builtin_nanf("");
     inv = dead ? 0.f : 1.f / s;
     ratio = dead ? 0.f : old * inv;
   }
   __device__ __forceinline__ unsigned encode(float4 v) const {
-    if (dead) v = make_float4(0.f, 0.f, 0.f, 0.f);
     return encode4<E4M3>(make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
   }
   // The rows before `off`, to the new scale, by `lanes` lanes of which this is `lane`: row
@@ -211,13 +210,37 @@ struct Side {
   }
 };
 
+// The largest magnitude of values as they lie in memory: without their signs floats are in
+// the order of their bits.
+template <bool BF16>
 struct Look {
-  float amax = 0.f, odd = 0.f;
-  __device__ __forceinline__ void at(float4 v) {
-    amax = fmaxf(fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-    odd += (v.x - v.x) + (v.y - v.y) + (v.z - v.z) + (v.w - v.w);  // 0, or NaN
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  unsigned top = 0, pair = 0;  // (pair: two of bf16)
+  template <bool VEC>
+  __device__ __forceinline__ void at(const Quad<BF16, VEC> &q) {
+    if constexpr (BF16) {
+      auto more = [&](unsigned x) {
+        pair = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, pair),
+                                                                      __builtin_bit_cast(u16x2, x & 0x7fff7fffu)));
+      };
+      more(q.r.x);
+      more(q.r.y);
+    } else {
+      auto more = [&](float x) { top = max(top, __float_as_uint(x) & 0x7fffffffu); };
+      more(q.r.x);
+      more(q.r.y);
+      more(q.r.z);
+      more(q.r.w);
+    }
   }
+  __device__ __forceinline__ unsigned bits() const { return BF16 ? max(pair << 16, pair & 0xffff0000u) : top; }
 };
+
+// The largest of a wave's bits.
+__device__ __forceinline__ unsigned wave_top(unsigned x) {
+  const float m = wave_max(__uint_as_float(min(x, 0x7f7fffffu)));
+  return __any(x >= 0x7f800000u) ? 0x7f800000u : __float_as_uint(m);
+}
 
 // The append goes by runs, the consecutive rows of one page. A workgroup finds those
 // that start among kWindow tokens (their slots and the next ones are one load) and
@@ -240,7 +263,7 @@ struct Look {
 template <bool E4M3, bool BF16, bool WIDE, bool SPLIT, bool VEC>
 __global__ __launch_bounds__(64 * kAppendWaves, WIDE ? 3 : 4) void append_kernel(CacheArgs a, uint32_t phases) {
   constexpr int kHalves = WIDE ? 2 : 1;
-  __shared__ float amax_lds[kAppendWaves], odd_lds[kAppendWaves];
+  __shared__ unsigned top_lds[kAppendWaves];
   const size_t i0 = (size_t)linear_block() * kWindow;
   if (i0 >= a.n) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane & 3, P = a.P, D = a.D, Dp = padded(D);
@@ -288,16 +311,14 @@ __global__ __launch_bounds__(64 * kAppendWaves, WIDE ? 3 : 4) void append_kernel
         x.clear();
         if (on && d < D)
           x.load(static_cast<const char *>(is_v ? a.v : a.k) + i * row_bytes, (uint32_t)(head_no * D + d), D - d);
-        Look look;
-        look.at(x.value());
+        Look<BF16> look;
+        look.at(x);
+        unsigned top = look.bits();
 #pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) {
-          look.amax = fmaxf(look.amax, __shfl_xor(look.amax, o, 64));
-          look.odd += __shfl_xor(look.odd, o, 64);
-        }
+        for (int o = 1; o < kLanes; o <<= 1) top = max(top, (unsigned)__shfl_xor((int)top, o, 64));
         Side<E4M3> side;
         side.codes = (is_v ? a.v_pool : a.k_pool) + head * (size_t)(P * Dp);
-        side.scale(look.amax, look.odd != 0.f, old);
+        side.scale(top, old);
         if (!on) continue;
         if (d == 0) *scale = side.s;
         if (off > 0 && side.ratio != 1.f) side.recode(is_v, off, P, D, lane % kLanes, kLanes);
@@ -351,12 +372,12 @@ __global__ __launch_bounds__(64 * kAppendWaves, WIDE ? 3 : 4) void append_kernel
           }
         }
       };
-      Look look;
+      Look<BF16> look;
       auto look_at = [&](const Quad<BF16, VEC> (&x)[4][kHalves]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int half = 0; half < kHalves; ++half) look.at(x[j][half].value());
+          for (int half = 0; half < kHalves; ++half) look.at(x[j][half]);
       };
       Quad<BF16, VEC> x[4][kHalves];
       int m = m0 - step;
@@ -365,24 +386,17 @@ __global__ __launch_bounds__(64 * kAppendWaves, WIDE ? 3 : 4) void append_kernel
         load(m, x);
         look_at(x);
       }
-      float amax = wave_max(look.amax);
-      bool odd = __any(look.odd != 0.f);
+      unsigned top = wave_top(look.bits());
       if constexpr (SPLIT) {
         __syncthreads();  // (the task before has been read)
-        if (lane == 0) {
-          amax_lds[wave] = amax;
-          odd_lds[wave] = odd ? 1.f : 0.f;
-        }
+        if (lane == 0) top_lds[wave] = top;
         __syncthreads();
 #pragma unroll
-        for (int v = 0; v < kAppendWaves; ++v) {
-          amax = fmaxf(amax, amax_lds[v]);
-          odd |= odd_lds[v] != 0.f;
-        }
+        for (int v = 0; v < kAppendWaves; ++v) top = max(top, top_lds[v]);
       }
       Side<E4M3> side;
       side.codes = (is_v ? a.v_pool : a.k_pool) + head * (size_t)(P * Dp);
-      side.scale(amax, odd, old);
+      side.scale(top, old);
       const bool writes = !SPLIT || wave == 0;
       if (writes && lane == 0) *scale = side.s;
       // (V's bytes of the run's first rows may share four with kept ones: the wave that has the
