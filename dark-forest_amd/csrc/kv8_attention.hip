@@ -144,8 +144,9 @@ struct Share {
   __device__ __forceinline__ Share(const uint32_t *before, const AttnArgs &a)
       : total(uniform(before[a.R * a.q_tiles])), per(max((total + a.parts - 1) / a.parts, kMinSteps)) {}
 };
+//
 // One workgroup: 16*QT columns (queries of one kv head) against the keys of one
-// split, 64 keys a wave and step, the waves' results merged at the end.
+// part, 64 keys a wave and step, the waves' results merged at the end.
 //
 // S^T = K Q^T on 16x16x32 tiles: A is K as it lies in memory, lane (m, g) =
 // (l % 16, l / 16) reading 16 bytes of one key, B is Q. Row m of tile t is key
@@ -728,10 +729,15 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
   if (l16 == 0 && a.lse) a.lse[(size_t)h * a.n_tokens + row] = (m + __builtin_log2f(l)) * kLn2;
 }
 
-// How a call is cut: columns (query tokens times heads of a kv head) by 16 or 32 (64
-// spill registers: 3 x 500 queries of 4096 keys 111 us, so 100). The work is shared out where sequences may be longer than kShareFrom keys and
-// the (request, tile) pairs fit LDS; else one workgroup takes each tile.
-constexpr uint32_t kShareFrom = 1024, kMaxPairs = 4096;
+// How a call is cut: columns (query tokens times heads of a kv head) by 16, 32 or 48. 48
+// share each widened code with half as many columns again, where d_head lets them fit
+// registers: 2 x 720 queries of 4096 keys, 12 heads of 64, 76 us, so 84 (bf16 56, so 62);
+// 8 x 64 queries leave a third of them empty, 37 us, so 32; and where the work isn't shared
+// out a second round of workgroups costs more (4 x 512 queries of 512 keys 24 us, so 23).
+// (64 columns spill registers: 3 x 500 queries 79 us, so 61.) The work is shared out where
+// sequences may be longer than kShareFrom keys and the (request, tile) pairs fit LDS; else
+// one workgroup takes each tile.
+constexpr uint32_t kShareFrom = 1024, kMaxPairs = 4096, kManyColumns = 192;
 struct Cut {
   uint32_t qt, cols, q_tiles, parts;  // parts: 0, not shared out
   size_t part_bytes, bytes;
@@ -739,7 +745,9 @@ struct Cut {
 Cut cut_of(uint32_t n_requests, uint32_t max_q, uint32_t max_len, uint32_t n_heads, uint32_t n_kv_heads, uint32_t d_head) {
   Cut c{};
   const uint64_t cols = (uint64_t)max_q * (n_heads / n_kv_heads);
-  c.qt = cols <= 16 ? 1 : 2;
+  const uint64_t tiles = n_requests * ((cols + 47) / 48);  // of 48
+  const bool at_once = max_len > kShareFrom ? tiles <= kMaxPairs : tiles * n_kv_heads <= kCus * kResident;
+  c.qt = cols <= 16 ? 1 : cols >= kManyColumns && d_head <= 64 && at_once ? 3 : 2;
   c.cols = (uint32_t)std::min<uint64_t>(cols, 16 * c.qt);
   c.q_tiles = (uint32_t)((cols + 16 * c.qt - 1) / (16 * c.qt));
   const uint64_t pairs = (uint64_t)n_requests * c.q_tiles;
@@ -765,8 +773,10 @@ template <bool E4M3, int NT>
 void launch_shape(const AttnArgs &a, uint32_t qt, hipStream_t s) {
   if (a.D <= 64 && qt == 1)
     launch<E4M3, NT, 1, 1>(a, s);
-  else if (a.D <= 64)
+  else if (a.D <= 64 && qt == 2)
     launch<E4M3, NT, 1, 2>(a, s);
+  else if (a.D <= 64)
+    launch<E4M3, NT, 1, 3>(a, s);
   else if (qt == 1)
     launch<E4M3, NT, 2, 1>(a, s);
   else

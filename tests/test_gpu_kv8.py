@@ -361,6 +361,11 @@ CUT = [
     ([20000], [20], 2, 1, 32, 16),
     ([1300], [1], 600, 600, 16, 16),                             # more heads than workgroups run at a time
     ([1025, 1024, 0, 513], [3, 0, 2, 513], 1, 1, 80, 48),
+    ([1500, 300, 64], [200, 1, 64], 1, 1, 64, 16),               # many queries of small heads
+    ([2200, 1100], [97, 30], 6, 2, 32, 48),
+    ([4100, 700], [191, 260], 2, 2, 33, 64),
+    ([900, 230], [230, 193], 2, 2, 64, 16),                      # ... of sequences that are not shared out
+    ([260] * 40, [200] + [1] * 38 + [195], 4, 4, 16, 16),        # ... in more tiles than run at once
 ]
 
 
