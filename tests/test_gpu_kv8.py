@@ -386,6 +386,34 @@ def test_attention_of_many_requests(device, r):
     check_attention(device, lens, qlens, 1, 1, 16, 16, "i8", "f32", seed=r)
 
 
+def test_attention_of_many_requests_with_long_bounds(device):
+    """Bounds that allow every request many queries, nearly as many (request, tile) pairs as are shared out."""
+    r = 815
+    lens, qlens = [1 + i % 3 for i in range(r)], [i % 2 for i in range(r)]
+    lens[400], qlens[400] = 1500, 200
+    say("requests", r)
+    check_attention(device, lens, qlens, 1, 1, 16, 16, "i8", "f32", seed=r)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_chunks_replayed_from_a_graph(device, d):
+    """Captured before any call of the kind, replayed with other queries."""
+    heads, lens, qlens = 2, [2100, 300], [230, 41]
+    cache, table, seq, _ = build(device, lens, heads, d, 16, "i8", 50 + d)
+    start = i32([0, 230, 271], device)
+    q = torch.zeros(271, heads * d, device=device)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = dfattn.kv8_attention(cache, q, table, start, seq, heads, 230, 2100)
+    for seed in range(3):
+        q.copy_(torch.randn(271, heads * d, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = dfattn.kv8_attention(cache, q, table, start, seq, heads, 230, 2100)
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+
+
 def test_requests_that_share_pages(device):
     """Two requests with a common prefix in the same pages, each with a last page of its own."""
     heads, d, page, n = 2, 64, 16, 200
