@@ -143,6 +143,9 @@ __device__ __forceinline__ float lane_bound(Shared<kWaves> &sh, float mine, int 
 // (some 30 of 512 threads hold one) are read again for the candidates, and each
 // candidate's rank among them is its place.
 //
+// Measured: 1000 rows of 50257 in fp32 38 us by themselves, 5.2 TB/s; 2048 in bf16 49 us, with 20
+// alternatives 59, where the rows' ends, two rounds of them, leave memory idle. 8 rows 10.5 us: seven
+// batches one after the other.
 // 512 threads a row, 256 where it is short: 8192 rows of 1000 28 us for 16, of 8192 52 for 48; of
 // 4096 rows of 32768 97 for 102, and of 2048 of 50257 (bf16, 20 alternatives) 59 for 67.
 template <bool BF16, bool TOP, int kThreads>
@@ -351,7 +354,8 @@ __device__ __forceinline__ unsigned short to_bf16(float f) {
 // g_j = g_l 1[j = token] - p_j (g_l + g_h (ln p_j + H)), elementwise: bound by
 // memory (a read and a write). 16 bytes a thread and step, from any element's
 // address. Everything a workgroup reads of its part of the row is read before it
-// is written, so the gradient may lie where the logits do.
+// is written, so the gradient may lie where the logits do. 1000 rows of 50257 in fp32 67 us,
+// 6.0 TB/s (after the forward, with part of the logits still in the Infinity Cache).
 constexpr int kGradSteps = 4;
 template <bool BF16>
 __global__ __launch_bounds__(256) void logprob_grad_kernel(GradArgs a) {
