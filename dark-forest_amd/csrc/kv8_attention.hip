@@ -740,10 +740,14 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
 // registers: 2 x 720 queries of 4096 keys, 12 heads of 64, 76 us, so 84 (bf16 56, so 62);
 // 8 x 64 queries leave a third of them empty, 37 us, so 32; and where the work isn't shared
 // out a second round of workgroups costs more (4 x 512 queries of 512 keys 24 us, so 23).
-// (64 columns spill registers: 3 x 500 queries 79 us, so 61.) The work is shared out where
-// sequences may be longer than kShareFrom keys and the (request, tile) pairs fit LDS; else
-// one workgroup takes each tile.
-constexpr uint32_t kShareFrom = 1024, kMaxPairs = 4096, kManyColumns = 192;
+// (64 columns spill registers: 3 x 500 queries 79 us, so 61.)
+//
+// The work is shared out where sequences may be longer than kShareFrom keys (kShareFromFew, up
+// to 16 columns) and the (request, tile) pairs fit LDS; else one workgroup takes each tile and
+// no merge is launched. 64 requests of up to 2048 keys take 39 us shared out, 32 not; one of
+// 1536 11 either way on the GPU, 21 and 16.5 with its calls; but one of 4096 11.6 and 23.6, 32 of up to
+// 4096 33 and 38, and 2 x 200 queries of 2048 keys 25 and 27.
+constexpr uint32_t kShareFrom = 1024, kShareFromFew = 2048, kMaxPairs = 4096, kManyColumns = 192;
 struct Cut {
   uint32_t qt, cols, q_tiles, parts;  // parts: 0, not shared out
   size_t part_bytes, bytes;
@@ -757,7 +761,7 @@ Cut cut_of(uint32_t n_requests, uint32_t max_q, uint32_t max_len, uint32_t n_hea
   c.cols = (uint32_t)std::min<uint64_t>(cols, 16 * c.qt);
   c.q_tiles = (uint32_t)((cols + 16 * c.qt - 1) / (16 * c.qt));
   const uint64_t pairs = (uint64_t)n_requests * c.q_tiles;
-  if (max_len <= kShareFrom || pairs > kMaxPairs) return c;
+  if (max_len <= (c.qt == 1 ? kShareFromFew : kShareFrom) || pairs > kMaxPairs) return c;
   // As many workgroups as run at a time.
   c.parts = std::max(1u, kCus * kResident / n_kv_heads);
   const uint64_t slots = 2ull * c.parts * n_kv_heads * c.cols;

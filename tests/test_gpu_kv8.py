@@ -359,7 +359,10 @@ CUT = [
     ([5000, 2300, 130], [9, 1, 100], 4, 2, 128, 64),
     ([9000], [20], 2, 1, 64, 16),
     ([20000], [20], 2, 1, 32, 16),
-    ([1300], [1], 600, 600, 16, 16),                             # more heads than workgroups run at a time
+    ([1300], [1], 600, 600, 16, 16),
+    ([2100], [1], 600, 600, 16, 16),                             # more heads than workgroups run at a time
+    ([2048, 100], [1, 3], 4, 2, 64, 16),                         # the longest few queries that one workgroup walks
+    ([2049, 100], [1, 3], 4, 2, 64, 16),
     ([1025, 1024, 0, 513], [3, 0, 2, 513], 1, 1, 80, 48),
     ([1500, 300, 64], [200, 1, 64], 1, 1, 64, 16),               # many queries of small heads
     ([2200, 1100], [97, 30], 6, 2, 32, 48),
@@ -377,12 +380,13 @@ def test_attention_cut_between_workgroups(device, case, fmt, act):
     check_attention(device, lens, qlens, heads, kv_heads, d, page, fmt, act, seed=100 + case)
 
 
+@pytest.mark.parametrize("longest", [1500, 2100])
 @pytest.mark.parametrize("r", [4096, 4097])
-def test_attention_of_many_requests(device, r):
+def test_attention_of_many_requests(device, r, longest):
     """The most requests whose work is shared out, and one more, with one long sequence among them."""
     say("requests", r)
     lens, qlens = [1 + i % 3 for i in range(r)], [1 - (i % 7 == 3) for i in range(r)]
-    lens[r // 2] = 1500
+    lens[r // 2] = longest
     check_attention(device, lens, qlens, 1, 1, 16, 16, "i8", "f32", seed=r)
 
 
@@ -691,19 +695,20 @@ def test_serving_loop_replayed_from_a_graph(device):
 
 
 def test_two_graphs_share_a_workspace_in_turn(device):
-    lens = [2000, 900]
+    lens = [2600, 900]
     cache, table, seq, _ = build(device, lens, 4, 64, 16, "i8", 3)
     start = i32([0, 1, 2], device)
-    need = dfattn.kv8_attention_workspace_bytes(2, 2, 1, 2000, 4, 4, 64)
-    ws = torch.empty(max(need, 4) // 4, device=device)
+    need = dfattn.kv8_attention_workspace_bytes(2, 2, 1, 2600, 4, 4, 64)
+    assert need > 0
+    ws = torch.empty(need // 4, device=device)
     qs = [torch.randn(2, 4 * 64, device=device) for _ in range(2)]
-    want = [dfattn.kv8_attention(cache, q, table, start, seq, 4, 1, 2000) for q in qs]
+    want = [dfattn.kv8_attention(cache, q, table, start, seq, 4, 1, 2600) for q in qs]
     graphs, outs = [], []
     for q in qs:
         out, lse = torch.empty_like(q), torch.empty(4, 2, device=device)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
-            dfattn.kv8_attention(cache, q, table, start, seq, 4, 1, 2000, out=out, lse=lse, workspace=ws)
+            dfattn.kv8_attention(cache, q, table, start, seq, 4, 1, 2600, out=out, lse=lse, workspace=ws)
         graphs.append(g)
         outs.append((out, lse))
     for _ in range(3):
