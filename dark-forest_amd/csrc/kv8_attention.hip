@@ -737,7 +737,8 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
 
 // How a call is cut: columns (query tokens times heads of a kv head) by 16, 32 or 48. 48
 // share each widened code with half as many columns again, where d_head lets them fit
-// registers: 2 x 720 queries of 4096 keys, 12 heads of 64, 76 us, so 84 (bf16 56, so 62);
+// registers: 2 x 720 queries of 4096 keys, 12 heads of 64, 76 us, so 84 (bf16 56, so 62), though
+// fewer tiles may share out less evenly: 3 x 500 of 900 to 4096 keys 64 us, so 62;
 // 8 x 64 queries leave a third of them empty, 37 us, so 32; and where the work isn't shared
 // out a second round of workgroups costs more (4 x 512 queries of 512 keys 24 us, so 23).
 // (64 columns spill registers: 3 x 500 queries 79 us, so 61.)
