@@ -65,6 +65,22 @@ __device__ __forceinline__ float column_sum(float v) {
   return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// 2^x, x <= 0 or -infinity, as part * 2^whole with part in (1/2, 1] (0 below 2^-1000): a weight too
+// small for fp32 may still count, where its values are that much larger.
+struct Power {
+  float part, whole;
+  __device__ __forceinline__ explicit Power(float x)
+      : whole(__builtin_ceilf(fmaxf(x, -1000.f))) {
+    part = __builtin_amdgcn_exp2f(x - whole);
+  }
+};
+
+__device__ __forceinline__ f32x4 scaled(f32x4 x, int e) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], e);
+  return x;
+}
+
 // 8 codes (two dwords) as 8 fp16 values, exactly. int8: the code plus 128 as
 // the low byte of 0x6400 is 1024 + 128 + code, which is exact in fp16.
 template <bool E4M3>
@@ -159,8 +175,9 @@ struct Share {
 // q and P enter as NT fp16 terms: q times a power of two that brings its
 // column's largest value to 2^14 .. 2^15; P times the page's scale and 2^(14 -
 // r), where 2^r (r whole) bounds the largest such product so far: m and r move
-// together, so weights keep 2^-39 of the largest one whatever the pages'
-// scales.
+// together, so products keep 2^-39 of the largest one whatever the pages'
+// scales. Powers of two that fp32 has no room for (a weight of 2^-200 before values of
+// 2^120) are kept apart as exponents, here and in the merges.
 //
 // Measured (12 heads of 64): one query on 2 x 131072 keys 60 us, 5.0 TB/s, on 64 requests of up to
 // 4096 (e4m3, bf16) 47 us, 4.4 TB/s: memory, of which two workgroups a CU keep enough on its
@@ -453,22 +470,32 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
       top *= f[t];
       const float m_new = fmaxf(m[t], column_max(top));
       const float base = m_new == -INFINITY ? 0.f : m_new;
-      const float dm = m[t] - base;  // <= 0, -inf at first
-      const float reach = column_max(top - base + __builtin_amdgcn_logf(vs[t]));
-      const float r_new = fmaxf(fmaxf(r[t] + __builtin_ceilf(fmaxf(dm, -1000.f)), __builtin_ceilf(reach)), -300.f);
+      const Power dm(m[t] - base);
+      const float lv = __builtin_amdgcn_logf(vs[t]), reach = column_max(top - base + lv);
+      const float r_new = fmaxf(fmaxf(r[t] + dm.whole, __builtin_ceilf(reach)), -300.f);
       if (__any(m_new != m[t] || r_new != r[t])) {
-        const float al = __builtin_amdgcn_exp2f(dm), ao = __builtin_amdgcn_ldexpf(al, (int)(r[t] - r_new));
-        l[t] *= al;
+        const float ao = __builtin_amdgcn_ldexpf(dm.part, (int)(dm.whole + (r[t] - r_new)));
+        l[t] *= __builtin_amdgcn_ldexpf(dm.part, (int)dm.whole);
 #pragma unroll
         for (int n = 0; n < NV; ++n) o[t][n] *= ao;
         m[t] = m_new;
         r[t] = r_new;
       }
-      const float pv = __builtin_amdgcn_ldexpf(vs[t], 14 - (int)r_new);
+      // A page may have a scale far above 2^r where its probabilities are as small: 2^k of the factor
+      // then goes into the exponentials (so that it stays in fp32's range) and out of their sum.
+      float add = -base, back = 1.f;
+      int x = 14 - (int)r_new;
+      if (__any(lv - r_new > 100.f)) {
+        const int k = lv - r_new > 100.f ? (int)(lv - r_new) - 50 : 0;
+        add += (float)k;
+        back = __builtin_amdgcn_ldexpf(1.f, -k);
+        x -= k;
+      }
+      const float pv = __builtin_amdgcn_ldexpf(vs[t], x);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], f[t], -base));
-        l[t] += e;
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[t][i >> 2][i & 3], f[t], add));
+        l[t] = fmaf(e, back, l[t]);
         const float u = e * pv;
         const half_t hi = (half_t)u;
         p[t][i >> 3][0][i & 7] = hi;
@@ -543,8 +570,9 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
     float ll = 0.f;
 #pragma unroll
     for (int v = 0; v < kWaves; ++v) ll += l_lds[v][c] * __builtin_amdgcn_exp2f(m_lds[v][c] - base);
-    weight[t] = ll == 0.f ? 0.f : __builtin_amdgcn_exp2f(m[t] - base) / ll;
-    shift[t] = (int)r[t] - 14;
+    const Power dm(m[t] - base);
+    weight[t] = ll == 0.f ? 0.f : dm.part / ll;
+    shift[t] = (int)(r[t] + dm.whole) - 14;
     if (wave == 0 && g == 0 && col0 + c < w.n_cols) {
       const int h = w.hk * G + (col0 + c) % G;
       const size_t row = w.q0 + (col0 + c) / G;
@@ -565,8 +593,7 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         f32x4 x = o[t][n] * weight[t];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __builtin_amdgcn_ldexpf(x[i], shift[t]);
+        x = scaled(x, shift[t]);
         *reinterpret_cast<f32x4 *>(&lds.o[wave][16 * t + m16][16 * (n - 4 * half) + 4 * g]) = x;
       }
     __syncthreads();
@@ -670,19 +697,19 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new;
-    const float old = __builtin_amdgcn_exp2f(m - base);
+    const Power old(m - base), piece(mp - base);
     m = m_new;
     // (l of a piece, and so its weight, is 0 where it saw nothing, and NaN where that is its sum.)
-    lp *= __builtin_amdgcn_exp2f(mp - base);
-    float sum = lp;
+    lp *= piece.part;
+    float sum = __builtin_amdgcn_ldexpf(lp, (int)piece.whole);
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) sum += __shfl_xor(sum, o, 64);
-    const float before = l * old;
-    l = before + sum;
+    const float before = l * old.part;
+    l = __builtin_amdgcn_ldexpf(before, (int)old.whole) + sum;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     lp *= inv;
 #pragma unroll
-    for (int k = 0; k < NC; ++k) x[k] *= before * inv;
+    for (int k = 0; k < NC; ++k) x[k] = before * inv * scaled(x[k], (int)old.whole);
 #pragma unroll
     for (uint32_t half = 0; half < 2; ++half) {
       if (half == 1) {
@@ -691,9 +718,10 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
       }
 #pragma unroll
       for (uint32_t i = 0; i < kAhead; ++i) {
-        const float f = __shfl(lp, (lane & 48) + (int)(half * kAhead + i), 64);
+        const int from = (lane & 48) + (int)(half * kAhead + i), whole = __shfl((int)piece.whole, from, 64);
+        const float f = __shfl(lp, from, 64);
 #pragma unroll
-        for (int k = 0; k < NC; ++k) x[k] += f * y[i][k];
+        for (int k = 0; k < NC; ++k) x[k] += f * scaled(y[i][k], whole);
       }
     }
   }
@@ -710,18 +738,21 @@ __global__ __launch_bounds__(64 * kReduceWaves) void attention_reduce_kernel(Att
     for (int v = 1; v < kReduceWaves; ++v) m = fmaxf(m, ml_lds[v][lane >> 4][0]);
     const float base = m == -INFINITY ? 0.f : m;
     float f[kReduceWaves];
+    int whole[kReduceWaves];
     l = 0.f;
 #pragma unroll
     for (int v = 0; v < kReduceWaves; ++v) {
-      f[v] = ml_lds[v][lane >> 4][1] * __builtin_amdgcn_exp2f(ml_lds[v][lane >> 4][0] - base);
-      l += f[v];
+      const Power dm(ml_lds[v][lane >> 4][0] - base);
+      f[v] = ml_lds[v][lane >> 4][1] * dm.part;
+      whole[v] = (int)dm.whole;
+      l += __builtin_amdgcn_ldexpf(f[v], whole[v]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
-      x[k] *= f[0] * inv;  // (wave 0's own)
+      x[k] = scaled(x[k], whole[0]) * (f[0] * inv);  // (wave 0's own)
 #pragma unroll
-      for (int v = 1; v < kReduceWaves; ++v) x[k] += o_lds[v][k][lane] * (f[v] * inv);
+      for (int v = 1; v < kReduceWaves; ++v) x[k] += scaled(o_lds[v][k][lane], whole[v]) * (f[v] * inv);
     }
   }
   if (!on) return;
