@@ -185,18 +185,20 @@ template <bool E4M3>
 struct Side {
   unsigned char *codes;
   float s, inv, ratio;
+  bool dead;
   // From the bits of the new rows' largest magnitude (an infinity or a NaN is above all
   // numbers) and the scale of the rows that are kept (0: none). With such a row, or after
-  // one, the scale is NaN, and with it every value, whatever its code.
+  // one, the scale is NaN, and with it every value; the codes are 0 (a NaN among them would
+  // reach attention's rows that do not see the page: their probability there is 0, and 0 * NaN is NaN).
   __device__ __forceinline__ void scale(unsigned top, float old) {
     s = fmaxf(old, pow2_scale<E4M3>(__uint_as_float(top)));
-    const bool dead = top >= 0x7f800000u || old != old;
+    dead = top >= 0x7f800000u || old != old;
     if (dead) s = __builtin_nanf("");
     inv = dead ? 0.f : 1.f / s;
     ratio = dead ? 0.f : old * inv;
   }
   __device__ __forceinline__ unsigned encode(float4 v) const {
-    return encode4<E4M3>(make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+    return dead ? 0u : encode4<E4M3>(make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
   }
   // The rows before `off`, to the new scale, by `lanes` lanes of which this is `lane`: row
   // by row of K, column by column of V (whose last four bytes may hold newer rows).
@@ -207,7 +209,8 @@ struct Side {
       unsigned *at = reinterpret_cast<unsigned *>(codes + line * (is_v ? P : Dp)) + q;
       const unsigned c = *at, keep = is_v && 4 * q + 4 > off ? ~0u << (8 * (off - 4 * q)) : 0u;
       const float4 v = decode4<E4M3>(c);
-      *at = (encode4<E4M3>(make_float4(v.x * ratio, v.y * ratio, v.z * ratio, v.w * ratio)) & ~keep) | (c & keep);
+      const unsigned to = dead ? 0u : encode4<E4M3>(make_float4(v.x * ratio, v.y * ratio, v.z * ratio, v.w * ratio));
+      *at = (to & ~keep) | (c & keep);
     }
   }
 };

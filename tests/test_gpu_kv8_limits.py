@@ -1,5 +1,7 @@
 """The paged 8-bit cache at the limits of its numbers, against float64 (kv8_reference.py): pages whose scales lie far
-apart."""
+apart, infinities and NaN beside rows that do not see them."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -79,3 +81,58 @@ def test_scales_far_apart(device, case, fmt, act):
                 err = np.abs(out.double().cpu().numpy() - want)
                 assert (err <= tol).all(), (low, high, gap, float(np.nanmax(err / tol)), bool(np.isnan(err).any()))
                 assert (np.abs(lse.double().cpu().numpy() - wlse) <= ltol).all()
+
+
+# ---------------------------------------------------------------- infinities and NaN
+UNSEEN = [
+    # cached, queries, heads, kv heads, d, page, the bad position
+    (40, 16, 2, 2, 64, 16, 36),      # 16 columns
+    (70, 70, 2, 2, 64, 16, 20),      # 32
+    (70, 70, 2, 2, 64, 16, 50),
+    (70, 35, 4, 2, 128, 32, 66),
+    (230, 230, 2, 2, 64, 16, 19),    # 48
+    (230, 230, 2, 2, 33, 16, 215),
+    (1300, 20, 2, 2, 64, 16, 1290),  # tiles cut between workgroups
+    (1300, 200, 2, 2, 64, 16, 1205),
+    (1300, 80, 2, 2, 100, 48, 1280),
+]
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("case", range(len(UNSEEN)))
+def test_rows_that_do_not_see_a_bad_page(device, case, bad, fmt):
+    """Queries before a page of NaN, in one tile with queries behind it, get what they get without it, bit for bit;
+    the page's head gives NaN to those that see it, the other head nothing. So it stays when rows are added."""
+    n, nq, heads, kv_heads, d, page, at = UNSEEN[case]
+    say("unseen", UNSEEN[case], bad, fmt)
+    rng = np.random.RandomState(case)
+    k, v = (rng.randn(n, kv_heads, d) for _ in range(2))
+    start, seq = i32([0, nq], device), i32([n], device)
+    for act in (torch.float32, torch.bfloat16):
+        q = torch.tensor(rng.randn(nq, heads * d), device=device).to(act)
+        for in_k, in_v in ((False, True), (True, False), (True, True)):
+            for later in (False, True):
+                got = []
+                for x in (0.0, bad):
+                    kx, vx = k.copy(), v.copy()
+                    if in_k:
+                        kx[at, 1, d // 3] = x
+                    if in_v:
+                        vx[at, 1, d // 2] = x
+                    first = at + 1 if later else n  # (the rest comes in a call of its own, behind the bad row)
+                    pos = np.arange(n)
+                    cache = dfattn.kv8_cache(-(-n // page), kv_heads, d, page, ref.DTYPE[fmt], device)
+                    for a, b in ((0, first), (first, n)):
+                        dfattn.kv8_append(cache, *(torch.tensor(y[a:b].reshape(b - a, kv_heads * d), dtype=torch.float32, device=device)
+                                                   for y in (kx, vx)), i32(pos[a:b], device))
+                    got.append(dfattn.kv8_attention(cache, q, i32([range(-(-n // page))], device), start, seq, heads, nq, n))
+                (want, wlse), (out, lse) = got
+                assert torch.isfinite(want).all()
+                sees = torch.arange(n - nq, n, device=device) >= at // page * page
+                group = torch.arange(heads, device=device) // (heads // kv_heads) == 1
+                hit = sees[:, None] & group[None, :]
+                bits = out.view(nq, heads, d)
+                assert torch.isnan(bits[hit]).all() and torch.equal(bits[~hit], want.view(nq, heads, d)[~hit])
+                assert torch.isnan(lse.t()[hit]).all() if in_k else torch.equal(lse, wlse)
+                assert torch.equal(lse.t()[~hit], wlse.t()[~hit])
