@@ -247,7 +247,8 @@ __device__ __forceinline__ unsigned wave_top(unsigned x) {
   return __any(x >= 0x7f800000u) ? 0x7f800000u : __float_as_uint(m);
 }
 
-// The append goes by runs, the consecutive rows of one page. A workgroup finds those
+// The append goes by runs, rows of one page whose slots follow each other (a row that stands behind
+// another one of its page and does not follow it is left out). A workgroup finds those
 // that start among kWindow tokens (their slots and the next ones are one load) and
 // takes every `phases`-th of them. A run's rows are taken per kv head and side (K or
 // V): the largest magnitude, the scale, the codes; rows already there are coded
@@ -278,11 +279,11 @@ __global__ __launch_bounds__(64 * kAppendWaves, WIDE ? 3 : 4) void append_kernel
   // Lane l holds the slot of token i0 - 1 + l.
   const size_t token = i0 + lane;  // (one more than the lane's)
   const uint32_t slots = token > 0 && token <= a.n ? a.slots[token - 1] : DFATTN_NO_SLOT;
-  const uint32_t before = __shfl_up(slots, 1, 64);
-  const bool valid = lane > 0 && slots < n_slots;
-  const bool follows = valid && slots % (uint32_t)P != 0 && slots == before + 1;
-  const unsigned long long links = __ballot(follows);
-  unsigned long long starts = __ballot(valid && !follows && lane <= kWindow);
+  const uint32_t slot_page = slots / (uint32_t)P, before = __shfl_up(slots, 1, 64), page_before = __shfl_up(slot_page, 1, 64);
+  const bool valid = lane > 0 && slots < n_slots, same = valid && slot_page == page_before;
+  const unsigned long long links = __ballot(same && slots == before + 1);
+  // A row of the page of the one before it never starts a run: two runs of one page would race.
+  unsigned long long starts = __ballot(valid && !same && lane <= kWindow);
   for (uint32_t nth = 0; starts; starts &= starts - 1, ++nth) {
     if (nth % phases != phase) continue;
     const int first = __builtin_ctzll(starts);

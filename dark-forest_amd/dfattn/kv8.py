@@ -171,7 +171,8 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, free_start, page_
 
 def kv8_append(cache, k, v, slot_map, stream=None):
     """dfattn_kv8_append: rows k, v [n, kv heads * d_head] (float32 or bfloat16; one row stride, so column blocks
-    of a fused projection will do) into the slots slot_map [n] of `cache`."""
+    of a fused projection will do) into the slots slot_map [n] of `cache`, each page's rows next to each other with
+    consecutive slots (paged_plan's maps are so)."""
     names = _names()
     _check_stream(stream, names[6])
     n, dm = k.shape

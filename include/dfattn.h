@@ -382,9 +382,11 @@ size_t dfattn_kv8_pool_bytes(uint32_t n_pages, uint32_t n_kv_heads, uint32_t pag
 
 /* Append: row i of k and v [n_tokens, n_kv_heads*d_head] goes to slot
  * slot_map[i] (rows whose slot is not in the pool are left out). The rows
- * of one page must stand next to each other in the map with rising slots, as
- * dfattn_paged_plan's maps have them; else the contents of that page are
- * unspecified. A page's rows before the first one written are kept, those
+ * of one page must stand next to each other in the map with consecutive slots,
+ * each one more than the last, as dfattn_paged_plan's maps have them: a row that
+ * stands next to one of its page with any other slot is left out, and so are
+ * those that follow it in the page; a page that the map comes back to
+ * behind other rows has unspecified contents. A page's rows before the first one written are kept, those
  * after the last are unspecified. Scales are powers of two: the smallest s
  * >= 2^-126 with |x| <= 127 s (int8) or 448 s (e4m3) for every new value, and
  * not below the page's scale where rows are kept. A new value is rounded once,

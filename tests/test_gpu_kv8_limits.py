@@ -1,5 +1,5 @@
 """The paged 8-bit cache at the limits of its numbers, against float64 (kv8_reference.py): pages whose scales lie far
-apart, infinities and NaN beside rows that do not see them."""
+apart, infinities and NaN beside rows that do not see them, slots that do not follow each other."""
 import math
 
 import numpy as np
@@ -136,3 +136,40 @@ def test_rows_that_do_not_see_a_bad_page(device, case, bad, fmt):
                 assert torch.isnan(bits[hit]).all() and torch.equal(bits[~hit], want.view(nq, heads, d)[~hit])
                 assert torch.isnan(lse.t()[hit]).all() if in_k else torch.equal(lse, wlse)
                 assert torch.equal(lse.t()[~hit], wlse.t()[~hit])
+
+
+# ---------------------------------------------------------------- slots that do not follow each other
+JUMPS = [[3, 5, 6], [3, 3], [5, 3], [2, 4, 6], [7, 8, 9, 12, 13], [0, 2], [15, 0]]
+
+
+@pytest.mark.parametrize("fmt,act", [("i8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("heads,d,page", [(2, 64, 16), (12, 100, 32), (2, 33, 64)])
+@pytest.mark.parametrize("ahead", [0, 43, 44, 45, 46, 47, 48, 61, 62, 63, 64])
+def test_append_of_slots_that_jump(device, ahead, heads, d, page, fmt, act):
+    """A row whose slot does not follow the one before it in the same page is left out with those that follow it: the
+    page's rows up to there, and every other page, hold what they hold without them."""
+    say("jump", ahead, heads, d, page, fmt, act)
+    rng = np.random.RandomState(ahead)
+    pages = ahead + len(JUMPS)
+    cache = dfattn.kv8_cache(pages, heads, d, page, ref.DTYPE[fmt], device)
+    refs = [ref.Cache(pages, heads, page, d, fmt) for _ in range(2)]
+    base = [(ahead + i) * page for i in range(len(JUMPS))]
+    calls = [[b + o for b in base for o in range(page)]]                    # whole pages
+    calls.append([i * page for i in range(ahead)] + [b + o for b, jump in zip(base, JUMPS) for o in jump])
+    written = [[s for s in calls[0]], [i * page for i in range(ahead)]]
+    for b, jump in zip(base, JUMPS):
+        n = next((j for j in range(1, len(jump)) if jump[j] != jump[j - 1] + 1), len(jump))
+        written[1] += [b + o for o in jump[:n]] + [-1] * (len(jump) - n)
+    for n, (slots, kept) in enumerate(zip(calls, written)):
+        k, v = (torch.tensor(rng.randn(len(slots), heads * d) * 4.0 ** n, device=device).to(ref.ACT[act]) for _ in range(2))
+        for r, x in zip(refs, (k, v)):
+            r.append(x.double().cpu().numpy().reshape(len(slots), heads, d), kept)
+        dfattn.kv8_append(cache, k, v, i32(slots, device))
+    at = [i * page for i in range(ahead)]
+    for b, jump in zip(base, JUMPS):
+        n = next(j for j in range(1, len(jump)) if jump[j] != jump[j - 1] + 1)
+        at += [b + o for o in range(jump[n - 1] + 1)]
+    for g, w in zip(dfattn.kv8_read(cache, i32(at, device), d), refs):
+        assert np.array_equal(g.double().cpu().numpy(), w.read(at))
+    for t, w in zip(cache[2:], refs):
+        assert np.array_equal(t.double().cpu().numpy(), w.scale)
