@@ -167,8 +167,9 @@ int dfgpt2_linear_backward_weight(const float *grad_out, const float *x, float *
  * is not below cols has logprob 0. Statistics are fp32, in one fixed order of sums. rows <= 2^21, cols <= 2^27.
  * backward: grad_logits [rows, cols] (the logits' type, contiguous, overwritten; may be logits itself
  * when that is contiguous, another overlap is refused) = grad_logprob (1[j = token] - p_j) - grad_entropy p_j (ln p_j + entropy), from
- * the forward's stats and entropy; either gradient may be NULL (0). A masked-out value and a row of
- * nothing else get 0; a token that is not below cols gets nothing of grad_logprob.           */
+ * the forward's stats and entropy; either gradient may be NULL (0). A masked-out value gets 0, but where it is
+ * the token itself grad_logprob (its p is 0), and a row of nothing else 0 everywhere; a token that is not below
+ * cols gets nothing of grad_logprob.                                                         */
 int dfgpt2_token_logprobs(const void *logits, const uint32_t *tokens, float *logprob, float *entropy, float *stats,
                           uint32_t *top_ids, float *top_logprobs, uint32_t dtype, uint32_t rows, uint32_t cols,
                           uint32_t row_stride, uint32_t top_k, hipStream_t stream);

@@ -1,0 +1,53 @@
+"""dfgpt2_token_logprobs and its backward where the token itself is masked out, against float64."""
+import math
+
+import pytest
+import torch
+
+import test_gpu_token_logprobs as base
+from dfattn import ops
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [2, 100, 5001, 50257])
+def test_a_masked_token(device, n, dtype):
+    """A token at -infinity or at the type's lowest value in a row that has others: it gets grad_logprob itself, the other
+    columns what the formula says, as the gradient of a gather from log_softmax."""
+    base.say("masked token", n, dtype)
+    g = torch.Generator().manual_seed(n)
+    x = (torch.randn(4, n, generator=g) * 3).to(dtype)
+    tokens = torch.tensor([0, n - 1, n // 2, n - 1])
+    for row, value in ((0, -math.inf), (1, -math.inf), (2, torch.finfo(dtype).min), (3, -math.inf)):
+        x[row, tokens[row]] = value
+    x[3, : n // 2] = -math.inf  # with other columns masked out beside it
+    if n == 2:
+        x[3, 0] = 1.0
+    dev, (_, entropy, stats, _, _), want = base.check(x, tokens, 0, device)
+    assert torch.isneginf(want[0][[0, 1, 3]]).all()
+    gl, ge = torch.randn(4, generator=g), torch.randn(4, generator=g)
+    got = ops.token_logprobs_backward(dev, tokens.int().to(device), stats, entropy, gl.to(device), ge.to(device)).cpu()
+    at = torch.arange(4)
+    assert torch.equal(got[at, tokens], gl.to(dtype))
+    want, p, logp, h = base.grad_reference(x.double(), tokens, gl.double(), ge.double())
+    # The bound of base.test_backward: half a step of each gradient's own value and what p and ln p are off by.
+    t_lse, t_ent = base.tolerances(x.double())
+    rel = t_lse[:, None] + 2.0 ** -21 + logp.abs() * 2.0 ** -22
+    half = torch.finfo(dtype).eps / 2
+
+    def bound(want, a, b):
+        tol = a.abs()[:, None] * (p * rel + 2.0 ** -22) + b.abs()[:, None] * p * (
+            (logp + h[:, None]).abs() * (rel + 2.0 ** -22) + t_lse[:, None] + t_ent[:, None] + (logp.abs() + 1) * 2.0 ** -22)
+        tol = tol + want.abs() * half + 1e-38
+        return tol + tol * half if dtype == torch.bfloat16 else tol
+
+    assert ((got.double() - want).abs() <= bound(want, gl.double(), ge.double())).all()
+    masked = torch.isneginf(x)
+    masked[at, tokens] = False
+    assert not got[masked].any()
+    # torch's own answer, in float64.
+    leaf = x.double().requires_grad_(True)
+    torch.log_softmax(leaf, 1).gather(1, tokens[:, None])[:, 0].backward(gl.double())
+    only = ops.token_logprobs_backward(dev, tokens.int().to(device), stats, entropy, gl.to(device)).double().cpu()
+    assert ((only - leaf.grad).abs() <= bound(leaf.grad, gl.double(), torch.zeros(4))).all()
