@@ -75,6 +75,13 @@ def _ptr(t, name, dtype, dev):
     return t.data_ptr()
 
 
+def _u32(x, name):
+    """x, which ctypes would otherwise pass modulo 2^32."""
+    if not 0 <= x < 1 << 32:
+        raise ValueError(f"{name} must be at least 0 and below 2^32")
+    return x
+
+
 def _rows(t, name, cols, n):
     """(pointer, row stride, type code) of a float32 or bfloat16 [rows, cols] tensor whose rows may be a
     column block of a wider one."""
@@ -89,6 +96,7 @@ def _rows(t, name, cols, n):
             stride = t.stride(0)
         if (t.stride(1) != 1 and cols > 1) or stride < cols:
             raise ValueError(f"{name} must be [rows, {cols}] with contiguous rows")
+        _u32(stride, f"{name}'s row stride")
     return t.data_ptr(), stride, 0 if dtype is n[2] else 1
 
 
@@ -149,6 +157,7 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, free_start, page_
     r = cached_lens.numel()
     if block_table.dim() != 2 or block_table.shape[0] != r or new_lens.numel() != r or free_start.numel() != 1:
         raise ValueError("cached_lens and new_lens are [R], block_table [R, max_pages], free_start [1]")
+    _u32(page_size, "page_size"), _u32(n_pages, "n_pages"), _u32(token_capacity, "token_capacity")
     with _on(stream, dev):
         on = cached_lens.device
         if seq_lens is None and query_start is None and slot_map is None and counts is None:
@@ -221,8 +230,9 @@ def kv8_attention(cache, q, block_table, query_start, seq_lens, n_heads, max_que
     lse [n_heads, n])."""
     names = _names()
     i32, f32, dev = names[1], names[2], names[6]
-    if q.dim() != 2 or q.shape[1] % n_heads:
+    if q.dim() != 2 or n_heads < 1 or q.shape[1] % n_heads:
         raise ValueError("q must be [n, n_heads * d_head]")
+    _u32(max_query_len, "max_query_len"), _u32(max_seq_len, "max_seq_len")
     n, dm = q.shape
     d_head = dm // n_heads
     ptrs, kv, heads, page, pages = _cache(cache, d_head, names)

@@ -254,8 +254,8 @@ def _logit_rows(t):
     if not t.is_contiguous():
         if rows > 1:
             stride = t.stride(0)
-        if (t.stride(1) != 1 and v > 1) or stride < v:
-            raise ValueError("logits must be [rows, V] with contiguous rows")
+        if (t.stride(1) != 1 and v > 1) or not v <= stride < 1 << 32:  # (ctypes takes a stride modulo 2^32)
+            raise ValueError("logits must be [rows, V] with contiguous rows, less than 2^32 elements apart")
     return rows, v, t.data_ptr(), stride, 0 if dtype is torch.float32 else 1
 
 

@@ -1,4 +1,4 @@
-"""dfgpt2_token_logprobs and its backward where the token itself is masked out, against float64."""
+"""dfgpt2_token_logprobs and its backward where the token itself is masked out, against float64; rows too far apart."""
 import math
 
 import pytest
@@ -51,3 +51,15 @@ def test_a_masked_token(device, n, dtype):
     torch.log_softmax(leaf, 1).gather(1, tokens[:, None])[:, 0].backward(gl.double())
     only = ops.token_logprobs_backward(dev, tokens.int().to(device), stats, entropy, gl.to(device)).double().cpu()
     assert ((only - leaf.grad).abs() <= bound(leaf.grad, gl.double(), torch.zeros(4))).all()
+
+
+def test_rows_too_far_apart(device):
+    """A row stride of 2^32 elements or more is refused: modulo 2^32 it is that of other rows."""
+    n = 100
+    far = torch.empty((1 << 32) + 4096 + n, dtype=torch.bfloat16, device=device).as_strided((2, n), ((1 << 32) + 4096, 1))
+    t = torch.zeros(2, dtype=torch.int32, device=device)
+    with pytest.raises(ValueError):
+        ops.token_logprobs_forward(far, t)
+    with pytest.raises(ValueError):
+        ops.token_logprobs_backward(far, t, torch.zeros(2, 2, device=device), torch.zeros(2, device=device))
+    assert ops.token_logprobs_forward(far[:1], t[:1])[0].shape == (1,)  # (one row has no stride)
