@@ -1,4 +1,5 @@
-"""dfgpt2_token_logprobs and its backward where the token itself is masked out, against float64; rows too far apart."""
+"""dfgpt2_token_logprobs and its backward where the token itself is masked out, against float64; rows too far apart; the most
+alternatives."""
 import math
 
 import pytest
@@ -63,3 +64,13 @@ def test_rows_too_far_apart(device):
     with pytest.raises(ValueError):
         ops.token_logprobs_backward(far, t, torch.zeros(2, 2, device=device), torch.zeros(2, device=device))
     assert ops.token_logprobs_forward(far[:1], t[:1])[0].shape == (1,)  # (one row has no stride)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_most_alternatives(device, dtype):
+    """64 alternatives of many ordinary rows, of which some have more logits above the bound that 64 reach than the
+    kernel keeps (7 of these in fp32)."""
+    base.say("64 alternatives", dtype)
+    g = torch.Generator().manual_seed(64)
+    x = (torch.randn(256, 20011, generator=g) * 2).to(dtype)
+    base.check(x, torch.randint(0, 20011, (256,), generator=g), 64, device)
