@@ -360,7 +360,7 @@ __device__ __forceinline__ unsigned short to_bf16(float f) {
 // memory (a read and a write). 16 bytes a thread and step, from any element's
 // address. Everything a workgroup reads of its part of the row is read before it
 // is written, so the gradient may lie where the logits do. 1000 rows of 50257 in fp32 67 us,
-// 6.0 TB/s (after the forward, with part of the logits still in the Infinity Cache).
+// 6.0 TB/s (after the forward, with part of the logits still in the Infinity Cache), in bf16 39, 5.2.
 constexpr int kGradSteps = 4;
 template <bool BF16>
 __global__ __launch_bounds__(256) void logprob_grad_kernel(GradArgs a) {

@@ -177,12 +177,17 @@ struct Share {
 // r), where 2^r (r whole) bounds the largest such product so far: m and r move
 // together, so products keep 2^-39 of the largest one whatever the pages'
 // scales. Powers of two that fp32 has no room for (a weight of 2^-200 before values of
-// 2^120) are kept apart as exponents, here and in the merges.
+// 2^120) are kept apart as exponents, here and in the merges. bf16 takes one term: q fits it, and P's
+// rounding of at most 2^-11 is an eighth of the output's (against float64 1.6e-3 as for fp32 sums
+// rounded once; 6 outputs in 100 are the neighbouring bf16 value).
 //
-// Measured (12 heads of 64): one query on 2 x 131072 keys 60 us, 5.0 TB/s, on 64 requests of up to
+// Measured (12 heads of 64): one query on 2 x 131072 keys 61 us, 4.9 TB/s, on 64 requests of up to
 // 4096 (e4m3, bf16) 47 us, 4.4 TB/s: memory, of which two workgroups a CU keep enough on its
-// way (three took 69 us for 67, with the merge). Chunks of 3 x 500 queries of up to 4096 keys 52-60
-// us: VALU instructions, some 460 for the 64 products of 32 columns and 64 keys.
+// way (three took 69 us for 67, with the merge). Chunks of 3 x 500 queries of up to 4096 keys 53-60
+// us: VALU instructions take 60 % of a SIMD's time (ten for each product), the matrix pipe 20 %, and the
+// waves wait 29 % of theirs: two waves a SIMD, in each of which the barriers keep products and
+// exponentials apart, overlap no better. fp32 with 48 columns, or 32 of more than 64 values, spills 4 to 22
+// registers, none of them in the loop.
 template <bool E4M3, int NT, int NC, int QT, bool SHARED>
 __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnArgs a) {
   constexpr bool BF16 = NT == 1;

@@ -456,7 +456,7 @@ __global__ __launch_bounds__(64 * kAppendWaves, WIDE ? 3 : 4) void append_kernel
 
 // ---------------------------------------------------------------- read
 // A wave takes four rows of the list and 64 columns of a head at a time, K and V together
-// (8197 rows of 8 heads of 128, bf16 to fp32, 85 MB, 22 us, one after the other 23), lane 4 i + j columns
+// (8309 rows of 8 heads of 128 to fp32, 85 MB, 22 us, one after the other 23; to bf16, 51 MB, 19), lane 4 i + j columns
 // 4 i .. of row j. V's codes of four consecutive rows of a page are read as the append
 // writes them; other rows byte by byte.
 constexpr int kReadWaves = 4;

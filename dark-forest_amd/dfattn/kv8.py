@@ -225,7 +225,8 @@ def kv8_attention(cache, q, block_table, query_start, seq_lens, n_heads, max_que
                   causal=True, out=None, lse=None, workspace="auto", stream=None):
     """dfattn_kv8_attention: q [n, n_heads * d_head] (float32 or bfloat16, rows may be a column block), the tokens of
     R requests packed by query_start [R+1], against seq_lens [R] cached positions in block_table [R, max_pages].
-    max_query_len, max_seq_len: bounds of the lengths. workspace: "auto" allocates
+    max_query_len, max_seq_len: bounds of the lengths (a long chunk beside many requests of one token is faster in a call of
+    its own). workspace: "auto" allocates
     dfattn_kv8_attention_workspace_bytes, None does not split the keys. Returns (out [n, n_heads * d_head] in q's type,
     lse [n_heads, n])."""
     names = _names()

@@ -359,8 +359,9 @@ int dfattn_decode(const float *q, const void *k_cache, const void *v_cache,
  * where a page id is not below n_pages) and counts [3]: requests admitted,
  * tokens, and the next call's free_start. Outputs that overlap inputs or each
  * other are refused (cached_lens and free_start: copy seq_lens and counts + 2
- * between calls). n_requests <= 8192, page_size any, n_pages * page_size <=
- * 2^31. Latency: 4 us for 64 tokens, 8 us for 65536.                         */
+ * between calls). n_requests is 1..8192 (a step without requests has no plan:
+ * it is refused), page_size any, n_pages * page_size <= 2^31. Latency: 4 us for
+ * 64 tokens, 8 us for 65536.                                                 */
 int dfattn_paged_plan(const uint32_t *cached_lens, const uint32_t *new_lens,
                       const uint32_t *free_pages, const uint32_t *free_start,
                       uint32_t *block_table, uint32_t *seq_lens,
@@ -423,11 +424,19 @@ int dfattn_kv8_read(const void *k_pool, const void *v_pool, const float *k_scale
  * n_pages are left out; a table entry past a request's length is not read, and
  * a length past the table's row counts as its end. max_query_len and
  * max_seq_len are bounds the caller knows of the lengths on the device; queries
- * past max_query_len are not computed, a longer sequence only costs time.
+ * past max_query_len are not computed, a longer sequence only costs time. Every
+ * request costs what max_query_len queries need to be looked at: a long chunk
+ * beside many requests of one token is slower than the two apart (63 requests
+ * of up to 4096 keys and a chunk of 2048 238 us, apart 56 and 65; 500 and one
+ * of 512 3347, apart 441 and 37), so give those to calls of their own.
  * n_requests <= 65535; max_pages * page_size, n_tokens and max_query_len *
- * (n_heads / n_kv_heads) <= 2^30; out and lse must not overlap what is read. Softmax statistics and sums are fp32; with fp32 activations
- * q and P enter the matrix products as two fp16 terms (22 bits), with bf16
- * as one (12 bits at least). |scale q| must stay below fp32's range over 2^16.
+ * (n_heads / n_kv_heads) <= 2^30; out and lse must not overlap what is read.
+ * Softmax statistics and sums are fp32. With fp32 activations q and P enter the
+ * matrix products as two fp16 terms (22 bits), with bf16 as one (q exactly, P
+ * in 11 bits), and anything below 2^-39 of a row's largest q or of its largest
+ * P * (scale of the value's page) may be lost. A row's largest |scale q| must
+ * stay below fp32's range over 2^16; where it is below 2^-110 its scores lose
+ * bits.
  * Workspace: dfattn_kv8_attention_workspace_bytes of the same sizes (0: none
  * needed); NULL: no split over the keys, one workgroup walks each row's. Calls
  * that may overlap need one each. Results are reproducible bit for bit.      */
