@@ -65,6 +65,11 @@ __device__ __forceinline__ float column_sum(float v) {
   return pair_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// The product rounded, never fused with what is added to it.
+__device__ __forceinline__ float times(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
 // 2^x, x <= 0 or -infinity, as part * 2^whole with part in (1/2, 1] (0 below 2^-1000): a weight too
 // small for fp32 may still count, where its values are that much larger.
 struct Power {
@@ -186,7 +191,7 @@ struct Share {
 // way (three took 69 us for 67, with the merge). Chunks of 3 x 500 queries of up to 4096 keys 53-60
 // us: VALU instructions take 60 % of a SIMD's time (ten for each product), the matrix pipe 20 %, and the
 // waves wait 29 % of theirs: two waves a SIMD, in each of which the barriers keep products and
-// exponentials apart, overlap no better. fp32 with 48 columns, or 32 of more than 64 values, spills 4 to 22
+// exponentials apart, overlap no better. fp32 with 48 columns, and 32 of more than 64 values, spill 2 to 19
 // registers, none of them in the loop.
 template <bool E4M3, int NT, int NC, int QT, bool SHARED>
 __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnArgs a) {
@@ -472,7 +477,7 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
       float top = s[t][0][0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) top = fmaxf(top, s[t][i >> 2][i & 3]);
-      top *= f[t];
+      top = times(top, f[t]);
       const float m_new = fmaxf(m[t], column_max(top));
       const float base = m_new == -INFINITY ? 0.f : m_new;
       const Power dm(m[t] - base);
@@ -486,10 +491,20 @@ __global__ __launch_bounds__(64 * kWaves, kResident) void attention_kernel(AttnA
         m[t] = m_new;
         r[t] = r_new;
       }
-      // A page may have a scale far above 2^r where its probabilities are as small: 2^k of the factor
-      // then goes into the exponentials (so that it stays in fp32's range) and out of their sum.
       float add = -base, back = 1.f;
       int x = 14 - (int)r_new;
+      // base is a rounded product: the fused one below is off from it by up to 2^-25 of a score, for the
+      // largest too. From 2^20 on that is more than the weights have room for.
+      if (__any(fabsf(base) > 0x1p20f)) {
+        const bool large = fabsf(base) > 0x1p20f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          s[t][i >> 2][i & 3] = large ? times(s[t][i >> 2][i & 3], f[t]) - base : s[t][i >> 2][i & 3];
+        f[t] = large ? 1.f : f[t];
+        add = large ? 0.f : add;
+      }
+      // A page may have a scale far above 2^r where its probabilities are as small: 2^k of the factor
+      // then goes into the exponentials (so that it stays in fp32's range) and out of their sum.
       if (__any(lv - r_new > 100.f)) {
         const int k = lv - r_new > 100.f ? (int)(lv - r_new) - 50 : 0;
         add += (float)k;

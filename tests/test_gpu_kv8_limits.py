@@ -1,5 +1,6 @@
 """The paged 8-bit cache at the limits of its numbers, against float64 (kv8_reference.py): pages whose scales lie far
-apart, infinities and NaN beside rows that do not see them, slots that do not follow each other."""
+apart, infinities and NaN beside rows that do not see them, slots that do not follow each other, scores up to
+2^100."""
 import math
 
 import numpy as np
@@ -173,3 +174,58 @@ def test_append_of_slots_that_jump(device, ahead, heads, d, page, fmt, act):
         assert np.array_equal(g.double().cpu().numpy(), w.read(at))
     for t, w in zip(cache[2:], refs):
         assert np.array_equal(t.double().cpu().numpy(), w.scale)
+
+
+# ---------------------------------------------------------------- large scores
+@pytest.mark.parametrize("fmt,act", [("i8", "f32"), ("e4m3", "bf16"), ("e4m3", "f32"), ("i8", "bf16")])
+@pytest.mark.parametrize("power", [16, 21, 24, 27, 30, 40, 60, 100])
+def test_large_scores(device, power, fmt, act):
+    """Scores of about 2^power, of either sign: each row's largest two keys are the same and lie far above the others, so
+    that the output is the mean of their values and lse the score and ln 2.
+
+    The bound: a score's products and sums are off by (u + (d + 4) 2^-24) sum|q||k| alike for the two, so their
+    weights are both 1 but for the exponential's 2^-22; the values' sum is fp32's of fp16 terms (u). lse is off by what
+    the score is, and 2^-22 of its size."""
+    heads, d, page = 2, 64, 16
+    u = 2.0 ** -22 if act == "f32" else 2.0 ** -11
+    step = 0.0 if act == "f32" else 2.0 ** -8
+    for n, nq in ((70, 1), (70, 20), (3000, 1), (1300, 200), (300, 300)):
+        for sign in (1.0, -1.0):
+            say("large scores", power, fmt, act, n, nq, sign)
+            rng = np.random.RandomState(power)
+            k, v = (rng.randn(n, heads, d) for _ in range(2))
+            k[:, :, 0] = np.where(np.arange(n) == 3, -1.0, -3.0)[:, None]  # all scores of one sign, key 3's next to 0
+            twins = [0, n - nq - 1 if nq < n else 1]
+            k[twins[1]] = k[twins[0]]
+            k[twins, :, 0] = 4.0
+            k[:, :, 1:] *= 2.0 ** -6
+            if sign < 0:  # (all scores negative, the twins' the least so)
+                k[:, :, 0] = -6.0
+                k[3, :, 0] = -5.0
+                k[twins, :, 0] = -1.0
+            cache, table, kr, vr = filled(device, k, v, page, fmt, power)
+            q = rng.randn(nq, heads, d) * 2.0 ** -6
+            q[:, :, 0] = rng.uniform(1, 2, (nq, heads))
+            q = torch.tensor(q.reshape(nq, -1), device=device).to(ref.ACT[act])
+            qd = q.double().cpu().numpy().reshape(nq, heads, d)
+            same = np.array_equal(kr[twins[0]], kr[twins[1]])
+            scale = 2.0 ** power
+            out, lse = dfattn.kv8_attention(cache, q, table, i32([0, nq], device), i32([n], device), heads, nq, n, scale)
+            out, lse = out.double().cpu().numpy().reshape(nq, heads, d), lse.double().cpu().numpy()
+            assert np.isfinite(out).all() and np.isfinite(lse).all()
+            for j in range(nq):
+                see = n - nq + j + 1
+                for h in range(heads):
+                    x = scale * (kr[:see, h] @ qd[j, h])
+                    err = scale * (np.abs(kr[:see, h]) @ np.abs(qd[j, h])).max() * (u + (d + 4) * 2.0 ** -24)
+                    err += 2.0 ** -22 * np.abs(x).max()
+                    top = np.nonzero(x >= x.max() - 2 * err - 60)[0]
+                    assert abs(lse[h, j] - x.max()) <= err + np.log(len(top)) + 1e-5
+                    if len(top) == 1 or (same and list(top) == twins):
+                        want = vr[top, h].mean(0)
+                        tol = np.abs(vr[top, h]).mean(0) * (2.0 ** -20 + u + step) + 2.0 ** -38 * np.abs(vr[:, h]).max()
+                        assert (np.abs(out[j, h] - want) <= tol).all(), (j, h, top)
+                    else:  # (a value between those of the keys that cannot be told apart)
+                        lo, hi = vr[top, h].min(0), vr[top, h].max(0)
+                        slack = (np.abs(lo) + np.abs(hi)) * (2.0 ** -20 + u + step) + 1e-6
+                        assert (out[j, h] >= lo - slack).all() and (out[j, h] <= hi + slack).all()
