@@ -1,5 +1,5 @@
 """dfgpt2_token_logprobs and its backward where the token itself is masked out, against float64; rows too far apart; the most
-alternatives."""
+alternatives; a training step in a graph."""
 import math
 
 import pytest
@@ -74,3 +74,42 @@ def test_the_most_alternatives(device, dtype):
     g = torch.Generator().manual_seed(64)
     x = (torch.randn(256, 20011, generator=g) * 2).to(dtype)
     base.check(x, torch.randint(0, 20011, (256,), generator=g), 64, device)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_training_step_replayed_from_a_graph(device, dtype):
+    """Forward and backward of the differentiable form captured together: every replay against the eager step."""
+    rows, dim, n = 33, 16, 3001
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(rows, dim, generator=g).to(device).to(dtype)
+    tokens = torch.randint(0, n, (rows,), generator=g).int().to(device)
+    weights = [torch.randn(dim, n, generator=g).to(device).to(dtype) for _ in range(3)]
+
+    def step(leaf):
+        logprob, entropy, ids, _ = ops.token_logprobs(x @ leaf, tokens, 3)
+        loss = -logprob.mean() - 0.01 * entropy.mean()
+        (grad,) = torch.autograd.grad(loss, leaf)
+        return loss.detach(), grad, ids
+
+    eager = []
+    for w in weights:
+        base.say("eager", dtype)
+        eager.append(step(w.clone().requires_grad_(True)))
+    leaf = torch.zeros_like(weights[0]).requires_grad_(True)  # (no eager graph of it)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(leaf)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    base.say("capture")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(leaf)
+    for _ in range(2):
+        for w, want in zip(weights, eager):
+            with torch.no_grad():
+                leaf.copy_(w)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(held, want))
