@@ -188,9 +188,9 @@ struct Share {
 //
 // Measured (12 heads of 64): one query on 2 x 131072 keys 61 us, 4.9 TB/s, on 64 requests of up to
 // 4096 (e4m3, bf16) 47 us, 4.4 TB/s: memory, of which two workgroups a CU keep enough on its
-// way (three took 69 us for 67, with the merge). Chunks of 3 x 500 queries of up to 4096 keys 53-60
+// way (three took 69 us for 67, with the merge). Chunks of 3 x 500 queries of up to 4096 keys 53-61
 // us: VALU instructions take 60 % of a SIMD's time (ten for each product), the matrix pipe 20 %, and the
-// waves wait 29 % of theirs: two waves a SIMD, in each of which the barriers keep products and
+// waves wait 30 % of theirs: two waves a SIMD, in each of which the barriers keep products and
 // exponentials apart, overlap no better. fp32 with 48 columns, and 32 of more than 64 values, spill 2 to 19
 // registers, none of them in the loop.
 template <bool E4M3, int NT, int NC, int QT, bool SHARED>
