@@ -1,0 +1,391 @@
+// gpt2_w4.hip — linear layers with 4-bit weights and a scale for each group of
+// inputs: quantising, the values back, and the products with bias, GELU and
+// residual (gfx950).
+//
+// codes [outputs, row bytes], input 2 b in the low half of byte b; scales bf16
+// and zeros (one byte) [groups, outputs].
+#include "dfattn_internal.h"
+#include "dfgpt2.h"
+#include "dfattn_status.h"
+#include "gpt2_device.h"
+
+#include <algorithm>
+#include <initializer_list>
+#include <string>
+#include <type_traits>
+
+namespace dfattn {
+namespace {
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+constexpr uint32_t kMaxFeatures = 1u << 24;
+
+enum Format { kI4 = DFGPT2_W4_I4, kU4 = DFGPT2_W4_U4, kE2M1 = DFGPT2_W4_E2M1 };
+
+__device__ __forceinline__ float bf16_value(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
+// To the nearest, ties to even; a NaN stays one.
+__device__ __forceinline__ unsigned short bf16_bits(float f) {
+  const unsigned u = __float_as_uint(f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)(u >> 16 | 0x40u);
+  return (unsigned short)((u + 0x7fffu + (u >> 16 & 1u)) >> 16);
+}
+// The value of code c (0..15) before its scale.
+template <Format F>
+__device__ __forceinline__ float code_value(unsigned c, float zero) {
+  if constexpr (F == kE2M1) {
+    // 0 1/2 1 3/2 2 3 4 6: from 2 on an exponent and one bit, below multiples of 1/2.
+    const unsigned m = c & 7;
+    const float v = m < 2 ? 0.5f * m : __uint_as_float((126 + (m >> 1)) << 23 | (m & 1) << 22);
+    return c & 8 ? -v : v;
+  } else {
+    return (float)c - zero;
+  }
+}
+
+template <bool BF16>
+__device__ __forceinline__ float load_value(const void *p, size_t i) {
+  if constexpr (BF16)
+    return bf16_value(static_cast<const unsigned short *>(p)[i]);
+  else
+    return static_cast<const float *>(p)[i];
+}
+template <bool BF16>
+__device__ __forceinline__ void store_value(void *p, size_t i, float v) {
+  if constexpr (BF16)
+    static_cast<unsigned short *>(p)[i] = bf16_bits(v);
+  else
+    static_cast<float *>(p)[i] = v;
+}
+
+// ---------------------------------------------------------------- quantise
+struct QuantArgs {
+  const void *w;
+  unsigned *codes;
+  unsigned short *scales;
+  unsigned char *zeros;
+  void *out;
+  size_t stride;
+  uint32_t N, K, log_group, row_dwords, column_blocks;
+};
+
+// The nearest bf16 to q >= 0, ties to even: by way of the float below it with the rest in its
+// last bit, so that the second rounding sees what the first left out.
+__device__ __forceinline__ unsigned short nearest_bf16(double q) {
+  float f = __double2float_rz(q);
+  if ((double)f != q) f = __uint_as_float(__float_as_uint(f) | 1u);
+  return bf16_bits(f);
+}
+
+// x / s to the nearest whole number, ties to even, for a bf16 s > 0 and |x| up to some 16 s: x * (1 / s)
+// is at most one off after rounding, and the remainder x - c s is exact (c s has at most 13 bits, and
+// where c is not 0 it is within a factor of two of x).
+struct Divider {
+  float f, s, inv, half;
+  __device__ __forceinline__ explicit Divider(float scale) {
+    f = scale < 0x1p-100f ? 0x1p64f : 1.f;  // (1 / s would be infinite)
+    s = scale * f;
+    inv = 1.f / s;
+    half = 0.5f * s;
+  }
+  __device__ __forceinline__ float nearest(float x) const {
+    x *= f;
+    float c = __builtin_rintf(x * inv);
+    const float r = fmaf(-c, s, x);
+    const bool odd = ((int)c & 1) != 0;
+    if (r > half || (r == half && odd))
+      c += 1.f;
+    else if (r < -half || (r == -half && odd))
+      c -= 1.f;
+    return c;
+  }
+};
+
+// A workgroup takes 32 outputs and 256 inputs: a lane 8 inputs of four outputs, 4 to 16 neighbours a
+// group. The scales go through LDS, so that neighbouring outputs' are written together.
+constexpr int kQuantRows = 32, kQuantCols = 256;
+template <Format F, bool BF16>
+__global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
+  __shared__ unsigned short scale_lds[kQuantCols / 32][kQuantRows];
+  __shared__ unsigned char zero_lds[kQuantCols / 32][kQuantRows];
+  const uint32_t block = linear_block(), n0 = block / a.column_blocks * kQuantRows, k0 = block % a.column_blocks * kQuantCols;
+  if (n0 >= a.N) return;
+  const uint32_t lane = threadIdx.x & 31, d = k0 / 8 + lane, lanes = 1u << (a.log_group - 3);
+  float x[4][8];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint32_t n = n0 + 8 * r + (threadIdx.x >> 5);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      x[r][j] = n < a.N && d * 8 + j < a.K ? load_value<BF16>(a.w, n * a.stride + d * 8 + j) : 0.f;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const uint32_t row = 8 * r + (threadIdx.x >> 5), n = n0 + row;
+    float lo = 0.f, hi = 0.f;
+    int bad = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      lo = fminf(lo, x[r][j]);
+      hi = fmaxf(hi, x[r][j]);
+      bad |= !(fabsf(x[r][j]) < __builtin_inff());
+    }
+    for (uint32_t o = 1; o < lanes; o <<= 1) {
+      lo = fminf(lo, __shfl_xor(lo, (int)o, 64));
+      hi = fmaxf(hi, __shfl_xor(hi, (int)o, 64));
+      bad |= __shfl_xor(bad, (int)o, 64);
+    }
+    const double top = F == kU4 ? ((double)hi - (double)lo) / 15.0 : (double)fmaxf(hi, -lo) / (F == kI4 ? 7.0 : 6.0);
+    const unsigned short bits = bad ? 0x7fc0u : nearest_bf16(top);
+    const float s = bf16_value(bits);
+    const bool some = s > 0.f;  // (neither 0 nor NaN)
+    const Divider by(some ? s : 1.f);
+    float zero = F == kI4 ? 8.f : 0.f;
+    if (F == kU4 && some) zero = fminf(fmaxf(by.nearest(-lo), 0.f), 15.f);
+    unsigned c = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      unsigned q;
+      if constexpr (F == kE2M1) {
+        const float y = fabsf(x[r][j]);
+        q = (y > 0.25f * s) + (y >= 0.75f * s) + (y > 1.25f * s) + (y >= 1.75f * s) + (y > 2.5f * s) + (y >= 3.5f * s) +
+            (y > 5.f * s);
+        q = some ? q | (__float_as_uint(x[r][j]) >> 31 << 3) : 0u;
+      } else {
+        const float v = (some ? by.nearest(x[r][j]) : 0.f) + zero;
+        q = (unsigned)fminf(fmaxf(v, 0.f), 15.f);
+      }
+      c |= q << (4 * j);
+    }
+    if (n < a.N && d < a.row_dwords) a.codes[(size_t)n * a.row_dwords + d] = c;
+    if ((lane & (lanes - 1)) == 0) {
+      scale_lds[lane / lanes][row] = bits;
+      if (F == kU4) zero_lds[lane / lanes][row] = (unsigned char)zero;
+    }
+  }
+  __syncthreads();
+  const uint32_t g = threadIdx.x >> 5, n = n0 + lane, at = (k0 >> a.log_group) + g;
+  if (g >= (uint32_t)kQuantCols >> a.log_group || n >= a.N || (size_t)at << a.log_group >= a.K) return;
+  a.scales[(size_t)at * a.N + n] = scale_lds[g][lane];
+  if (F == kU4) a.zeros[(size_t)at * a.N + n] = zero_lds[g][lane];
+}
+
+// ---------------------------------------------------------------- values
+template <Format F, bool BF16>
+__global__ __launch_bounds__(kThreads) void dequantize_kernel(QuantArgs a) {
+  const size_t id = (size_t)linear_block() * kThreads + threadIdx.x;
+  const uint32_t per_row = (a.K + 7) / 8;
+  const size_t n = id / per_row;
+  const uint32_t d = (uint32_t)(id % per_row);
+  if (n >= a.N) return;
+  const unsigned c = a.codes[n * a.row_dwords + d];
+  const size_t at = (size_t)(d * 8 >> a.log_group) * a.N + n;
+  const float s = bf16_value(a.scales[at]), zero = F == kU4 ? (float)a.zeros[at] : 8.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (d * 8 + j < a.K) store_value<BF16>(a.out, n * a.K + d * 8 + j, code_value<F>(c >> (4 * j) & 15u, zero) * s);
+}
+
+// ---------------------------------------------------------------- products
+struct LinearArgs {
+  const void *x;
+  const unsigned *codes;
+  const unsigned short *scales;
+  const unsigned char *zeros;
+  const float *bias;
+  const void *residual;
+  void *out;
+  size_t stride;
+  uint32_t M, N, K, log_group, row_dwords;
+  int gelu;
+};
+
+// One output of kRows rows a wave; a lane has 8 inputs at a time, all of one group.
+constexpr int kRows = 4;
+template <Format F, bool BF16>
+__global__ __launch_bounds__(kThreads) void linear_kernel(LinearArgs a) {
+  const uint32_t n = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63, m0 = blockIdx.y * kRows;
+  if (n >= a.N) return;
+  float sum[kRows] = {};
+  for (uint32_t d = lane; d * 8 < a.K; d += 64) {
+    const unsigned c = a.codes[(size_t)n * a.row_dwords + d];
+    const size_t at = (size_t)(d * 8 >> a.log_group) * a.N + n;
+    const float s = bf16_value(a.scales[at]), zero = F == kU4 ? (float)a.zeros[at] : 8.f;
+    for (int r = 0; r < kRows; ++r) {
+      if (m0 + r >= a.M) break;
+      float part = 0.f;
+      for (int j = 0; j < 8; ++j)
+        if (d * 8 + j < a.K) part = fmaf(code_value<F>(c >> (4 * j) & 15u, zero), load_value<BF16>(a.x, (m0 + r) * a.stride + d * 8 + j), part);
+      sum[r] = fmaf(part, s, sum[r]);
+    }
+  }
+  for (int r = 0; r < kRows; ++r) {
+    float y = sum[r];
+    for (int o = 32; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
+    if (lane != 0 || m0 + r >= a.M) continue;
+    const size_t at = (size_t)(m0 + r) * a.N + n;
+    if (a.bias != nullptr) y += a.bias[n];
+    if (a.gelu) y = gelu_f(y);
+    if (a.residual != nullptr) y += load_value<BF16>(a.residual, at);
+    store_value<BF16>(a.out, at, y);
+  }
+}
+
+// ---------------------------------------------------------------- host
+template <typename G>
+void by_format(uint32_t format, uint32_t dtype, G go) {
+  auto with = [&](auto f) {
+    if (dtype == DFATTN_KV_BF16)
+      go(f, std::true_type{});
+    else
+      go(f, std::false_type{});
+  };
+  if (format == DFGPT2_W4_I4)
+    with(std::integral_constant<Format, kI4>{});
+  else if (format == DFGPT2_W4_U4)
+    with(std::integral_constant<Format, kU4>{});
+  else
+    with(std::integral_constant<Format, kE2M1>{});
+}
+
+int check_weights(const char *fn, const void *codes, const uint16_t *scales, const void *zeros, uint32_t dtype,
+                  uint32_t format, uint32_t group, uint32_t out_features, uint32_t in_features) {
+  const std::string at = std::string(fn) + ": ";
+  if (dtype != DFATTN_KV_F32 && dtype != DFATTN_KV_BF16)
+    return record_error(DFATTN_ERR_FLAGS, at + "dtype must be DFATTN_KV_F32 or DFATTN_KV_BF16");
+  if (format > DFGPT2_W4_E2M1) return record_error(DFATTN_ERR_FLAGS, at + "format must be one of DFGPT2_W4_*");
+  if (group != 32 && group != 64 && group != 128)
+    return record_error(DFATTN_ERR_SHAPE, at + "a group has 32, 64 or 128 inputs");
+  if (out_features == 0 || in_features == 0)
+    return record_error(DFATTN_ERR_SHAPE, at + "out_features and in_features must be >= 1");
+  if (out_features > kMaxFeatures || in_features > kMaxFeatures)
+    return record_error(DFATTN_ERR_OVERFLOW, at + "shape is too large");
+  if (codes == nullptr || scales == nullptr || (format == DFGPT2_W4_U4 && zeros == nullptr))
+    return record_error(DFATTN_ERR_NULL_POINTER, at + "null pointer");
+  if (reinterpret_cast<uintptr_t>(codes) % 16 != 0 || reinterpret_cast<uintptr_t>(scales) % 2 != 0)
+    return record_error(DFATTN_ERR_MISALIGNED, at + "misaligned pointer");
+  return DFATTN_OK;
+}
+
+int need(const char *fn, std::initializer_list<const void *> ptrs, size_t align) {
+  for (const void *p : ptrs)
+    if (p == nullptr) return record_error(DFATTN_ERR_NULL_POINTER, std::string(fn) + ": null pointer");
+  for (const void *p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % align != 0)
+      return record_error(DFATTN_ERR_MISALIGNED, std::string(fn) + ": misaligned pointer");
+  return DFATTN_OK;
+}
+
+int launched(const char *fn) {
+  const hipError_t err = hipGetLastError();
+  if (err == hipSuccess) return DFATTN_OK;
+  return record_error(DFATTN_ERR_HIP, std::string(fn) + ": " + hipGetErrorString(err));
+}
+
+struct Span {
+  const void *p;
+  size_t bytes;
+};
+bool overlap(const Span &x, const Span &y) {
+  const char *a = static_cast<const char *>(x.p), *b = static_cast<const char *>(y.p);
+  return a != nullptr && b != nullptr && a < b + y.bytes && b < a + x.bytes;
+}
+
+uint32_t log2_of(uint32_t group) { return group == 32 ? 5 : group == 64 ? 6 : 7; }
+uint32_t dwords_of(uint32_t in_features) { return (in_features + 31) / 32 * 4; }
+
+}  // namespace
+}  // namespace dfattn
+
+using namespace dfattn;
+
+extern "C" {
+
+size_t dfgpt2_w4_row_bytes(uint32_t in_features) { return in_features > kMaxFeatures ? 0 : 4 * (size_t)dwords_of(in_features); }
+
+int dfgpt2_w4_quantize(const void *w, void *codes, uint16_t *scales, void *zeros, uint32_t dtype, uint32_t format,
+                       uint32_t group, uint32_t out_features, uint32_t in_features, uint32_t row_stride,
+                       hipStream_t stream) {
+  const char *fn = "dfgpt2_w4_quantize";
+  int st = check_weights(fn, codes, scales, zeros, dtype, format, group, out_features, in_features);
+  if (st == DFATTN_OK) st = need(fn, {w}, dtype == DFATTN_KV_F32 ? 4 : 2);
+  if (st != DFATTN_OK) return st;
+  if (row_stride < in_features)
+    return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": row_stride must be at least in_features");
+  const size_t item = dtype == DFATTN_KV_F32 ? 4 : 2, groups = (in_features + group - 1) / group;
+  const Span spans[] = {{codes, (size_t)out_features * dwords_of(in_features) * 4}, {scales, 2 * groups * out_features},
+                        {format == DFGPT2_W4_U4 ? zeros : nullptr, groups * out_features},
+                        {w, ((size_t)(out_features - 1) * row_stride + in_features) * item}};
+  for (int i = 0; i < 3; ++i)
+    for (int j = i + 1; j < 4; ++j)
+      if (overlap(spans[i], spans[j]))
+        return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": outputs must not overlap inputs or each other");
+  QuantArgs a{w, static_cast<unsigned *>(codes), scales, static_cast<unsigned char *>(zeros), nullptr, row_stride,
+              out_features, in_features, log2_of(group), dwords_of(in_features), (in_features + kQuantCols - 1) / kQuantCols};
+  const dim3 grid = linear_grid((size_t)((out_features + kQuantRows - 1) / kQuantRows) * a.column_blocks);
+  by_format(format, dtype, [&](auto f, auto bf16) {
+    hipLaunchKernelGGL((quantize_kernel<decltype(f)::value, decltype(bf16)::value>), grid, dim3(kThreads), 0, stream, a);
+  });
+  return launched(fn);
+}
+
+int dfgpt2_w4_dequantize(const void *codes, const uint16_t *scales, const void *zeros, void *w, uint32_t dtype,
+                         uint32_t format, uint32_t group, uint32_t out_features, uint32_t in_features,
+                         hipStream_t stream) {
+  const char *fn = "dfgpt2_w4_dequantize";
+  int st = check_weights(fn, codes, scales, zeros, dtype, format, group, out_features, in_features);
+  if (st == DFATTN_OK) st = need(fn, {w}, dtype == DFATTN_KV_F32 ? 4 : 2);
+  if (st != DFATTN_OK) return st;
+  const size_t item = dtype == DFATTN_KV_F32 ? 4 : 2, groups = (in_features + group - 1) / group;
+  const Span to{w, (size_t)out_features * in_features * item};
+  if (overlap(to, {codes, (size_t)out_features * dwords_of(in_features) * 4}) ||
+      overlap(to, {scales, 2 * groups * out_features}) || (format == DFGPT2_W4_U4 && overlap(to, {zeros, groups * out_features})))
+    return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": w must not overlap what is read");
+  QuantArgs a{nullptr, static_cast<unsigned *>(const_cast<void *>(codes)), const_cast<uint16_t *>(scales),
+              static_cast<unsigned char *>(const_cast<void *>(zeros)), w, 0, out_features, in_features, log2_of(group),
+              dwords_of(in_features), 0};
+  const size_t lanes = (size_t)out_features * ((in_features + 7) / 8);
+  by_format(format, dtype, [&](auto f, auto bf16) {
+    hipLaunchKernelGGL((dequantize_kernel<decltype(f)::value, decltype(bf16)::value>),
+                       linear_grid((lanes + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, a);
+  });
+  return launched(fn);
+}
+
+int dfgpt2_w4_linear(const void *x, const void *codes, const uint16_t *scales, const void *zeros, const float *bias,
+                     const void *residual, void *out, uint32_t dtype, uint32_t format, uint32_t group, uint32_t rows,
+                     uint32_t in_features, uint32_t out_features, uint32_t row_stride, uint32_t gelu,
+                     hipStream_t stream) {
+  const char *fn = "dfgpt2_w4_linear";
+  int st = check_weights(fn, codes, scales, zeros, dtype, format, group, out_features, in_features);
+  if (st != DFATTN_OK) return st;
+  if (row_stride < in_features)
+    return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": row_stride must be at least in_features");
+  if (rows > (1u << 20) || (uint64_t)rows * out_features > (1ull << 40) || row_stride > (1u << 28))
+    return record_error(DFATTN_ERR_OVERFLOW, std::string(fn) + ": shape is too large");
+  if (rows == 0) return DFATTN_OK;
+  const size_t item = dtype == DFATTN_KV_F32 ? 4 : 2, groups = (in_features + group - 1) / group;
+  st = need(fn, {x, out}, item);
+  if (st == DFATTN_OK && bias != nullptr) st = need(fn, {bias}, 4);
+  if (st == DFATTN_OK && residual != nullptr) st = need(fn, {residual}, item);
+  if (st != DFATTN_OK) return st;
+  const Span to{out, (size_t)rows * out_features * item};
+  if (overlap(to, {x, ((size_t)(rows - 1) * row_stride + in_features) * item}) ||
+      overlap(to, {codes, (size_t)out_features * dwords_of(in_features) * 4}) ||
+      overlap(to, {scales, 2 * groups * out_features}) ||
+      (format == DFGPT2_W4_U4 && overlap(to, {zeros, groups * out_features})) || overlap(to, {bias, 4 * (size_t)out_features}) ||
+      (residual != out && overlap(to, {residual, to.bytes})))
+    return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": out must not overlap what is read, or be the residual itself");
+  LinearArgs a{x, static_cast<const unsigned *>(codes), scales, static_cast<const unsigned char *>(zeros), bias, residual,
+               out, row_stride, rows, out_features, in_features, log2_of(group), dwords_of(in_features), (int)gelu};
+  const dim3 grid((out_features + 3) / 4, (rows + kRows - 1) / kRows);
+  if (grid.y > 65535u) return record_error(DFATTN_ERR_OVERFLOW, std::string(fn) + ": shape is too large");
+  by_format(format, dtype, [&](auto f, auto bf16) {
+    hipLaunchKernelGGL((linear_kernel<decltype(f)::value, decltype(bf16)::value>), grid, dim3(kThreads), 0, stream, a);
+  });
+  return launched(fn);
+}
+
+}  // extern "C"

@@ -13,7 +13,10 @@ The library's C ABI is include/dfattn.h. This module loads the in-tree build
   ``fused_attention_forward`` / ``attention_backward_host`` (lib.rs:2371, 2421);
 * ``FusedCausalAttention``, a torch.autograd.Function over the fast path;
 * serving batches of requests from a paged 8-bit cache (``paged_plan``,
-  ``kv8_cache``, ``kv8_append``, ``kv8_read``, ``kv8_attention``: kv8.py).
+  ``kv8_cache``, ``kv8_append``, ``kv8_read``, ``kv8_attention``: kv8.py), and
+  the cache's pages between steps (``paged_fork``, ``paged_free``,
+  ``paged_compact``, ``paged_copy``);
+* linear layers with 4-bit weights (the module ``w4``).
 
 There is no CPU fallback: if the library is missing every call raises
 ``DfattnNotBuilt``.
@@ -72,6 +75,11 @@ SYMBOLS = {
     "dfattn_decode_workspace_bytes": (ctypes.c_size_t, [_U32, _U32, _U32]),
     "dfattn_decode": (ctypes.c_int, [_P] * 4 + [_U32, _U32, _P, _P, _U32, _U32, _U32, _F, _P, ctypes.c_size_t, _P]),
     "dfattn_paged_plan": (ctypes.c_int, [_P] * 9 + [_U32] * 6 + [_P]),
+    "dfattn_paged_workspace_bytes": (ctypes.c_size_t, [_U32] * 2),
+    "dfattn_paged_fork": (ctypes.c_int, [_P] * 12 + [_U32] * 5 + [_P, ctypes.c_size_t, _P]),
+    "dfattn_paged_free": (ctypes.c_int, [_P] * 6 + [_U32] * 4 + [_P, ctypes.c_size_t, _P]),
+    "dfattn_paged_compact": (ctypes.c_int, [_P] * 9 + [_U32] * 4 + [_P, ctypes.c_size_t, _P]),
+    "dfattn_paged_copy": (ctypes.c_int, [_P, _U32, _P, _P, _P, _U32, _U32, _P]),
     "dfattn_kv8_pool_bytes": (ctypes.c_size_t, [_U32] * 4),
     "dfattn_kv8_append": (ctypes.c_int, [_P] * 7 + [_U32] * 8 + [_P]),
     "dfattn_kv8_read": (ctypes.c_int, [_P] * 7 + [_U32] * 7 + [_P]),
@@ -663,4 +671,5 @@ class FusedCausalAttention:
 
 # ---------------------------------------------------------------- the paged 8-bit cache
 from .kv8 import (KV_E4M3, KV_I8, KV8Cache, kv8_append, kv8_attention,  # noqa: E402
-                  kv8_attention_workspace_bytes, kv8_cache, kv8_read, paged_plan)
+                  kv8_attention_workspace_bytes, kv8_cache, kv8_read, PagedCompact, PagedFork, PagePools,
+                  page_pools, paged_compact, paged_copy, paged_fork, paged_free, paged_plan)

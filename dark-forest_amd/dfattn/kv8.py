@@ -10,6 +10,14 @@ A step of a serving loop, with nothing read on the host between the calls:
     out, lse = dfattn.kv8_attention(cache, q, block_table, query_start, seq_lens, n_heads, max_q, max_len)
     cached.copy_(seq_lens); free_start.copy_(counts[2:])                        # before the next step
 
+Between steps requests go on more than once (beams, several answers to a prompt), or end, still with nothing read on
+the host; the free list is made again from the tables:
+
+    f = dfattn.paged_fork(block_table, cached, parents, page_size, n_pages)     # row i goes on from row parents[i]
+    dfattn.paged_copy(caches, f.copy_src, f.copy_dst, f.counts)                 # all layers' caches
+    block_table, cached, free_pages, free_start = f.block_table, f.seq_lens, f.free_pages, f.free_start
+    refs, free_pages, free_start = dfattn.paged_free(block_table, cached, page_size, n_pages, ended)
+
 Ids and lengths are int32 tensors, activations float32 or bfloat16, a cache's codes int8 or
 float8_e4m3fn. Tensors live on the current device. What a call allocates (outputs that are not given,
 the workspace) belongs to the stream it runs on.
@@ -18,6 +26,7 @@ from __future__ import annotations
 
 import collections
 import contextlib
+import ctypes
 
 from . import _check, _stream_ptr, _torch, lib
 
@@ -176,6 +185,129 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, free_start, page_
         _ptr(block_table, "block_table", i32, dev), ps, pq, pm, pc, free_pages.numel(), r, block_table.shape[1],
         token_capacity, page_size, n_pages, _stream_ptr(stream)))
     return seq_lens, query_start, slot_map, counts
+
+
+# A batch's rows after a fork: the new table and lengths, how often each page is held, the page ids (held ones, then free
+# ones), the first free one's place, the pairs of pages to copy and counts [2] = pairs, rows cut for want of a page.
+PagedFork = collections.namedtuple("PagedFork", "block_table seq_lens refs free_pages free_start copy_src copy_dst counts")
+PagedCompact = collections.namedtuple("PagedCompact", "block_table refs free_pages free_start copy_src copy_dst counts")
+
+
+def _table(block_table, seq_lens, names):
+    """(pointers of both, R, max_pages) of a batch's table."""
+    if block_table.dim() != 2 or seq_lens.shape != block_table.shape[:1]:
+        raise ValueError("block_table is [R, max_pages], seq_lens [R]")
+    i32, dev = names[1], names[6]
+    return (_ptr(block_table, "block_table", i32, dev), _ptr(seq_lens, "seq_lens", i32, dev)) + tuple(block_table.shape)
+
+
+def _parts(names, on, *sizes):
+    """int32 tensors of these sizes in one allocation, and the pointer of the workspace of the last size behind them."""
+    parts = names[0].empty_strided((sum(sizes),), (1,), dtype=names[1], device=on).split_with_sizes(sizes)
+    return parts[:-1], [t.data_ptr() for t in parts]
+
+
+def paged_fork(block_table, seq_lens, parents, page_size, n_pages, keep_lens=None, new_table=None, stream=None):
+    """dfattn_paged_fork: row i of the result goes on from row parents[i] of block_table [R, max_pages] (none: an id
+    outside 0..R-1), from its seq_lens[parents[i]] tokens or the first keep_lens[i]. new_table [n, max_pages] (allocated
+    where it is not given) keeps what stands behind a row's pages. Returns a PagedFork; follow it with paged_copy."""
+    names = _names()
+    i32, dev = names[1], names[6]
+    pt, pl, r, width = _table(block_table, seq_lens, names)
+    _u32(page_size, "page_size"), _u32(n_pages, "n_pages")
+    n = parents.numel()
+    if keep_lens is not None:
+        _same(keep_lens, "keep_lens", (n,))
+    ws = lib().dfattn_paged_workspace_bytes(n, n_pages)
+    with _on(stream, dev):
+        on = block_table.device
+        if new_table is None:
+            new_table = names[0].empty_strided((n, width), (width, 1), dtype=i32, device=on)
+        _same(new_table, "new_table", (n, width))
+        pages = n_pages if ws else 0  # (0: the call refuses the sizes)
+        parts, ptrs = _parts(names, on, n, pages, pages, 1, n, n, 2, ws // 4)
+    _check(lib().dfattn_paged_fork(
+        pt, pl, _ptr(parents, "parents", i32, dev), None if keep_lens is None else _ptr(keep_lens, "keep_lens", i32, dev),
+        _ptr(new_table, "new_table", i32, dev), *ptrs[:7], r, n, width, page_size, n_pages, ptrs[7], ws, _stream_ptr(stream)))
+    return PagedFork(new_table, *parts)
+
+
+def paged_free(block_table, seq_lens, page_size, n_pages, ended=None, stream=None):
+    """dfattn_paged_free: seq_lens[r] becomes 0 where ended[r] is not 0 (int32). Returns (refs [n_pages], free_pages
+    [n_pages], free_start [1]) of the rows that remain."""
+    names = _names()
+    pt, pl, r, width = _table(block_table, seq_lens, names)
+    _u32(page_size, "page_size"), _u32(n_pages, "n_pages")
+    if ended is not None:
+        _same(ended, "ended", (r,))
+    ws = lib().dfattn_paged_workspace_bytes(r, n_pages)
+    with _on(stream, names[6]):
+        pages = n_pages if ws else 0
+        parts, ptrs = _parts(names, block_table.device, pages, pages, 1, ws // 4)
+    _check(lib().dfattn_paged_free(pt, pl, None if ended is None else _ptr(ended, "ended", names[1], names[6]), *ptrs[:3],
+                                   r, width, page_size, n_pages, ptrs[3], ws, _stream_ptr(stream)))
+    return tuple(parts)
+
+
+def paged_compact(block_table, seq_lens, page_size, n_pages, new_table=None, stream=None):
+    """dfattn_paged_compact: the held pages move below their number. new_table [R, max_pages] may be block_table itself,
+    which it is where it is not given. Returns a PagedCompact (counts [1]: pairs); follow it with paged_copy."""
+    names = _names()
+    pt, pl, r, width = _table(block_table, seq_lens, names)
+    _u32(page_size, "page_size"), _u32(n_pages, "n_pages")
+    new_table = block_table if new_table is None else new_table
+    _same(new_table, "new_table", (r, width))
+    ws = lib().dfattn_paged_workspace_bytes(r, n_pages)
+    with _on(stream, names[6]):
+        pages = n_pages if ws else 0
+        parts, ptrs = _parts(names, block_table.device, pages, pages, 1, pages // 2, pages // 2, 1, ws // 4)
+    _check(lib().dfattn_paged_compact(pt, pl, _ptr(new_table, "new_table", names[1], names[6]), *ptrs[:6], r, width,
+                                      page_size, n_pages, ptrs[6], ws, _stream_ptr(stream)))
+    return PagedCompact(new_table, *parts)
+
+
+class PagePools:
+    """The pools that paged_copy copies in (page_pools makes one): what the library takes, the tensors, their pages."""
+
+    def __init__(self, array, tensors, n_pages, device):
+        self.array, self.tensors, self.n_pages, self.device = array, tensors, n_pages, device
+
+
+def page_pools(pools):
+    """PagePools of a list of tensors [n_pages, ...] (any type, contiguous) and of KV8Caches, to be kept by a program that
+    copies in the same ones each step."""
+    tensors = []
+    for p in pools:
+        tensors.extend(p if isinstance(p, KV8Cache) else (p,))
+    if not tensors:
+        raise ValueError("there must be at least one pool")
+    n_pages, dev = tensors[0].shape[0] if tensors[0].dim() else 0, _names()[6]
+    array = (ctypes.c_size_t * (2 * len(tensors)))()  # (a dfattn_page_pool is a pointer and a size)
+    for i, t in enumerate(tensors):
+        if t.dim() < 1 or t.shape[0] != n_pages or t.numel() == 0:
+            raise ValueError("the pools are [n_pages, ...], of one n_pages and not empty")
+        array[2 * i] = _ptr(t, "a pool", t.dtype, dev)
+        array[2 * i + 1] = t.numel() // n_pages * t.element_size()
+    return PagePools(array, tensors, n_pages, dev)
+
+
+def paged_copy(pools, copy_src, copy_dst, n_copies=None, stream=None):
+    """dfattn_paged_copy: page copy_src[m] to page copy_dst[m] of all pools (a list as page_pools takes, or what it
+    returned), for the first n_copies[0] pairs (a device tensor, such as a fork's counts; None: all)."""
+    names = _names()
+    i32, dev = names[1], names[6]
+    if not isinstance(pools, PagePools):
+        pools = page_pools(pools)
+    if pools.device != dev:
+        raise ValueError("the pools are not on the current device")
+    _check_stream(stream, dev)
+    n = copy_src.numel()
+    _same(copy_src, "copy_src", (n,)), _same(copy_dst, "copy_dst", (n,))
+    if n_copies is not None and n_copies.numel() < 1:
+        raise ValueError("n_copies must have at least one entry")
+    _check(lib().dfattn_paged_copy(
+        pools.array, len(pools.tensors), _ptr(copy_src, "copy_src", i32, dev), _ptr(copy_dst, "copy_dst", i32, dev),
+        None if n_copies is None else _ptr(n_copies, "n_copies", i32, dev), n, pools.n_pages, _stream_ptr(stream)))
 
 
 def kv8_append(cache, k, v, slot_map, stream=None):

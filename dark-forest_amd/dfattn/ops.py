@@ -61,6 +61,10 @@ SYMBOLS = {
     "dfgpt2_linear_backward_weight": (_I, [_P] * 3 + [_U32, _U32, _U32, _P]),
     "dfgpt2_token_logprobs": (_I, [_P] * 7 + [_U32] * 5 + [_P]),
     "dfgpt2_token_logprobs_backward": (_I, [_P] * 7 + [_U32] * 4 + [_P]),
+    "dfgpt2_w4_row_bytes": (_SZ, [_U32]),
+    "dfgpt2_w4_quantize": (_I, [_P] * 4 + [_U32] * 6 + [_P]),
+    "dfgpt2_w4_dequantize": (_I, [_P] * 4 + [_U32] * 5 + [_P]),
+    "dfgpt2_w4_linear": (_I, [_P] * 7 + [_U32] * 8 + [_P]),
     "dfgpt2_layernorm_backward_fused": (_I, [_P] * 11 + [_SZ, _U32, _U32, _P]),
 }
 

@@ -370,6 +370,82 @@ int dfattn_paged_plan(const uint32_t *cached_lens, const uint32_t *new_lens,
                       uint32_t token_capacity, uint32_t page_size,
                       uint32_t n_pages, void *stream);
 
+/* Pages between the steps of a batch. A request holds the first ceil(seq_lens[r]
+ * / page_size) pages of its row of the table (seq_lens past the row count as
+ * its end; ids not below n_pages belong to nobody); several may hold the same
+ * page, and a page that no row holds is free. These calls find that out from
+ * the tables each time: refs [n_pages] receives how often each page is held,
+ * free_pages [n_pages] all ids, first those held and then the free ones, each
+ * in rising order, and free_start [1] the place of the first free one:
+ * what dfattn_paged_plan takes (n_free = n_pages). Rows of a request that has ended
+ * have the length 0.
+ *
+ * fork: the batch's n_children requests go on from parents[i] (any number of
+ * times, or not at all; an id not below n_requests: an empty row), from its
+ * whole length or its first keep_lens[i] tokens (keep_lens may be NULL): row i of
+ * new_table [n_children, max_pages] gets the parent's pages (entries behind
+ * them are left as they are) and new_lens[i] the length. Full pages are
+ * shared. A page that a child will write to behind its tokens must be its own:
+ * the lowest such child keeps it where nobody holds it whole; each other one
+ * gets, in order, the lowest free page, and the pair (page, new page) is listed in
+ * copy_src and copy_dst [n_children] (DFATTN_NO_SLOT behind the last). Where
+ * no page is left, new_lens[i] falls to the last whole page. counts [2]: pairs,
+ * and children cut like that. refs, free_pages and free_start are of the new
+ * rows (with the new pages held). The free pages' contents are kept until they
+ * are given out, so the copies may follow the call.
+ *
+ * free: seq_lens[r] becomes 0 where ended[r] != 0 (ended may be NULL), and refs,
+ * free_pages and free_start are of the rest.
+ *
+ * compact: the pages held move to the ids below their number U, so that a
+ * pool can be cut to U pages: the m-th held id from U on goes to the m-th free one
+ * below, listed in copy_src and copy_dst [n_pages / 2] (DFATTN_NO_SLOT behind
+ * the last); counts [1]: the pairs. new_table [n_requests, max_pages] (may be
+ * block_table itself) gets the rows with their new ids, entries behind them
+ * left as they are. refs, free_pages and free_start are of the new ids.
+ *
+ * All tables have max_pages entries a row; n_requests and n_children are
+ * 1..8192, n_pages up to 2^24, n_pages * page_size and max_pages * page_size up
+ * to 2^31; outputs must not overlap inputs or each other. Workspace:
+ * dfattn_paged_workspace_bytes of the rows of the result; calls that may overlap need one each.
+ * Results do not depend on the order in which the GPU works.                 */
+size_t dfattn_paged_workspace_bytes(uint32_t n_rows, uint32_t n_pages);
+int dfattn_paged_fork(const uint32_t *block_table, const uint32_t *seq_lens,
+                      const uint32_t *parents, const uint32_t *keep_lens,
+                      uint32_t *new_table, uint32_t *new_lens, uint32_t *refs,
+                      uint32_t *free_pages, uint32_t *free_start, uint32_t *copy_src,
+                      uint32_t *copy_dst, uint32_t *counts, uint32_t n_requests,
+                      uint32_t n_children, uint32_t max_pages, uint32_t page_size,
+                      uint32_t n_pages, void *workspace, size_t workspace_bytes,
+                      void *stream);
+int dfattn_paged_free(const uint32_t *block_table, uint32_t *seq_lens, const uint32_t *ended,
+                      uint32_t *refs, uint32_t *free_pages, uint32_t *free_start,
+                      uint32_t n_requests, uint32_t max_pages, uint32_t page_size,
+                      uint32_t n_pages, void *workspace, size_t workspace_bytes,
+                      void *stream);
+int dfattn_paged_compact(const uint32_t *block_table, const uint32_t *seq_lens,
+                         uint32_t *new_table, uint32_t *refs, uint32_t *free_pages,
+                         uint32_t *free_start, uint32_t *copy_src, uint32_t *copy_dst,
+                         uint32_t *counts, uint32_t n_requests, uint32_t max_pages,
+                         uint32_t page_size, uint32_t n_pages, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* The copies of a fork or a compaction: page copy_src[m] of each pool to page
+ * copy_dst[m], for the first *n_copies (at most max_copies; n_copies NULL: all
+ * max_copies) pairs; pairs with an id not below n_pages are left out. pools: an
+ * array of n_pools dfattn_page_pool in host memory (read during the call only): device memory
+ * of n_pages pages of page_bytes (up to 2^30) bytes one after the other, of any
+ * type: the codes and the scales of 8-bit caches, fp32 or bf16 pools, of all
+ * layers in one call. A page that is a destination of two pairs, or a source and
+ * a destination, gets unspecified contents; pools must not overlap.         */
+typedef struct dfattn_page_pool {
+  void *data;
+  size_t page_bytes;
+} dfattn_page_pool;
+int dfattn_paged_copy(const void *pools, uint32_t n_pools, const uint32_t *copy_src,
+                      const uint32_t *copy_dst, const uint32_t *n_copies,
+                      uint32_t max_copies, uint32_t n_pages, void *stream);
+
 /* The 8-bit cache: codes of one byte and, for each page and kv head, one fp32
  * scale; a value is code * scale. k_pool is [n_pages, n_kv_heads, page_size,
  * Dp], v_pool [n_pages, n_kv_heads, Dp, page_size] (a page's values of one

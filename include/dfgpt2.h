@@ -178,6 +178,41 @@ int dfgpt2_token_logprobs_backward(const void *logits, const uint32_t *tokens, c
                                    void *grad_logits, uint32_t dtype, uint32_t rows, uint32_t cols,
                                    uint32_t row_stride, hipStream_t stream);
 
+/* Linear layers with 4-bit weights and a scale for each group of inputs (no reference counterpart), for
+ * generated tokens and chunks beside dfgpt2_linear_forward. A weight matrix [out_features, in_features] is
+ *   codes  [out_features, dfgpt2_w4_row_bytes(in_features)], 16-byte aligned: input 2 b in the low half of
+ *          byte b, input 2 b + 1 in its high half; what lies behind in_features is not looked at;
+ *   scales bf16 [groups, out_features], groups = ceil(in_features / group), group 32, 64 or 128 inputs;
+ *   zeros  one byte [groups, out_features], 0..15 (DFGPT2_W4_U4 only, else not looked at);
+ * value = (code - 8) * scale (DFGPT2_W4_I4), (code - zero) * scale (DFGPT2_W4_U4), or s e m read as the numbers
+ * 0, 1/2, 1, 3/2, 2, 3, 4, 6 (s: negative) * scale (DFGPT2_W4_E2M1).
+ * quantize: w [out_features, in_features] (dtype DFATTN_KV_F32 or DFATTN_KV_BF16, rows row_stride elements
+ * apart). The scale of a group is the bf16 number nearest to its largest magnitude / 7 (I4) or / 6 (E2M1), or to
+ * (high - low) / 15 with low and high its extremes and 0 (U4; zero is -low / scale, rounded, at most 15); a code is
+ * the nearest one, ties to even, at the border where that is past it. All roundings are exact ones of the quotients. A group of
+ * zeros, or whose scale is below bf16's range, has the scale 0 and values 0; one with an infinity or NaN the scale NaN.
+ * dequantize: the values, [out_features, in_features] contiguous, in dtype (exact in fp32, rounded to bf16).
+ * linear: out [rows, out_features] = x W^T + bias, then GELU where gelu is not 0, then + residual, in dtype (x's
+ * type; rows of x row_stride elements apart, at most 2^28; bias fp32; bias and residual may be NULL, residual
+ * [rows, out_features] in dtype may be out itself). Sums are fp32. With bf16 activations every product is exact; a
+ * fp32 activation takes part as the sum of three bf16 terms, which is exact down to 2^-110. An infinity or NaN in a row of x
+ * makes that row's results infinite or NaN; 32 times the sum of a row's magnitudes in a group must stay below fp32's
+ * range. rows <= 2^20; features <= 2^24; outputs must not overlap what is read. Results are reproducible bit for bit. */
+#define DFGPT2_W4_I4 0u
+#define DFGPT2_W4_U4 1u
+#define DFGPT2_W4_E2M1 2u
+size_t dfgpt2_w4_row_bytes(uint32_t in_features);
+int dfgpt2_w4_quantize(const void *w, void *codes, uint16_t *scales, void *zeros, uint32_t dtype, uint32_t format,
+                       uint32_t group, uint32_t out_features, uint32_t in_features, uint32_t row_stride,
+                       hipStream_t stream);
+int dfgpt2_w4_dequantize(const void *codes, const uint16_t *scales, const void *zeros, void *w, uint32_t dtype,
+                         uint32_t format, uint32_t group, uint32_t out_features, uint32_t in_features,
+                         hipStream_t stream);
+int dfgpt2_w4_linear(const void *x, const void *codes, const uint16_t *scales, const void *zeros, const float *bias,
+                     const void *residual, void *out, uint32_t dtype, uint32_t format, uint32_t group, uint32_t rows,
+                     uint32_t in_features, uint32_t out_features, uint32_t row_stride, uint32_t gelu,
+                     hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -32,6 +32,12 @@ pub const DFATTN_KV_I8: u32 = 2;
 pub const DFATTN_KV_E4M3: u32 = 3;
 /// A slot that is none (`dfattn_paged_plan`).
 pub const DFATTN_NO_SLOT: u32 = 0xffffffff;
+/// One pool of `dfattn_paged_copy`.
+#[repr(C)]
+pub struct DfattnPagePool {
+    pub data: *mut c_void,
+    pub page_bytes: usize,
+}
 /// Bytes of the static device array `dfattn_bwd_noalloc` uses as its workspace (per GPU).
 pub const DFATTN_NOALLOC_SCRATCH_BYTES: usize = 32 << 20;
 
@@ -155,6 +161,26 @@ extern "C" {
                              query_start: *mut u32, slot_map: *mut u32, counts: *mut u32, n_free: u32,
                              n_requests: u32, max_pages: u32, token_capacity: u32, page_size: u32,
                              n_pages: u32, stream: *mut c_void) -> c_int;
+    pub fn dfattn_paged_workspace_bytes(n_rows: u32, n_pages: u32) -> usize;
+    pub fn dfattn_paged_fork(block_table: *const u32, seq_lens: *const u32, parents: *const u32,
+                             keep_lens: *const u32, new_table: *mut u32, new_lens: *mut u32, refs: *mut u32,
+                             free_pages: *mut u32, free_start: *mut u32, copy_src: *mut u32,
+                             copy_dst: *mut u32, counts: *mut u32, n_requests: u32, n_children: u32,
+                             max_pages: u32, page_size: u32, n_pages: u32, workspace: *mut c_void,
+                             workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn dfattn_paged_free(block_table: *const u32, seq_lens: *mut u32, ended: *const u32, refs: *mut u32,
+                             free_pages: *mut u32, free_start: *mut u32, n_requests: u32, max_pages: u32,
+                             page_size: u32, n_pages: u32, workspace: *mut c_void, workspace_bytes: usize,
+                             stream: *mut c_void) -> c_int;
+    pub fn dfattn_paged_compact(block_table: *const u32, seq_lens: *const u32, new_table: *mut u32,
+                                refs: *mut u32, free_pages: *mut u32, free_start: *mut u32,
+                                copy_src: *mut u32, copy_dst: *mut u32, counts: *mut u32, n_requests: u32,
+                                max_pages: u32, page_size: u32, n_pages: u32, workspace: *mut c_void,
+                                workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    /// `pools`: an array of `n_pools` [`DfattnPagePool`].
+    pub fn dfattn_paged_copy(pools: *const c_void, n_pools: u32, copy_src: *const u32, copy_dst: *const u32,
+                             n_copies: *const u32, max_copies: u32, n_pages: u32,
+                             stream: *mut c_void) -> c_int;
     pub fn dfattn_kv8_pool_bytes(n_pages: u32, n_kv_heads: u32, page_size: u32, d_head: u32) -> usize;
     pub fn dfattn_kv8_append(k: *const c_void, v: *const c_void, slot_map: *const u32, k_pool: *mut c_void,
                              v_pool: *mut c_void, k_scales: *mut f32, v_scales: *mut f32, act_dtype: u32,

@@ -4,6 +4,11 @@
 
 use std::os::raw::{c_int, c_void};
 
+/// Formats of 4-bit weights (`dfgpt2_w4_*`).
+pub const DFGPT2_W4_I4: u32 = 0;
+pub const DFGPT2_W4_U4: u32 = 1;
+pub const DFGPT2_W4_E2M1: u32 = 2;
+
 #[link(name = "dfattn")]
 extern "C" {
     // The reference's launchers (layernorm.cu:97, 187; elementwise.cu:62, 91, 119, 195, 217, 242, 268, 291;
@@ -88,4 +93,15 @@ extern "C" {
                                           entropy: *const f32, grad_logprob: *const f32,
                                           grad_entropy: *const f32, grad_logits: *mut c_void, dtype: u32,
                                           rows: u32, cols: u32, row_stride: u32, stream: *mut c_void) -> c_int;
+    pub fn dfgpt2_w4_row_bytes(in_features: u32) -> usize;
+    pub fn dfgpt2_w4_quantize(w: *const c_void, codes: *mut c_void, scales: *mut u16, zeros: *mut c_void,
+                              dtype: u32, format: u32, group: u32, out_features: u32, in_features: u32,
+                              row_stride: u32, stream: *mut c_void) -> c_int;
+    pub fn dfgpt2_w4_dequantize(codes: *const c_void, scales: *const u16, zeros: *const c_void, w: *mut c_void,
+                                dtype: u32, format: u32, group: u32, out_features: u32, in_features: u32,
+                                stream: *mut c_void) -> c_int;
+    pub fn dfgpt2_w4_linear(x: *const c_void, codes: *const c_void, scales: *const u16, zeros: *const c_void,
+                            bias: *const f32, residual: *const c_void, out: *mut c_void, dtype: u32,
+                            format: u32, group: u32, rows: u32, in_features: u32, out_features: u32,
+                            row_stride: u32, gelu: u32, stream: *mut c_void) -> c_int;
 }
