@@ -1,0 +1,78 @@
+// gpt2_w4.h — what the 4-bit linear layers' kernels share: formats, types and
+// the products' arguments.
+//
+// codes [outputs, row bytes], input 2 b in the low half of byte b; scales bf16
+// and zeros (one byte) [groups, outputs].
+#pragma once
+
+#include "dfattn_internal.h"
+#include "dfgpt2.h"
+
+namespace dfattn {
+namespace w4 {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+
+enum Format { kI4 = DFGPT2_W4_I4, kU4 = DFGPT2_W4_U4, kE2M1 = DFGPT2_W4_E2M1 };
+
+__device__ __forceinline__ float bf16_value(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
+// To the nearest, ties to even; a NaN stays one.
+__device__ __forceinline__ unsigned short bf16_bits(float f) {
+  const unsigned u = __float_as_uint(f);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)(u >> 16 | 0x40u);
+  return (unsigned short)((u + 0x7fffu + (u >> 16 & 1u)) >> 16);
+}
+template <bool BF16>
+__device__ __forceinline__ float load_value(const void *p, size_t i) {
+  if constexpr (BF16)
+    return bf16_value(static_cast<const unsigned short *>(p)[i]);
+  else
+    return static_cast<const float *>(p)[i];
+}
+template <bool BF16>
+__device__ __forceinline__ void store_value(void *p, size_t i, float v) {
+  if constexpr (BF16)
+    static_cast<unsigned short *>(p)[i] = bf16_bits(v);
+  else
+    static_cast<float *>(p)[i] = v;
+}
+
+struct LinearArgs {
+  const void *x;
+  const unsigned char *codes;
+  const unsigned short *scales;
+  const unsigned char *zeros;
+  const float *bias;
+  const void *residual;
+  void *out;
+  float *partial;  // (matrix_kernel) [splits, M, N], or NULL
+  size_t stride;
+  uint32_t M, N, K, row_bytes, groups;
+  uint32_t log_group;
+  uint32_t k_waves;  // waves of a workgroup that share out the inputs of one block of outputs
+  uint32_t units;    // (vector_kernel) 32 inputs each, of one wave
+  int gelu;
+};
+
+// Up to kVectorRows rows take vector_kernel, up to kStreamRows stream_kernel, more matrix_kernel, whose workgroups take
+// kMatrixRows x kMatrixOutputs results.
+constexpr uint32_t kVectorRows = 2, kStreamRows = 16, kMatrixRows = 32, kMatrixOutputs = 128;
+
+// Splits of the inputs for matrix_kernel: up to 8, for no more than some 512 workgroups, or two where there are
+// up to 512 and many inputs (4096 x 4096 in bf16: 500 rows 42 us whole, 40 in two, 48 in four; 64 rows 23 us whole, 15 in four
+// and in eight).
+inline uint32_t splits_of(uint32_t M, uint32_t N, uint32_t K) {
+  const uint64_t groups = (uint64_t)((M + kMatrixRows - 1) / kMatrixRows) * ((N + kMatrixOutputs - 1) / kMatrixOutputs);
+  const uint32_t tiles = (K + 127) / 128;
+  uint32_t s = 1;
+  while (s < 8 && groups * s * 2 <= 512 && s * 2 <= tiles) s *= 2;
+  return s == 1 && groups <= 512 && tiles >= 16 ? 2 : s;
+}
+
+template <Format F>
+void launch_linear_format(const LinearArgs &a, bool bf16, uint32_t group, float *workspace, hipStream_t stream);
+
+}  // namespace w4
+}  // namespace dfattn

@@ -1,15 +1,8 @@
 // gpt2_w4.hip — linear layers with 4-bit weights and a scale for each group of
-// inputs: quantising, the values back, and the products with bias, GELU and
-// residual (gfx950).
-//
-// codes [outputs, row bytes], input 2 b in the low half of byte b; scales bf16
-// and zeros (one byte) [groups, outputs].
-#include "dfattn_internal.h"
-#include "dfgpt2.h"
+// inputs: quantising, the values back, and the entry points (gfx950).
+#include "gpt2_w4.h"
 #include "dfattn_status.h"
-#include "gpt2_device.h"
 
-#include <algorithm>
 #include <initializer_list>
 #include <string>
 #include <type_traits>
@@ -17,21 +10,10 @@
 namespace dfattn {
 namespace {
 
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+using namespace w4;
 
-constexpr int kThreads = 256;
 constexpr uint32_t kMaxFeatures = 1u << 24;
 
-enum Format { kI4 = DFGPT2_W4_I4, kU4 = DFGPT2_W4_U4, kE2M1 = DFGPT2_W4_E2M1 };
-
-__device__ __forceinline__ float bf16_value(unsigned short b) { return __uint_as_float((unsigned)b << 16); }
-// To the nearest, ties to even; a NaN stays one.
-__device__ __forceinline__ unsigned short bf16_bits(float f) {
-  const unsigned u = __float_as_uint(f);
-  if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)(u >> 16 | 0x40u);
-  return (unsigned short)((u + 0x7fffu + (u >> 16 & 1u)) >> 16);
-}
 // The value of code c (0..15) before its scale.
 template <Format F>
 __device__ __forceinline__ float code_value(unsigned c, float zero) {
@@ -43,21 +25,6 @@ __device__ __forceinline__ float code_value(unsigned c, float zero) {
   } else {
     return (float)c - zero;
   }
-}
-
-template <bool BF16>
-__device__ __forceinline__ float load_value(const void *p, size_t i) {
-  if constexpr (BF16)
-    return bf16_value(static_cast<const unsigned short *>(p)[i]);
-  else
-    return static_cast<const float *>(p)[i];
-}
-template <bool BF16>
-__device__ __forceinline__ void store_value(void *p, size_t i, float v) {
-  if constexpr (BF16)
-    static_cast<unsigned short *>(p)[i] = bf16_bits(v);
-  else
-    static_cast<float *>(p)[i] = v;
 }
 
 // ---------------------------------------------------------------- quantise
@@ -188,51 +155,6 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(QuantArgs a) {
     if (d * 8 + j < a.K) store_value<BF16>(a.out, n * a.K + d * 8 + j, code_value<F>(c >> (4 * j) & 15u, zero) * s);
 }
 
-// ---------------------------------------------------------------- products
-struct LinearArgs {
-  const void *x;
-  const unsigned *codes;
-  const unsigned short *scales;
-  const unsigned char *zeros;
-  const float *bias;
-  const void *residual;
-  void *out;
-  size_t stride;
-  uint32_t M, N, K, log_group, row_dwords;
-  int gelu;
-};
-
-// One output of kRows rows a wave; a lane has 8 inputs at a time, all of one group.
-constexpr int kRows = 4;
-template <Format F, bool BF16>
-__global__ __launch_bounds__(kThreads) void linear_kernel(LinearArgs a) {
-  const uint32_t n = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63, m0 = blockIdx.y * kRows;
-  if (n >= a.N) return;
-  float sum[kRows] = {};
-  for (uint32_t d = lane; d * 8 < a.K; d += 64) {
-    const unsigned c = a.codes[(size_t)n * a.row_dwords + d];
-    const size_t at = (size_t)(d * 8 >> a.log_group) * a.N + n;
-    const float s = bf16_value(a.scales[at]), zero = F == kU4 ? (float)a.zeros[at] : 8.f;
-    for (int r = 0; r < kRows; ++r) {
-      if (m0 + r >= a.M) break;
-      float part = 0.f;
-      for (int j = 0; j < 8; ++j)
-        if (d * 8 + j < a.K) part = fmaf(code_value<F>(c >> (4 * j) & 15u, zero), load_value<BF16>(a.x, (m0 + r) * a.stride + d * 8 + j), part);
-      sum[r] = fmaf(part, s, sum[r]);
-    }
-  }
-  for (int r = 0; r < kRows; ++r) {
-    float y = sum[r];
-    for (int o = 32; o > 0; o >>= 1) y += __shfl_xor(y, o, 64);
-    if (lane != 0 || m0 + r >= a.M) continue;
-    const size_t at = (size_t)(m0 + r) * a.N + n;
-    if (a.bias != nullptr) y += a.bias[n];
-    if (a.gelu) y = gelu_f(y);
-    if (a.residual != nullptr) y += load_value<BF16>(a.residual, at);
-    store_value<BF16>(a.out, at, y);
-  }
-}
-
 // ---------------------------------------------------------------- host
 template <typename G>
 void by_format(uint32_t format, uint32_t dtype, G go) {
@@ -300,6 +222,7 @@ uint32_t dwords_of(uint32_t in_features) { return (in_features + 31) / 32 * 4; }
 }  // namespace dfattn
 
 using namespace dfattn;
+using namespace dfattn::w4;
 
 extern "C" {
 
@@ -354,10 +277,18 @@ int dfgpt2_w4_dequantize(const void *codes, const uint16_t *scales, const void *
   return launched(fn);
 }
 
+size_t dfgpt2_w4_linear_workspace_bytes(uint32_t rows, uint32_t in_features, uint32_t out_features) {
+  if (rows <= kStreamRows || rows > (1u << 20) || in_features == 0 || in_features > kMaxFeatures || out_features == 0 ||
+      out_features > kMaxFeatures)
+    return 0;
+  const uint32_t splits = splits_of(rows, out_features, in_features);
+  return splits == 1 ? 0 : 4 * (size_t)splits * rows * out_features;
+}
+
 int dfgpt2_w4_linear(const void *x, const void *codes, const uint16_t *scales, const void *zeros, const float *bias,
                      const void *residual, void *out, uint32_t dtype, uint32_t format, uint32_t group, uint32_t rows,
                      uint32_t in_features, uint32_t out_features, uint32_t row_stride, uint32_t gelu,
-                     hipStream_t stream) {
+                     void *workspace, size_t workspace_bytes, hipStream_t stream) {
   const char *fn = "dfgpt2_w4_linear";
   int st = check_weights(fn, codes, scales, zeros, dtype, format, group, out_features, in_features);
   if (st != DFATTN_OK) return st;
@@ -367,7 +298,11 @@ int dfgpt2_w4_linear(const void *x, const void *codes, const uint16_t *scales, c
     return record_error(DFATTN_ERR_OVERFLOW, std::string(fn) + ": shape is too large");
   if (rows == 0) return DFATTN_OK;
   const size_t item = dtype == DFATTN_KV_F32 ? 4 : 2, groups = (in_features + group - 1) / group;
+  const size_t need_bytes = dfgpt2_w4_linear_workspace_bytes(rows, in_features, out_features);
+  if (workspace != nullptr && workspace_bytes < need_bytes)
+    return record_error(DFATTN_ERR_WORKSPACE, std::string(fn) + ": the workspace is too small");
   st = need(fn, {x, out}, item);
+  if (st == DFATTN_OK && workspace != nullptr && need_bytes > 0) st = need(fn, {workspace}, 4);
   if (st == DFATTN_OK && bias != nullptr) st = need(fn, {bias}, 4);
   if (st == DFATTN_OK && residual != nullptr) st = need(fn, {residual}, item);
   if (st != DFATTN_OK) return st;
@@ -376,15 +311,19 @@ int dfgpt2_w4_linear(const void *x, const void *codes, const uint16_t *scales, c
       overlap(to, {codes, (size_t)out_features * dwords_of(in_features) * 4}) ||
       overlap(to, {scales, 2 * groups * out_features}) ||
       (format == DFGPT2_W4_U4 && overlap(to, {zeros, groups * out_features})) || overlap(to, {bias, 4 * (size_t)out_features}) ||
-      (residual != out && overlap(to, {residual, to.bytes})))
+      (residual != out && overlap(to, {residual, to.bytes})) || overlap(to, {need_bytes > 0 ? workspace : nullptr, need_bytes}))
     return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": out must not overlap what is read, or be the residual itself");
-  LinearArgs a{x, static_cast<const unsigned *>(codes), scales, static_cast<const unsigned char *>(zeros), bias, residual,
-               out, row_stride, rows, out_features, in_features, log2_of(group), dwords_of(in_features), (int)gelu};
-  const dim3 grid((out_features + 3) / 4, (rows + kRows - 1) / kRows);
-  if (grid.y > 65535u) return record_error(DFATTN_ERR_OVERFLOW, std::string(fn) + ": shape is too large");
-  by_format(format, dtype, [&](auto f, auto bf16) {
-    hipLaunchKernelGGL((linear_kernel<decltype(f)::value, decltype(bf16)::value>), grid, dim3(kThreads), 0, stream, a);
-  });
+  LinearArgs a{x, static_cast<const unsigned char *>(codes), scales,
+               static_cast<const unsigned char *>(zeros), bias, residual, out, nullptr, row_stride,
+               rows, out_features, in_features, 4 * dwords_of(in_features), (uint32_t)groups, log2_of(group), 1, 1, (int)gelu};
+  float *sums = need_bytes > 0 ? static_cast<float *>(workspace) : nullptr;
+  const bool bf16 = dtype == DFATTN_KV_BF16;
+  if (format == DFGPT2_W4_I4)
+    launch_linear_format<kI4>(a, bf16, group, sums, stream);
+  else if (format == DFGPT2_W4_U4)
+    launch_linear_format<kU4>(a, bf16, group, sums, stream);
+  else
+    launch_linear_format<kE2M1>(a, bf16, group, sums, stream);
   return launched(fn);
 }
 

@@ -64,7 +64,8 @@ SYMBOLS = {
     "dfgpt2_w4_row_bytes": (_SZ, [_U32]),
     "dfgpt2_w4_quantize": (_I, [_P] * 4 + [_U32] * 6 + [_P]),
     "dfgpt2_w4_dequantize": (_I, [_P] * 4 + [_U32] * 5 + [_P]),
-    "dfgpt2_w4_linear": (_I, [_P] * 7 + [_U32] * 8 + [_P]),
+    "dfgpt2_w4_linear_workspace_bytes": (_SZ, [_U32] * 3),
+    "dfgpt2_w4_linear": (_I, [_P] * 7 + [_U32] * 8 + [_P, _SZ, _P]),
     "dfgpt2_layernorm_backward_fused": (_I, [_P] * 11 + [_SZ, _U32, _U32, _P]),
 }
 

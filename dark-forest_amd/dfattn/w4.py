@@ -77,10 +77,14 @@ def dequantize(w, dtype=None, out=None, stream=None):
     return out
 
 
-def linear(x, w, bias=None, residual=None, gelu=False, out=None, stream=None):
+def linear_workspace_bytes(rows, in_features, out_features):
+    return ops_lib().dfgpt2_w4_linear_workspace_bytes(rows, in_features, out_features)
+
+
+def linear(x, w, bias=None, residual=None, gelu=False, out=None, workspace="auto", stream=None):
     """dfgpt2_w4_linear: x W^T + bias, then GELU where gelu is true, then + residual; x [rows, inputs] (float32 or
     bfloat16, rows may be a column block), bias [outputs] float32, residual and out [rows, outputs] in x's type (out may be
-    the residual)."""
+    the residual). workspace: "auto" allocates dfgpt2_w4_linear_workspace_bytes, None does without."""
     names = _names()
     dev = names[6]
     *ptrs, fmt, group, n, k = _weight(w, names)
@@ -92,8 +96,12 @@ def linear(x, w, bias=None, residual=None, gelu=False, out=None, stream=None):
         raise ValueError(f"residual must be {list(shape)}")
     with _on(stream, dev):
         out, po = _out(out, "out", shape, x.dtype, x.device, names)
+        if isinstance(workspace, str):
+            need = linear_workspace_bytes(shape[0], k, n) if shape[0] > 16 else 0
+            workspace = names[0].empty((need // 4,), dtype=names[2], device=x.device) if need else None
+    ws, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace, "workspace", names[2], dev), workspace.numel() * 4)
     _check(ops_lib().dfgpt2_w4_linear(
         px, *ptrs, None if bias is None else _ptr(bias, "bias", names[2], dev),
         None if residual is None else _ptr(residual, "residual", x.dtype, dev), po, dtype, fmt, group, shape[0], k, n, stride,
-        1 if gelu else 0, _stream_ptr(stream)))
+        1 if gelu else 0, ws, ws_bytes, _stream_ptr(stream)))
     return out

@@ -197,7 +197,9 @@ int dfgpt2_token_logprobs_backward(const void *logits, const uint32_t *tokens, c
  * [rows, out_features] in dtype may be out itself). Sums are fp32. With bf16 activations every product is exact; a
  * fp32 activation takes part as the sum of three bf16 terms, which is exact down to 2^-110. An infinity or NaN in a row of x
  * makes that row's results infinite or NaN; 32 times the sum of a row's magnitudes in a group must stay below fp32's
- * range. rows <= 2^20; features <= 2^24; outputs must not overlap what is read. Results are reproducible bit for bit. */
+ * range. rows <= 2^20; features <= 2^24; outputs must not overlap what is read. Workspace:
+ * dfgpt2_w4_linear_workspace_bytes (0: none needed; 4-byte aligned), one for each call that may overlap; NULL: the inputs
+ * are not shared out, slower for some 17 to 200 rows. Results are reproducible bit for bit. */
 #define DFGPT2_W4_I4 0u
 #define DFGPT2_W4_U4 1u
 #define DFGPT2_W4_E2M1 2u
@@ -208,10 +210,11 @@ int dfgpt2_w4_quantize(const void *w, void *codes, uint16_t *scales, void *zeros
 int dfgpt2_w4_dequantize(const void *codes, const uint16_t *scales, const void *zeros, void *w, uint32_t dtype,
                          uint32_t format, uint32_t group, uint32_t out_features, uint32_t in_features,
                          hipStream_t stream);
+size_t dfgpt2_w4_linear_workspace_bytes(uint32_t rows, uint32_t in_features, uint32_t out_features);
 int dfgpt2_w4_linear(const void *x, const void *codes, const uint16_t *scales, const void *zeros, const float *bias,
                      const void *residual, void *out, uint32_t dtype, uint32_t format, uint32_t group, uint32_t rows,
                      uint32_t in_features, uint32_t out_features, uint32_t row_stride, uint32_t gelu,
-                     hipStream_t stream);
+                     void *workspace, size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -100,8 +100,10 @@ extern "C" {
     pub fn dfgpt2_w4_dequantize(codes: *const c_void, scales: *const u16, zeros: *const c_void, w: *mut c_void,
                                 dtype: u32, format: u32, group: u32, out_features: u32, in_features: u32,
                                 stream: *mut c_void) -> c_int;
+    pub fn dfgpt2_w4_linear_workspace_bytes(rows: u32, in_features: u32, out_features: u32) -> usize;
     pub fn dfgpt2_w4_linear(x: *const c_void, codes: *const c_void, scales: *const u16, zeros: *const c_void,
                             bias: *const f32, residual: *const c_void, out: *mut c_void, dtype: u32,
                             format: u32, group: u32, rows: u32, in_features: u32, out_features: u32,
-                            row_stride: u32, gelu: u32, stream: *mut c_void) -> c_int;
+                            row_stride: u32, gelu: u32, workspace: *mut c_void, workspace_bytes: usize,
+                            stream: *mut c_void) -> c_int;
 }
