@@ -227,6 +227,169 @@ __global__ __launch_bounds__(kThreads) void rename_kernel(PagesArgs a) {
   }
 }
 
+// ---------------------------------------------------------------- small batches: one workgroup, one launch
+constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
+constexpr uint32_t kSmallPages = 8192, kSmallRows = 2048, kSmallEntries = 32768, kStrips = kSmallPages / kSmallThreads;
+
+// The five steps above with everything in LDS between barriers.
+template <Mode M>
+__global__ __launch_bounds__(kSmallThreads) void small_kernel(PagesArgs a) {
+  // first, last: fork: the lowest row that writes in a page and how many do; compact: the pages that move, and where to.
+  __shared__ uint32_t refs[kSmallPages], first[M == kFree ? 1 : kSmallPages], last[M == kFree ? 1 : kSmallPages];
+  __shared__ uint32_t from[M == kFork ? kSmallRows : 1], pages[kSmallRows], opened[M == kFork ? kSmallRows : 1];
+  __shared__ uint32_t counts[kStrips * kSmallWaves], holes_lds, needs;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (uint32_t p = tid; p < a.n_pages; p += kSmallThreads) {
+    refs[p] = 0;
+    if constexpr (M == kFork) {
+      first[p] = kNone;
+      last[p] = 0;
+    }
+  }
+  if (tid < kStrips * kSmallWaves) counts[tid] = 0;
+  if (tid == 0) holes_lds = 0;
+  for (uint32_t i = tid; i < a.N; i += kSmallThreads) {
+    const Row r = row_of<M>(a, i);
+    pages[i] = r.pages;
+    if constexpr (M == kFork) {
+      from[i] = r.from;
+      opened[i] = open_page(a, r);
+      a.new_lens[i] = r.len;
+    }
+    if (M == kFree && a.ended != nullptr && a.ended[i] != 0) a.new_lens[i] = 0;
+  }
+  __syncthreads();
+  // A wave takes 64 entries of a row at a time.
+  const uint32_t parts = (a.W + 63) / 64;
+  for (uint32_t item = wave; item < a.N * parts; item += kSmallWaves) {
+    const uint32_t i = item / parts, j = item % parts * 64 + lane;
+    if (j >= pages[i]) continue;
+    const uint32_t p = a.table[(size_t)(M == kFork ? from[i] : i) * a.W + j];
+    if constexpr (M == kFork) a.new_table[(size_t)i * a.W + j] = p;
+    if (p < a.n_pages) atomicAdd(refs + p, 1u);
+  }
+  if constexpr (M == kFork)
+    for (uint32_t i = tid; i < a.N; i += kSmallThreads)
+      if (opened[i] != kNone) {
+        atomicMin(first + opened[i], i);
+        atomicAdd(last + opened[i], 1u);
+      }
+  __syncthreads();
+  // The free pages of each 64.
+  for (uint32_t strip = 0; strip * kSmallThreads < a.n_pages; ++strip) {
+    const uint32_t p = strip * kSmallThreads + tid;
+    const uint64_t free = __ballot(p < a.n_pages && refs[p] == 0);
+    if (lane == 0) counts[strip * kSmallWaves + wave] = __popcll(free);
+  }
+  uint32_t need = 0;
+  if constexpr (M == kFork) {
+    if (wave == 0) {  // (the rows in order; their places go where their pages were)
+      for (uint32_t i0 = 0; i0 < a.N; i0 += 64) {
+        const uint32_t i = i0 + lane, p = i < a.N ? opened[i] : kNone;
+        const bool takes = p != kNone && (first[p] != i || refs[p] != last[p]);
+        const uint64_t who = __ballot(takes);
+        if (takes) from[need + __popcll(who & ((1ull << lane) - 1))] = i;  // (`from` has been read)
+        need += __popcll(who);
+      }
+      if (lane == 0) needs = need;
+    }
+  }
+  __syncthreads();
+  if constexpr (M == kFork) need = needs;
+  if (wave == 0) {  // sums before each 64, over all
+    static_assert(kStrips * kSmallWaves == 128, "two a lane");
+    const uint32_t x = counts[2 * lane], y = counts[2 * lane + 1];
+    uint32_t s = x + y;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t t = __shfl_up(s, o, 64);
+      if ((int)lane >= o) s += t;
+    }
+    counts[2 * lane] = s - x - y;
+    counts[2 * lane + 1] = s - y;
+    if (lane == 63) holes_lds = s;
+  }
+  __syncthreads();
+  const uint32_t n_free = holes_lds, used = a.n_pages - n_free;
+  if constexpr (M == kCompact) {
+    __syncthreads();
+    for (uint32_t strip = 0; strip * kSmallThreads < a.n_pages; ++strip) {
+      const uint32_t p = strip * kSmallThreads + tid;
+      const bool free = p < a.n_pages && refs[p] == 0;
+      const uint32_t k = counts[strip * kSmallWaves + wave] + __popcll(__ballot(free) & ((1ull << lane) - 1));
+      if (p >= a.n_pages) continue;
+      a.order[p] = p;
+      if (free && p < used) last[k] = p;  // the m-th free page below
+      if (p == used) holes_lds = k;
+      if (p + 1 == a.n_pages && used == a.n_pages) holes_lds = 0;
+    }
+    __syncthreads();
+    const uint32_t moves = holes_lds;
+    for (uint32_t strip = 0; strip * kSmallThreads < a.n_pages; ++strip) {
+      const uint32_t p = strip * kSmallThreads + tid;
+      const bool free = p < a.n_pages && refs[p] == 0;
+      const uint32_t k = counts[strip * kSmallWaves + wave] + __popcll(__ballot(free) & ((1ull << lane) - 1));
+      if (p >= a.n_pages) continue;
+      if (p < used) {
+        if (!free) a.refs[p] = refs[p];
+        continue;
+      }
+      a.refs[p] = 0;
+      if (free) continue;
+      const uint32_t m = p - k - (used - moves), to = last[m];
+      first[p] = to;
+      a.src[m] = p;
+      a.dst[m] = to;
+      a.refs[to] = refs[p];
+    }
+    for (uint32_t k = moves + tid; k < a.n_pairs; k += kSmallThreads) a.src[k] = a.dst[k] = kNone;
+    if (tid == 0) {
+      *a.free_start = used;
+      a.counts[0] = moves;
+    }
+    __syncthreads();
+    for (uint32_t item = wave; item < a.N * parts; item += kSmallWaves) {
+      const uint32_t i = item / parts, j = item % parts * 64 + lane;
+      if (j >= pages[i]) continue;
+      const uint32_t p = a.table[(size_t)i * a.W + j];
+      a.new_table[(size_t)i * a.W + j] = p >= used && p < a.n_pages ? first[p] : p;
+    }
+    return;
+  }
+  const uint32_t pairs = M == kFork ? min(need, n_free) : 0;
+  if constexpr (M == kFork)
+    for (uint32_t k = tid; k < a.N; k += kSmallThreads) {
+      if (k >= pairs) a.src[k] = a.dst[k] = kNone;
+      if (k >= need) continue;
+      const uint32_t i = from[k];
+      atomicSub(refs + opened[i], 1u);  // (never to 0: the page's owner, or a row that has it whole, stays)
+      if (k >= pairs) a.new_lens[i] = row_of<M>(a, i).len / a.P * a.P;
+    }
+  __syncthreads();
+  for (uint32_t strip = 0; strip * kSmallThreads < a.n_pages; ++strip) {
+    const uint32_t p = strip * kSmallThreads + tid;
+    const uint32_t n = p < a.n_pages ? refs[p] : 1;
+    const uint32_t k = counts[strip * kSmallWaves + wave] + __popcll(__ballot(n == 0) & ((1ull << lane) - 1));
+    if (p >= a.n_pages) continue;
+    a.order[n == 0 ? used + k : p - k] = p;
+    const bool taken = M == kFork && n == 0 && k < pairs;
+    a.refs[p] = taken ? 1 : n;
+    if (M == kFork && taken) {
+      const uint32_t i = from[k];
+      a.new_table[(size_t)i * a.W + pages[i] - 1] = p;
+      a.src[k] = opened[i];
+      a.dst[k] = p;
+    }
+  }
+  if (tid == 0) {
+    *a.free_start = used + pairs;
+    if constexpr (M == kFork) {
+      a.counts[0] = pairs;
+      a.counts[1] = need - pairs;
+    }
+  }
+}
+
 // ---------------------------------------------------------------- copies
 struct Pool {
   char *data;
@@ -264,10 +427,33 @@ __device__ __forceinline__ void copy_pool(const CopyArgs &a, T *data, uint32_t u
   }
 }
 
+// Pages of many units: a workgroup copies kPiece of one page at a time. The copies are not
+// read again soon, so their stores pass the caches by (80 MB copied 25 us, 27 with plain ones).
+constexpr uint32_t kPieceSteps = 4, kPiece = kPieceSteps * kThreads;
+__device__ __forceinline__ void copy_pages(const CopyArgs &a, u32x4 *data, uint32_t units, uint32_t n) {
+  const uint32_t pieces = (units + kPiece - 1) / kPiece;
+  const uint64_t total = (uint64_t)n * pieces;
+  for (uint64_t item = blockIdx.x; item < total; item += gridDim.x) {
+    const uint32_t pair = (uint32_t)(item / pieces), at = (uint32_t)(item % pieces) * kPiece + threadIdx.x;
+    const uint32_t s = a.src[pair], d = a.dst[pair];
+    if (s >= a.n_pages || d >= a.n_pages) continue;
+    const u32x4 *from = data + (size_t)s * units;
+    u32x4 *to = data + (size_t)d * units, x[kPieceSteps];
+#pragma unroll
+    for (uint32_t j = 0; j < kPieceSteps; ++j)
+      if (at + j * kThreads < units) x[j] = from[at + j * kThreads];
+#pragma unroll
+    for (uint32_t j = 0; j < kPieceSteps; ++j)
+      if (at + j * kThreads < units) __builtin_nontemporal_store(x[j], to + at + j * kThreads);
+  }
+}
+
 __global__ __launch_bounds__(kThreads) void copy_kernel(CopyArgs a) {
   const Pool pool = a.pools[blockIdx.y];
   const uint32_t n = a.count != nullptr ? min(*a.count, a.max_copies) : a.max_copies;
-  if (pool.log2 == 4)
+  if (pool.log2 == 4 && pool.units >= kThreads)
+    copy_pages(a, reinterpret_cast<u32x4 *>(pool.data), pool.units, n);
+  else if (pool.log2 == 4)
     copy_pool(a, reinterpret_cast<u32x4 *>(pool.data), pool.units, n);
   else if (pool.log2 == 2)
     copy_pool(a, reinterpret_cast<uint32_t *>(pool.data), pool.units, n);
@@ -311,6 +497,11 @@ int run_pages(const char *fn, PagesArgs &a, void *workspace, size_t workspace_by
   if (workspace == nullptr || workspace_bytes < workspace_bytes_for(a.N, a.n_pages))
     return record_error(DFATTN_ERR_WORKSPACE, std::string(fn) + ": the workspace is too small");
   if (!aligned_to(workspace, 4)) return record_error(DFATTN_ERR_MISALIGNED, std::string(fn) + ": misaligned pointer");
+  // One workgroup as long as it is about as fast as the others' five launches.
+  if (a.n_pages <= kSmallPages && a.N <= kSmallRows && (uint64_t)a.N * a.W <= kSmallEntries) {
+    hipLaunchKernelGGL(small_kernel<M>, dim3(1), dim3(kSmallThreads), 0, stream, a);
+    return launched(fn);
+  }
   a.owner = static_cast<uint32_t *>(workspace);
   a.lasts = a.owner + a.n_pages;
   a.sums = a.lasts + a.n_pages;
@@ -487,8 +678,8 @@ int dfattn_paged_copy(const void *pools, uint32_t n_pools, const uint32_t *copy_
       a.pools[i] = {static_cast<char *>(p.data), (uint32_t)(p.page_bytes >> log2), log2};
       most = std::max(most, (uint64_t)max_copies * a.pools[i].units);
     }
-    // About 2048 workgroups in all.
-    const uint32_t each = std::max(1u, 2048 / n);
+    // About 8192 workgroups in all (1.2 GB of 32 KB pages 246 us, with 2048 266).
+    const uint32_t each = std::max(1u, 8192 / n);
     const uint32_t groups = (uint32_t)std::min<uint64_t>(each, (most + 4 * kThreads - 1) / (4 * kThreads));
     hipLaunchKernelGGL(copy_kernel, dim3(groups, n), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
   }

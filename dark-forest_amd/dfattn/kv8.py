@@ -24,9 +24,9 @@ the workspace) belongs to the stream it runs on.
 """
 from __future__ import annotations
 
+import array
 import collections
 import contextlib
-import ctypes
 
 from . import _check, _stream_ptr, _torch, lib
 
@@ -269,26 +269,29 @@ def paged_compact(block_table, seq_lens, page_size, n_pages, new_table=None, str
 class PagePools:
     """The pools that paged_copy copies in (page_pools makes one): what the library takes, the tensors, their pages."""
 
-    def __init__(self, array, tensors, n_pages, device):
-        self.array, self.tensors, self.n_pages, self.device = array, tensors, n_pages, device
+    def __init__(self, fields, tensors, n_pages, device):
+        self.fields, self.tensors, self.n_pages, self.device = fields, tensors, n_pages, device
 
 
 def page_pools(pools):
     """PagePools of a list of tensors [n_pages, ...] (any type, contiguous) and of KV8Caches, to be kept by a program that
     copies in the same ones each step."""
-    tensors = []
-    for p in pools:
-        tensors.extend(p if isinstance(p, KV8Cache) else (p,))
-    if not tensors:
-        raise ValueError("there must be at least one pool")
-    n_pages, dev = tensors[0].shape[0] if tensors[0].dim() else 0, _names()[6]
-    array = (ctypes.c_size_t * (2 * len(tensors)))()  # (a dfattn_page_pool is a pointer and a size)
-    for i, t in enumerate(tensors):
-        if t.dim() < 1 or t.shape[0] != n_pages or t.numel() == 0:
-            raise ValueError("the pools are [n_pages, ...], of one n_pages and not empty")
-        array[2 * i] = _ptr(t, "a pool", t.dtype, dev)
-        array[2 * i + 1] = t.numel() // n_pages * t.element_size()
-    return PagePools(array, tensors, n_pages, dev)
+    if KV8Cache in map(type, pools):
+        tensors = [t for p in pools for t in (p if type(p) is KV8Cache else (p,))]
+    else:
+        tensors = list(pools)
+    dev = _names()[6]
+    # (A list for each question: 48 pools 14 us, tensor after tensor 35.)
+    for t in [t for t in tensors if t.get_device() != dev or not t.is_contiguous()]:
+        _ptr(t, "a pool", t.dtype, dev)
+    pages, sizes = {t.shape[:1] for t in tensors}, [t.nbytes for t in tensors]
+    if len(pages) != 1 or 0 in sizes or () in pages:
+        raise ValueError("there must be at least one pool, all [n_pages, ...] of one n_pages and not empty")
+    n_pages = next(iter(pages))[0]
+    fields = array.array("Q", bytes(16 * len(tensors)))  # (a dfattn_page_pool is a pointer and a size)
+    fields[0::2] = array.array("Q", [t.data_ptr() for t in tensors])
+    fields[1::2] = array.array("Q", [s // n_pages for s in sizes])
+    return PagePools(fields, tensors, n_pages, dev)
 
 
 def paged_copy(pools, copy_src, copy_dst, n_copies=None, stream=None):
@@ -306,7 +309,7 @@ def paged_copy(pools, copy_src, copy_dst, n_copies=None, stream=None):
     if n_copies is not None and n_copies.numel() < 1:
         raise ValueError("n_copies must have at least one entry")
     _check(lib().dfattn_paged_copy(
-        pools.array, len(pools.tensors), _ptr(copy_src, "copy_src", i32, dev), _ptr(copy_dst, "copy_dst", i32, dev),
+        pools.fields.buffer_info()[0], len(pools.tensors), _ptr(copy_src, "copy_src", i32, dev), _ptr(copy_dst, "copy_dst", i32, dev),
         None if n_copies is None else _ptr(n_copies, "n_copies", i32, dev), n, pools.n_pages, _stream_ptr(stream)))
 
 
