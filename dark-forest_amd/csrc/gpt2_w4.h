@@ -39,6 +39,16 @@ __device__ __forceinline__ void store_value(void *p, size_t i, float v) {
     static_cast<float *>(p)[i] = v;
 }
 
+// v of the lane that a DPP control names.
+template <int CONTROL>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CONTROL, 0xf, 0xf, false);
+}
+template <int CONTROL>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(dpp<CONTROL>(__float_as_uint(v)));
+}
+
 struct LinearArgs {
   const void *x;
   const unsigned char *codes;

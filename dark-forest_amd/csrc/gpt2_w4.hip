@@ -62,16 +62,21 @@ struct Divider {
     float c = __builtin_rintf(x * inv);
     const float r = fmaf(-c, s, x);
     const bool odd = ((int)c & 1) != 0;
-    if (r > half || (r == half && odd))
-      c += 1.f;
-    else if (r < -half || (r == -half && odd))
-      c -= 1.f;
+    if (fabsf(r) > half || (fabsf(r) == half && odd)) c += r > 0.f ? 1.f : -1.f;
     return c;
   }
+  // The same without the correction; *far grows to the largest remainder. Right for all x where that stays below near().
+  __device__ __forceinline__ float first(float x, float *far) const {
+    const float c = __builtin_rintf(x * inv);
+    *far = fmaxf(*far, fabsf(fmaf(-c, s, x)));
+    return c;
+  }
+  __device__ __forceinline__ float near() const { return f == 1.f ? half * (1.f - 0x1p-20f) : 0.f; }
 };
 
 // A workgroup takes 32 outputs and 256 inputs: a lane 8 inputs of four outputs, 4 to 16 neighbours a
-// group. The scales go through LDS, so that neighbouring outputs' are written together.
+// group. Each of four neighbours divides for one of the four outputs. The scales go through LDS, so that neighbouring
+// outputs' are written together.
 constexpr int kQuantRows = 32, kQuantCols = 256;
 template <Format F, bool BF16>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
@@ -81,36 +86,85 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
   if (n0 >= a.N) return;
   const uint32_t lane = threadIdx.x & 31, d = k0 / 8 + lane, lanes = 1u << (a.log_group - 3);
   float x[4][8];
+  const char *w = static_cast<const char *>(a.w) + ((n0 + (threadIdx.x >> 5)) * a.stride + d * 8) * (BF16 ? 2 : 4);
+  const size_t rows8 = 8 * a.stride * (BF16 ? 2 : 4);
+  if (n0 + kQuantRows <= a.N && k0 + kQuantCols <= a.K) {
+    if constexpr (BF16) {  // (all loads before the first use)
+      unsigned v[4][4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) __builtin_memcpy(v[r], w + r * rows8, 16);
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[r][j] = __uint_as_float(j & 1 ? v[r][j / 2] & 0xffff0000u : v[r][j / 2] << 16);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) __builtin_memcpy(x[r], w + r * rows8, 32);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        x[r][j] = n0 + 8 * r + (threadIdx.x >> 5) < a.N && d * 8 + j < a.K ? load_value<BF16>(w + r * rows8, j) : 0.f;
+  }
+  // The groups' extremes: the largest magnitude by its bits (an infinity or NaN is above all numbers), and with zero
+  // points the lowest and highest, over 4, 8 or 16 neighbouring lanes.
+  auto among = [&](auto v, auto better) {
+    v = better(v, dpp<0xb1>(v));
+    v = better(v, dpp<0x4e>(v));
+    if (lanes > 4) v = better(v, dpp<0x141>(v));
+    if (lanes > 8) v = better(v, dpp<0x140>(v));
+    return v;
+  };
+  float lo[4], hi[4];
+  unsigned most[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    const uint32_t n = n0 + 8 * r + (threadIdx.x >> 5);
+    lo[r] = hi[r] = 0.f;
+    most[r] = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      x[r][j] = n < a.N && d * 8 + j < a.K ? load_value<BF16>(a.w, n * a.stride + d * 8 + j) : 0.f;
+    for (int j = 0; j < 8; ++j) {
+      if (F == kU4) {
+        lo[r] = fminf(lo[r], x[r][j]);
+        hi[r] = fmaxf(hi[r], x[r][j]);
+      }
+      most[r] = max(most[r], __float_as_uint(x[r][j]) & 0x7fffffffu);
+    }
+    if (F == kU4) {
+      lo[r] = among(lo[r], [](float a, float b) { return fminf(a, b); });
+      hi[r] = among(hi[r], [](float a, float b) { return fmaxf(a, b); });
+    }
+    most[r] = among(most[r], [](unsigned a, unsigned b) { return max(a, b); });
   }
+  const uint32_t which = lane & 3;
+  float low = lo[0], high = F == kU4 ? hi[0] : __uint_as_float(most[0]);
+#pragma unroll
+  for (uint32_t r = 1; r < 4; ++r) {
+    low = which == r ? lo[r] : low;
+    high = which == r ? F == kU4 ? hi[r] : __uint_as_float(most[r]) : high;
+  }
+  const double top = F == kU4 ? ((double)high - (double)low) / 15.0 : (double)high / (F == kI4 ? 7.0 : 6.0);
+  const unsigned near = nearest_bf16(top);
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const uint32_t row = 8 * r + (threadIdx.x >> 5), n = n0 + row;
-    float lo = 0.f, hi = 0.f;
-    int bad = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lo = fminf(lo, x[r][j]);
-      hi = fmaxf(hi, x[r][j]);
-      bad |= !(fabsf(x[r][j]) < __builtin_inff());
-    }
-    for (uint32_t o = 1; o < lanes; o <<= 1) {
-      lo = fminf(lo, __shfl_xor(lo, (int)o, 64));
-      hi = fmaxf(hi, __shfl_xor(hi, (int)o, 64));
-      bad |= __shfl_xor(bad, (int)o, 64);
-    }
-    const double top = F == kU4 ? ((double)hi - (double)lo) / 15.0 : (double)fmaxf(hi, -lo) / (F == kI4 ? 7.0 : 6.0);
-    const unsigned short bits = bad ? 0x7fc0u : nearest_bf16(top);
+    const unsigned short bits = most[r] >= 0x7f800000u ? 0x7fc0u : (unsigned short)__shfl((int)near, (int)((threadIdx.x & 63 & ~3u) + r), 64);
     const float s = bf16_value(bits);
     const bool some = s > 0.f;  // (neither 0 nor NaN)
     const Divider by(some ? s : 1.f);
     float zero = F == kI4 ? 8.f : 0.f;
-    if (F == kU4 && some) zero = fminf(fmaxf(by.nearest(-lo), 0.f), 15.f);
+    if (F == kU4 && some) zero = fminf(fmaxf(by.nearest(-lo[r]), 0.f), 15.f);
+    float v[8], far = 0.f;
+    if constexpr (F != kE2M1) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = by.first(x[r][j], &far);
+      // (Few values are next to a border: 16384 x 4096 weights with the correction always 70 us, like this 67.)
+      if (__any(some && !(far < by.near()))) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = by.nearest(x[r][j]);
+      }
+    }
     unsigned c = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -121,8 +175,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
             (y > 5.f * s);
         q = some ? q | (__float_as_uint(x[r][j]) >> 31 << 3) : 0u;
       } else {
-        const float v = (some ? by.nearest(x[r][j]) : 0.f) + zero;
-        q = (unsigned)fminf(fmaxf(v, 0.f), 15.f);
+        q = (unsigned)fminf(fmaxf((some ? v[j] : 0.f) + zero, 0.f), 15.f);
       }
       c |= q << (4 * j);
     }
@@ -140,19 +193,43 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
 }
 
 // ---------------------------------------------------------------- values
+// A lane writes 16 bytes at a time, neighbours next to each other: 4 fp32 or 8 bf16 values of a row; kValueSteps
+// times 256 lanes a workgroup.
+constexpr uint32_t kValueSteps = 8;
 template <Format F, bool BF16>
 __global__ __launch_bounds__(kThreads) void dequantize_kernel(QuantArgs a) {
-  const size_t id = (size_t)linear_block() * kThreads + threadIdx.x;
-  const uint32_t per_row = (a.K + 7) / 8;
-  const size_t n = id / per_row;
-  const uint32_t d = (uint32_t)(id % per_row);
-  if (n >= a.N) return;
-  const unsigned c = a.codes[n * a.row_dwords + d];
-  const size_t at = (size_t)(d * 8 >> a.log_group) * a.N + n;
-  const float s = bf16_value(a.scales[at]), zero = F == kU4 ? (float)a.zeros[at] : 8.f;
+  constexpr uint32_t V = BF16 ? 8 : 4;
+  const uint32_t per_row = (a.K + V - 1) / V;
+  const size_t base = (size_t)linear_block() * (kThreads * kValueSteps), row0 = base / per_row;
+  const uint32_t at0 = (uint32_t)(base % per_row);
+  const unsigned char *codes = reinterpret_cast<const unsigned char *>(a.codes);
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (d * 8 + j < a.K) store_value<BF16>(a.out, n * a.K + d * 8 + j, code_value<F>(c >> (4 * j) & 15u, zero) * s);
+  for (uint32_t i = 0; i < kValueSteps; ++i) {
+    const uint32_t at = at0 + i * kThreads + threadIdx.x, k = at % per_row * V;
+    const size_t n = row0 + at / per_row;
+    if (n >= a.N) return;
+    unsigned c;
+    if constexpr (BF16)
+      c = *reinterpret_cast<const unsigned *>(codes + n * a.row_dwords * 4 + k / 2);
+    else
+      c = *reinterpret_cast<const unsigned short *>(codes + n * a.row_dwords * 4 + k / 2);
+    const size_t group = (size_t)(k >> a.log_group) * a.N + n;
+    const float s = bf16_value(a.scales[group]), zero = F == kU4 ? (float)a.zeros[group] : 8.f;
+    float v[V];
+#pragma unroll
+    for (uint32_t j = 0; j < V; ++j) v[j] = code_value<F>(c >> (4 * j) & 15u, zero) * s;
+    if (k + V <= a.K) {
+      u32x4 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o[j] = BF16 ? (unsigned)bf16_bits(v[2 * j % V]) | (unsigned)bf16_bits(v[(2 * j + 1) % V]) << 16 : __float_as_uint(v[j]);
+      __builtin_memcpy(static_cast<char *>(a.out) + (n * a.K + k) * (BF16 ? 2 : 4), &o, 16);
+    } else {
+#pragma unroll
+      for (uint32_t j = 0; j < V; ++j)
+        if (k + j < a.K) store_value<BF16>(a.out, n * a.K + k + j, v[j]);
+    }
+  }
 }
 
 // ---------------------------------------------------------------- host
@@ -269,10 +346,10 @@ int dfgpt2_w4_dequantize(const void *codes, const uint16_t *scales, const void *
   QuantArgs a{nullptr, static_cast<unsigned *>(const_cast<void *>(codes)), const_cast<uint16_t *>(scales),
               static_cast<unsigned char *>(const_cast<void *>(zeros)), w, 0, out_features, in_features, log2_of(group),
               dwords_of(in_features), 0};
-  const size_t lanes = (size_t)out_features * ((in_features + 7) / 8);
+  const size_t values = dtype == DFATTN_KV_F32 ? 4 : 8, lanes = (size_t)out_features * ((in_features + values - 1) / values);
   by_format(format, dtype, [&](auto f, auto bf16) {
     hipLaunchKernelGGL((dequantize_kernel<decltype(f)::value, decltype(bf16)::value>),
-                       linear_grid((lanes + kThreads - 1) / kThreads), dim3(kThreads), 0, stream, a);
+                       linear_grid((lanes + kThreads * kValueSteps - 1) / (kThreads * kValueSteps)), dim3(kThreads), 0, stream, a);
   });
   return launched(fn);
 }

@@ -481,7 +481,7 @@ int check_pages(const char *fn, uint32_t n_requests, uint32_t n_rows, uint32_t m
   return DFATTN_OK;
 }
 
-uint32_t pages_per_block(uint32_t n_pages) { return std::max(1024u, ((n_pages + 1023) / 1024 + 1023) & ~1023u); }
+uint32_t pages_per_block(uint32_t n_pages) { return std::max(256u, ((n_pages + 1023) / 1024 + 255) & ~255u); }
 
 size_t workspace_bytes_for(uint32_t n_rows, uint32_t n_pages) {
   return 4 * (2 * (size_t)n_pages + 1024 + n_rows + 1);
