@@ -44,12 +44,6 @@ struct Eight<true> {
   u32x4 r;
   static constexpr int kTerms = 1;
   __device__ __forceinline__ void load(const char *p) { __builtin_memcpy(&r, p, 16); }
-  __device__ __forceinline__ float sum() const {
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s += __uint_as_float(r[j] << 16) + __uint_as_float(r[j] & 0xffff0000u);
-    return s;
-  }
   __device__ __forceinline__ void load_some(const char *p, int n) {  // the first n
     unsigned x[8];
 #pragma unroll
@@ -70,7 +64,6 @@ struct Eight<false> {
   float r[8];
   static constexpr int kTerms = 3;
   __device__ __forceinline__ void load(const char *p) { __builtin_memcpy(r, p, 32); }
-  __device__ __forceinline__ float sum() const { return ((r[0] + r[1]) + (r[2] + r[3])) + ((r[4] + r[5]) + (r[6] + r[7])); }
   __device__ __forceinline__ void load_some(const char *p, int n) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = j < n ? reinterpret_cast<const float *>(p)[j] : 0.f;
@@ -472,24 +465,27 @@ __global__ __launch_bounds__(512) void vector_kernel(LinearArgs a) {
   }
 }
 
-// More rows: a workgroup of four waves takes R x 16 rows and 4 T x 16 outputs. x goes through LDS, 128 inputs at a
+// More rows: a workgroup of four waves takes 32 rows and 128 outputs, a wave 32 of those. x goes through LDS, 128 inputs at a
 // time in two buffers, as operands that are made once for the four waves: [term][product][16 rows][quarter][row], 16 bytes
 // each, the row's place turned by the 8 inputs' number so that neither the writes (16 pieces of a row) nor the reads meet in
-// banks. The groups' sums of x (for the zero points) are added on the way. Codes come straight from memory, as above.
+// banks. Codes come straight from memory, as above. A group's products are scaled once, sum += s (sum q x); what
+// the zero points take off, sum over the groups of (sum x)(zero s), is a product itself: four groups at a time on the fp32
+// matrix instruction, with the groups' sums of x by products with ones, 16 rows each by two of the waves.
 // Where rows and outputs give too few workgroups, `splits` share out the inputs and leave fp32 sums, which join_kernel adds.
 template <Format F, bool BF16, int GROUP>
-__global__ __launch_bounds__(kThreads) void matrix_kernel(LinearArgs a) {
+__global__ __launch_bounds__(kThreads, 2) void matrix_kernel(LinearArgs a) {  // (2: no sums in accumulation registers)
   constexpr bool E2M1 = F == kE2M1;
   constexpr int R = kMatrixRows / 16, T = kMatrixOutputs / 64;
   constexpr int kGroups = 128 / GROUP, kSteps = GROUP / 32;
   constexpr int kTerms = Eight<BF16>::kTerms, kItem = BF16 ? 2 : 4;
   __shared__ f32x4 operands[2][kTerms][4][R][64];
-  __shared__ f32x4 x_sums[2][kGroups][R * 4];
+  __shared__ f32x4 x_sums[2][4][R * 4];  // of four groups
   const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t n0 = (xcd_block(blockIdx.x, gridDim.x) * 4 + wave) * (16 * T), m0 = blockIdx.y * (16 * R);
   const uint32_t tiles = (a.K + 127) / 128;
   const uint32_t t0 = (uint32_t)((uint64_t)tiles * blockIdx.z / gridDim.z), t1 = (uint32_t)((uint64_t)tiles * (blockIdx.z + 1) / gridDim.z);
+  const uint32_t g1 = min(t1 * kGroups, a.groups);
   const unsigned char *codes[T];
   uint32_t n[T];
 #pragma unroll
@@ -499,15 +495,19 @@ __global__ __launch_bounds__(kThreads) void matrix_kernel(LinearArgs a) {
   }
   struct Codes {
     u32x4 c[T];
-    unsigned scale[T], zero[F == kU4 ? T : 1];  // of group `quarter` of the tile
   };
   auto load_codes = [&](uint32_t tile, Codes &d) {
-    const uint32_t g = tile * kGroups + (kGroups == 1 ? 0 : quarter % kGroups);
-    const size_t at = (size_t)min(g, a.groups - 1) * a.N;
     const bool there = tile * 64 + 16 * quarter < a.row_bytes;
 #pragma unroll
+    for (int t = 0; t < T; ++t) d.c[t] = *reinterpret_cast<const u32x4 *>(codes[t] + (there ? tile * 64 : 0));  // (x is 0 behind the inputs)
+  };
+  struct Scales {
+    unsigned scale[T], zero[F == kU4 ? T : 1];  // of group first + quarter
+  };
+  auto load_scales = [&](uint32_t first, Scales &d) {
+    const size_t at = (size_t)min(first + quarter, a.groups - 1) * a.N;
+#pragma unroll
     for (int t = 0; t < T; ++t) {
-      d.c[t] = *reinterpret_cast<const u32x4 *>(codes[t] + (there ? tile * 64 : 0));  // (x is 0 behind the inputs)
       d.scale[t] = a.scales[at + n[t]];
       if constexpr (F == kU4) d.zero[t] = a.zeros[at + n[t]];
     }
@@ -515,36 +515,33 @@ __global__ __launch_bounds__(kThreads) void matrix_kernel(LinearArgs a) {
   // Staging: a thread has 8 inputs of R rows.
   const uint32_t octet = threadIdx.x & 15, row = threadIdx.x >> 4;
   const uint32_t step = GROUP == 128 ? octet & 3 : octet >> 2, part = GROUP == 128 ? octet >> 2 : octet & 3;
-  Eight<BF16> x[R];
-  auto load_x = [&](uint32_t tile) {
+  struct Inputs {
+    Eight<BF16> x[R];
+  };
+  auto load_x = [&](uint32_t tile, Inputs &in) {
     const uint32_t k = tile * 128 + octet * 8;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint32_t m = m0 + 16 * r + row;
       const char *at = static_cast<const char *>(a.x) + ((size_t)min(m, a.M - 1) * a.stride + k) * kItem;
       if (tile * 128 + 128 <= a.K)
-        x[r].load(at);
+        in.x[r].load(at);
       else
-        x[r].load_some(at, (int)a.K - (int)k);
+        in.x[r].load_some(at, (int)a.K - (int)k);
     }
   };
-  auto stage = [&](int buffer) {
+  auto stage = [&](int buffer, const Inputs &in) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       bf16x8 term[kTerms];
-      x[r].template terms<E2M1>(term);
+      in.x[r].template terms<E2M1>(term);
 #pragma unroll
       for (int k = 0; k < kTerms; ++k) operands[buffer][k][step][r][part * 16 + (row ^ octet)] = __builtin_bit_cast(f32x4, term[k]);
-      if constexpr (!E2M1) {
-        float v = x[r].sum();
-        // Over the group's 4, 8 or 16 neighbouring lanes: neighbours, pairs, mirrored halves of 8, of 16.
-        v += dpp<0xb1>(v);
-        v += dpp<0x4e>(v);
-        if (GROUP > 32) v += dpp<0x141>(v);
-        if (GROUP > 64) v += dpp<0x140>(v);
-        if (octet % (GROUP / 8) == 0) reinterpret_cast<float *>(x_sums[buffer][octet / (GROUP / 8)])[16 * r + row] = v;
-      }
     }
+  };
+  auto operand = [&](int buffer, int k, int s, uint32_t r) {
+    const uint32_t o = GROUP == 128 ? quarter * 4 + s : s * 4 + quarter;
+    return __builtin_bit_cast(bf16x8, operands[buffer][k][s][r][quarter * 16 + (col ^ o)]);
   };
 
   f32x4 sum[T][R];
@@ -562,25 +559,49 @@ __global__ __launch_bounds__(kThreads) void matrix_kernel(LinearArgs a) {
     x = r[0];
     y = r[1];
   };
-  // A quarter's value in all lanes, for quarters 0 .. kGroups - 1.
-  auto spread = [&](unsigned v, unsigned (&to)[kGroups]) {
-    to[0] = v;
-    if constexpr (kGroups == 2) {
-      unsigned even = v, odd = v;
-      swap16(even, odd);
-      to[0] = even, to[1] = odd;
-    } else if constexpr (kGroups == 4) {
-      unsigned low = v, high = v;
-      swap32(low, high);
+  unsigned scale[T][4];  // of the four groups at hand
+  float taken[T] = {};   // - zero * scale of group `quarter` of the four before
+  // The four groups from `first` on come next: their scales, from `d`.
+  auto next_four = [&](uint32_t first, const Scales &d, float (&take)[T]) {
+    const bool real = first + quarter < g1;  // (behind them x is 0, or another split's)
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      unsigned low = real ? d.scale[t] : 0u, high = low;
+      take[t] = -bf16_value((unsigned short)low) * (F == kU4 ? (float)d.zero[t] : 8.f);
+      swap32(low, high);  // quarters 0 1 0 1, 2 3 2 3
       unsigned low2 = low, high2 = high;
       swap16(low, low2);
       swap16(high, high2);
-      to[0] = low, to[1] = low2, to[2] = high, to[3] = high2;
+      scale[t][0] = low, scale[t][1] = low2, scale[t][2] = high, scale[t][3] = high2;
     }
   };
-  auto use = [&](uint32_t tile, int buffer, const Codes &d) {
-    unsigned v[T][4], scale[T][kGroups], zero[T][kGroups];
-    const uint32_t g = tile * kGroups + (kGroups == 1 ? 0 : quarter % kGroups);
+  // What the zero points of four groups take off.
+  auto take_off = [&](uint32_t first, int fours) {
+    if constexpr (!E2M1) {
+      const bool real = first + quarter < g1;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const float xs = reinterpret_cast<const float *>(x_sums[fours][quarter])[16 * r + col];
+#pragma unroll
+        for (int t = 0; t < T; ++t) sum[t][r] = __builtin_amdgcn_mfma_f32_16x16x4f32(real ? xs : 0.f, taken[t], sum[t][r], 0, 0, 0);
+      }
+    }
+  };
+  const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
+  // One tile; its groups are numbers `at` .. of the four.
+  auto use = [&](int buffer, const Codes &d, int at, int fours) {
+    if (!E2M1 && wave < R) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        f32x4 xs = {};
+#pragma unroll
+        for (int s = g * kSteps; s < (g + 1) * kSteps; ++s)
+#pragma unroll
+          for (int k = 0; k < kTerms; ++k) xs = mfma16(operand(buffer, k, s, wave), ones, xs);
+        if (col == 0) x_sums[fours][at + g][4 * wave + quarter] = xs;
+      }
+    }
+    unsigned v[T][4];
 #pragma unroll
     for (int t = 0; t < T; ++t) {
 #pragma unroll
@@ -591,8 +612,6 @@ __global__ __launch_bounds__(kThreads) void matrix_kernel(LinearArgs a) {
         swap16(v[t][0], v[t][1]);
         swap16(v[t][2], v[t][3]);
       }
-      spread(g < a.groups ? d.scale[t] : 0u, scale[t]);  // (behind the inputs the sums are 0)
-      if constexpr (F == kU4) spread(d.zero[t], zero[t]);
     }
 #pragma unroll
     for (int g = 0; g < kGroups; ++g) {
@@ -607,50 +626,60 @@ __global__ __launch_bounds__(kThreads) void matrix_kernel(LinearArgs a) {
         bf16x8 w[T];
 #pragma unroll
         for (int t = 0; t < T; ++t) w[t] = operand_of<E2M1>(v[t][s]);
-        const uint32_t o = GROUP == 128 ? quarter * 4 + s : s * 4 + quarter;
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int k = 0; k < kTerms; ++k) {
-            const bf16x8 in = __builtin_bit_cast(bf16x8, operands[buffer][k][s][r][quarter * 16 + (col ^ o)]);
+            const bf16x8 in = operand(buffer, k, s, r);
 #pragma unroll
             for (int t = 0; t < T; ++t) acc[t][r] = mfma16(in, w[t], acc[t][r]);
           }
       }
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        f32x4 xs = {};
-        if constexpr (!E2M1) xs = x_sums[buffer][g][4 * r + quarter];
+      for (int t = 0; t < T; ++t) {
+        const float f = __uint_as_float(scale[t][at + g] << 16);
 #pragma unroll
-        for (int t = 0; t < T; ++t) {
-          const float f = __uint_as_float(scale[t][g] << 16), z = F == kU4 ? (float)zero[t][g] : 8.f;
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            sum[t][r][e] = fmaf(f, E2M1 ? acc[t][r][e] : fmaf(-z, xs[e], acc[t][r][e]), sum[t][r][e]);
-        }
+          for (int e = 0; e < 4; ++e) sum[t][r][e] = fmaf(f, acc[t][r][e], sum[t][r][e]);
       }
     }
   };
+  // Rounds of four tiles, which hold kGroups times four groups. Codes and activations come one tile ahead (two: 2000 rows of
+  // 4096 x 4096 122 us for 113, as three workgroups a CU are left of four).
   Codes d[2];
+  Inputs in;
+  Scales sc;
   if (t0 < t1) {
-    load_x(t0);
+    load_x(t0, in);
     load_codes(t0, d[0]);
-    stage(0);
+    load_scales(t0 * kGroups, sc);
+    stage(0, in);
     __syncthreads();
-    auto round = [&](uint32_t tile, int buffer, Codes &now, Codes &next) {
-      const bool more = tile + 1 < t1;
-      if (more) {
-        load_x(tile + 1);  // (loads come back in order: what is waited for first, first)
-        load_codes(tile + 1, next);
+    for (uint32_t tile = t0; tile < t1; tile += 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (tile + i >= t1) break;
+        const bool more = tile + i + 1 < t1;
+        const uint32_t group = (tile + i) * kGroups;
+        if (more) {
+          load_x(tile + i + 1, in);  // (loads come back in order: what is waited for first, first)
+          load_codes(tile + i + 1, d[(i + 1) % 2]);
+        }
+        // (The sums of x of the four groups before were written before the last barrier.)
+        const int fours = kGroups == 1 ? (int)((tile - t0) / 4 % 2) : i * kGroups / 4 % 2;
+        if (i * kGroups % 4 == 0) {
+          if (tile + i > t0) take_off(group - 4, fours ^ 1);
+          next_four(group, sc, taken);
+          load_scales(group + 4, sc);
+        }
+        use(i % 2, d[i % 2], i * kGroups % 4, fours);
+        if (more) stage((i + 1) % 2, in);
+        __syncthreads();
       }
-      use(tile, buffer, now);
-      if (more) stage(buffer ^ 1);
-      __syncthreads();
-    };
-    for (uint32_t tile = t0; tile < t1; tile += 2) {
-      round(tile, 0, d[0], d[1]);
-      if (tile + 1 < t1) round(tile + 1, 1, d[1], d[0]);
     }
+    const uint32_t last = (t1 - t0 - 1) * kGroups / 4;  // the last four groups
+    take_off(t0 * kGroups + 4 * last, (int)(last % 2));
   }
 #pragma unroll
   for (int t = 0; t < T; ++t) {

@@ -51,7 +51,7 @@ def gelu64(y):
     return 0.5 * y * (1 + torch.tanh(math.sqrt(2 / math.pi) * (y + 0.044715 * y ** 3)))
 
 
-def check(x, w, bias=None, residual=None, gelu=False, out=None):
+def check(x, w, bias=None, residual=None, gelu=False, out=None, **kw):
     want, g = values(w), torch.arange(w.in_features, device="cuda") // w.group
     y = x.double() @ want.t().contiguous()
     size = x.double().abs() @ w.scales.double().t()[:, g].t().contiguous() * 15
@@ -65,7 +65,7 @@ def check(x, w, bias=None, residual=None, gelu=False, out=None):
     if residual is not None:
         y = y + residual.double()
         bound = bound + 2.0 ** -24 * y.abs()
-    got = w4.linear(x, w, bias, residual, gelu, out)
+    got = w4.linear(x, w, bias, residual, gelu, out, **kw)
     assert got.dtype == x.dtype and got.shape == y.shape
     far = (got.double() - y).abs() - bound - HALF[x.dtype] * (y.abs() + bound)
     assert far.max() <= 0, (far.max().item(), y.abs().max().item())
@@ -156,6 +156,17 @@ def test_linear_sizes(device, fmt, group, dtype, rows, n, k):
     x = torch.randn(rows, k, generator=generator(k), device="cuda").to(dtype)
     bias = torch.randn(n, generator=generator(n), device="cuda") if k % 2 else None
     check(x, weight(2, n, k, group, fmt), bias)
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n,k", [(1, 70, 4500), (2, 70, 2100), (4, 70, 5000), (16, 40, 9000), (33, 140, 4321), (200, 1100, 2048)])
+def test_linear_many_inputs(device, fmt, group, dtype, rows, n, k):
+    """Many tiles of inputs, whole and shared out, and without a workspace."""
+    x = torch.randn(rows, k, generator=generator(k), device="cuda").to(dtype)
+    w = weight(3, n, k, group, fmt)
+    check(x, w)
+    check(x, w, workspace=None)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
