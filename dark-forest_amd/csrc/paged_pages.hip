@@ -678,8 +678,9 @@ int dfattn_paged_copy(const void *pools, uint32_t n_pools, const uint32_t *copy_
       a.pools[i] = {static_cast<char *>(p.data), (uint32_t)(p.page_bytes >> log2), log2};
       most = std::max(most, (uint64_t)max_copies * a.pools[i].units);
     }
-    // About 8192 workgroups in all (1.2 GB of 32 KB pages 246 us, with 2048 266).
-    const uint32_t each = std::max(1u, 8192 / n);
+    // Up to 4096 workgroups in all (1.2 GB of 32 KB pages 254 us, with 2048 266, with 8192 249; but 300 a us start, also
+    // where *n_copies turns out to be small).
+    const uint32_t each = std::max(1u, 4096 / n);
     const uint32_t groups = (uint32_t)std::min<uint64_t>(each, (most + 4 * kThreads - 1) / (4 * kThreads));
     hipLaunchKernelGGL(copy_kernel, dim3(groups, n), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
   }

@@ -194,10 +194,10 @@ int dfgpt2_token_logprobs_backward(const void *logits, const uint32_t *tokens, c
  * dequantize: the values, [out_features, in_features] contiguous, in dtype (exact in fp32, rounded to bf16).
  * linear: out [rows, out_features] = x W^T + bias, then GELU where gelu is not 0, then + residual, in dtype (x's
  * type; rows of x row_stride elements apart, at most 2^28; bias fp32; bias and residual may be NULL, residual
- * [rows, out_features] in dtype may be out itself). Sums are fp32. With bf16 activations every product is exact; a
- * fp32 activation takes part as the sum of three bf16 terms, which is exact down to 2^-110. An infinity or NaN in a row of x
- * makes that row's results infinite or NaN; 32 times the sum of a row's magnitudes in a group must stay below fp32's
- * range. rows <= 2^20; features <= 2^24; outputs must not overlap what is read. Workspace:
+ * [rows, out_features] in dtype may be out itself). Every activation times code is exact (a fp32 activation takes part
+ * as the sum of three bf16 terms, exactly from 2^-100 on) and summed in fp32; a group's sum is scaled once. An infinity
+ * or NaN in a row of x makes that row's results infinite or NaN; 32 times the sum of a row's magnitudes in a group,
+ * and that times the group's scale, must stay below fp32's range. rows <= 2^20; features <= 2^24; outputs must not overlap what is read. Workspace:
  * dfgpt2_w4_linear_workspace_bytes (0: none needed; 4-byte aligned), one for each call that may overlap; NULL: the inputs
  * are not shared out, slower for some 17 to 200 rows. Results are reproducible bit for bit. */
 #define DFGPT2_W4_I4 0u

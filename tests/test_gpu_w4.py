@@ -169,6 +169,16 @@ def test_linear_many_inputs(device, fmt, group, dtype, rows, n, k):
     check(x, w, workspace=None)
 
 
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n,k", [(1, 16389, 300), (2, 16389, 300), (1, 16399, 1000), (2, 16399, 1000), (1, 16390, 1100), (2, 9000, 2200),
+                                      (3, 16401, 300), (16, 16401, 300), (5, 8300, 900), (9, 33000, 300), (34, 16401, 300)])
+def test_linear_many_outputs(device, fmt, group, dtype, rows, n, k):
+    """Layers wide enough for the forms that give a wave more outputs."""
+    x = torch.randn(rows, k, generator=generator(k + rows), device="cuda").to(dtype)
+    check(x, weight(4, n, k, group, fmt), torch.randn(n, generator=generator(n), device="cuda"))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,n,k", [(1, 768, 768), (4, 1000, 640), (50, 77, 300), (150, 200, 512)])
 def test_epilogue(device, dtype, rows, n, k):
@@ -234,17 +244,25 @@ def test_far_values(device, dtype):
     check((torch.randn(4, k, generator=g, device="cuda") * torch.exp2(e)).to(dtype), w)
 
 
-def test_exact_products(device):
-    """fp32 activations of 24 bits, one at a time: nothing of them is lost."""
-    n, k = 32, 128
-    w = weight(8, n, k, 128, "i4")
-    x = torch.zeros(k, k, device="cuda")
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("rows,n", [(1, 40), (2, 16400), (16, 40), (16, 16400), (1024, 40), (1024, 150)])
+def test_exact_products(device, fmt, group, rows, n):
+    """fp32 activations of 24 bits, one at a time in each of 1024 places: nothing of them is lost, wherever it stands.
+
+    The code's product (28 bits, added up from three) is rounded at most twice to 24 bits at up to 15 |x| scale, the zero point's share and
+    the scaled sum once each: 3 * 15 |x| scale and |result|, times 2^-24."""
+    k = 1024
+    w = weight(8, n, k, group, fmt)
     v = (torch.randint(2 ** 23, 2 ** 24, (k,), generator=generator(1), device="cuda") | 1).float()
-    x[torch.arange(k), torch.arange(k)] = v
-    got = w4.linear(x, w).double()
-    want = v.double()[:, None] * values(w).t()
-    # The code's product (28 bits) and the zero point's share are each rounded to 24 bits, and so is the scaled sum.
-    assert ((got - want).abs() <= 2.0 ** -24 * (3 * 15 * v.double()[:, None] * w.scales.double() + want.abs())).all()
+    exact, g = values(w), torch.arange(k, device="cuda") // group
+    for first in range(0, k, rows if rows > 2 else 37):
+        at = (first + torch.arange(rows, device="cuda")) % k
+        x = torch.zeros(rows, k, device="cuda")
+        x[torch.arange(rows), at] = v[at]
+        got = w4.linear(x, w).double()
+        size = v[at].double()[:, None]
+        want = size * exact[:, at].t()
+        assert ((got - want).abs() <= 2.0 ** -24 * (3 * 15 * size * w.scales.double()[g[at]] + want.abs())).all(), first
 
 
 def test_streams_and_capture(device):
