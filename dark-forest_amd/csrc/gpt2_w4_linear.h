@@ -472,10 +472,10 @@ __global__ __launch_bounds__(512) void vector_kernel(LinearArgs a) {
 // the zero points take off, sum over the groups of (sum x)(zero s), is a product itself: four groups at a time on the fp32
 // matrix instruction, with the groups' sums of x by products with ones, 16 rows each by two of the waves.
 // Where rows and outputs give too few workgroups, `splits` share out the inputs and leave fp32 sums, which join_kernel adds.
-template <Format F, bool BF16, int GROUP>
+template <Format F, bool BF16, int GROUP, int R>
 __global__ __launch_bounds__(kThreads, 2) void matrix_kernel(LinearArgs a) {  // (2: no sums in accumulation registers)
   constexpr bool E2M1 = F == kE2M1;
-  constexpr int R = kMatrixRows / 16, T = kMatrixOutputs / 64;
+  constexpr int T = kMatrixOutputs / 64;
   constexpr int kGroups = 128 / GROUP, kSteps = GROUP / 32;
   constexpr int kTerms = Eight<BF16>::kTerms, kItem = BF16 ? 2 : 4;
   __shared__ f32x4 operands[2][kTerms][4][R][64];
@@ -590,7 +590,7 @@ __global__ __launch_bounds__(kThreads, 2) void matrix_kernel(LinearArgs a) {  //
   const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
   // One tile; its groups are numbers `at` .. of the four.
   auto use = [&](int buffer, const Codes &d, int at, int fours) {
-    if (!E2M1 && wave < R) {
+    if (!E2M1 && wave < (uint32_t)R) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) {
         f32x4 xs = {};
@@ -793,7 +793,10 @@ void launch_matrix(const LinearArgs &args, float *workspace, hipStream_t stream)
   uint32_t splits = workspace == nullptr ? 1 : splits_of(a.M, a.N, a.K);
   if (splits > 1) a.partial = workspace;
   const dim3 grid((a.N + kMatrixOutputs - 1) / kMatrixOutputs, (a.M + kMatrixRows - 1) / kMatrixRows, splits);
-  hipLaunchKernelGGL((matrix_kernel<F, BF16, GROUP>), grid, dim3(kThreads), 0, stream, a);
+  if (a.M <= 16)
+    hipLaunchKernelGGL((matrix_kernel<F, BF16, GROUP, 1>), grid, dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((matrix_kernel<F, BF16, GROUP, kMatrixRows / 16>), grid, dim3(kThreads), 0, stream, a);
   if (splits == 1) return;
   const size_t groups = ((size_t)a.M * a.N + kThreads - 1) / kThreads;
   hipLaunchKernelGGL((join_kernel<BF16>), dim3((uint32_t)std::min<size_t>(2048, groups)), dim3(kThreads), 0, stream, a, splits);
@@ -805,13 +808,14 @@ void launch_linear_format(const LinearArgs &a, bool bf16, uint32_t group, float 
   auto with_group = [&](auto b, auto g) {
     constexpr bool B = decltype(b)::value;
     constexpr int G = decltype(g)::value;
-    // (fp32 rows make three operands each, which matrix_kernel does once for 128 outputs: from 8 rows on faster where no
-    // inputs are shared out. 16 rows of 50257 x 768: 17.6 us for 21.7; of 4096 x 4096 14.2 for 12.6.)
-    const bool wide = !B && a.M >= 8 && a.N >= 32768;
-    if (a.M <= kStreamRows && !wide)
-      launch_stream<F, B, G>(a, stream);
+    // Wide layers have workgroups enough for matrix_kernel without sharing out the inputs (16 rows of 768 x 50257 in fp32
+    // 13.4 us, in bf16 10.8; stream_kernel 21 and 12.6. Of 4096 x 16384 in bf16 24 and 15).
+    if (a.M > kStreamRows)
+      launch_matrix<F, B, G>(a, workspace, stream);
+    else if (a.N >= 32768)
+      launch_matrix<F, B, G>(a, nullptr, stream);
     else
-      launch_matrix<F, B, G>(a, a.M <= kStreamRows ? nullptr : workspace, stream);
+      launch_stream<F, B, G>(a, stream);
   };
   auto with = [&](auto b) {
     if (a.M <= kVectorRows) return launch_vector<F, decltype(b)::value>(a, stream);

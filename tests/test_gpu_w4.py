@@ -245,7 +245,7 @@ def test_far_values(device, dtype):
 
 
 @pytest.mark.parametrize("fmt,group", FORMATS)
-@pytest.mark.parametrize("rows,n", [(1, 40), (2, 16400), (16, 40), (16, 16400), (1024, 40), (1024, 150)])
+@pytest.mark.parametrize("rows,n", [(1, 40), (2, 16400), (16, 40), (16, 16400), (16, 32800), (1024, 40), (1024, 150)])
 def test_exact_products(device, fmt, group, rows, n):
     """fp32 activations of 24 bits, one at a time in each of 1024 places: nothing of them is lost, wherever it stands.
 
