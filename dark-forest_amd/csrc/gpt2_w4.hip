@@ -46,15 +46,15 @@ __device__ __forceinline__ unsigned short nearest_bf16(double q) {
   return bf16_bits(f);
 }
 
-// x / s to the nearest whole number, ties to even, for a bf16 s > 0 and |x| up to some 16 s: x * (1 / s)
-// is at most one off after rounding, and the remainder x - c s is exact (c s has at most 13 bits, and
-// where c is not 0 it is within a factor of two of x).
+// x / s to the nearest whole number, ties to even, for a bf16 s > 0 and |x| up to some 16 s: x times the
+// hardware's 1 / s (one unit in the last place off) is at most one off after rounding, and the remainder
+// x - c s is exact (c s has at most 13 bits, and where c is not 0 it is within a factor of two of x).
 struct Divider {
   float f, s, inv, half;
   __device__ __forceinline__ explicit Divider(float scale) {
     f = scale < 0x1p-100f ? 0x1p64f : 1.f;  // (1 / s would be infinite)
     s = scale * f;
-    inv = 1.f / s;
+    inv = __builtin_amdgcn_rcpf(s);
     half = 0.5f * s;
   }
   __device__ __forceinline__ float nearest(float x) const {
@@ -166,18 +166,22 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
       }
     }
     unsigned c = 0;
+    if constexpr (F == kE2M1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      unsigned q;
-      if constexpr (F == kE2M1) {
+      for (int j = 0; j < 8; ++j) {
         const float y = fabsf(x[r][j]);
-        q = (y > 0.25f * s) + (y >= 0.75f * s) + (y > 1.25f * s) + (y >= 1.75f * s) + (y > 2.5f * s) + (y >= 3.5f * s) +
-            (y > 5.f * s);
-        q = some ? q | (__float_as_uint(x[r][j]) >> 31 << 3) : 0u;
-      } else {
-        q = (unsigned)fminf(fmaxf((some ? v[j] : 0.f) + zero, 0.f), 15.f);
+        const unsigned q = (y > 0.25f * s) + (y >= 0.75f * s) + (y > 1.25f * s) + (y >= 1.75f * s) + (y > 2.5f * s) +
+                           (y >= 3.5f * s) + (y > 5.f * s);
+        c |= (some ? q | (__float_as_uint(x[r][j]) >> 31 << 3) : 0u) << (4 * j);
       }
-      c |= q << (4 * j);
+    } else {  // (four codes are a float's 16 bits)
+      float low = 0.f, high = 0.f;
+#pragma unroll
+      for (int j = 3; j >= 0; --j) {
+        low = fmaf(low, 16.f, fminf(fmaxf((some ? v[j] : 0.f) + zero, 0.f), 15.f));
+        high = fmaf(high, 16.f, fminf(fmaxf((some ? v[j + 4] : 0.f) + zero, 0.f), 15.f));
+      }
+      c = (unsigned)low | (unsigned)high << 16;
     }
     if (n < a.N && d < a.row_dwords) a.codes[(size_t)n * a.row_dwords + d] = c;
     if ((lane & (lanes - 1)) == 0) {
@@ -203,31 +207,39 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(QuantArgs a) {
   const size_t base = (size_t)linear_block() * (kThreads * kValueSteps), row0 = base / per_row;
   const uint32_t at0 = (uint32_t)(base % per_row);
   const unsigned char *codes = reinterpret_cast<const unsigned char *>(a.codes);
+  size_t n[kValueSteps];
+  uint32_t k[kValueSteps];
+  unsigned c[kValueSteps];
+  float scale[kValueSteps], zero[kValueSteps];
+#pragma unroll
+  for (uint32_t i = 0; i < kValueSteps; ++i) {  // (all loads before the first use)
+    const uint32_t at = at0 + i * kThreads + threadIdx.x;
+    k[i] = at % per_row * V;
+    n[i] = row0 + at / per_row;
+    const size_t row = min(n[i], (size_t)a.N - 1), group = (size_t)(k[i] >> a.log_group) * a.N + row;
+    if constexpr (BF16)
+      c[i] = *reinterpret_cast<const unsigned *>(codes + row * a.row_dwords * 4 + k[i] / 2);
+    else
+      c[i] = *reinterpret_cast<const unsigned short *>(codes + row * a.row_dwords * 4 + k[i] / 2);
+    scale[i] = bf16_value(a.scales[group]);
+    zero[i] = F == kU4 ? (float)a.zeros[group] : 8.f;
+  }
 #pragma unroll
   for (uint32_t i = 0; i < kValueSteps; ++i) {
-    const uint32_t at = at0 + i * kThreads + threadIdx.x, k = at % per_row * V;
-    const size_t n = row0 + at / per_row;
-    if (n >= a.N) return;
-    unsigned c;
-    if constexpr (BF16)
-      c = *reinterpret_cast<const unsigned *>(codes + n * a.row_dwords * 4 + k / 2);
-    else
-      c = *reinterpret_cast<const unsigned short *>(codes + n * a.row_dwords * 4 + k / 2);
-    const size_t group = (size_t)(k >> a.log_group) * a.N + n;
-    const float s = bf16_value(a.scales[group]), zero = F == kU4 ? (float)a.zeros[group] : 8.f;
+    if (n[i] >= a.N) break;
     float v[V];
 #pragma unroll
-    for (uint32_t j = 0; j < V; ++j) v[j] = code_value<F>(c >> (4 * j) & 15u, zero) * s;
-    if (k + V <= a.K) {
+    for (uint32_t j = 0; j < V; ++j) v[j] = code_value<F>(c[i] >> (4 * j) & 15u, zero[i]) * scale[i];
+    if (k[i] + V <= a.K) {
       u32x4 o;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         o[j] = BF16 ? (unsigned)bf16_bits(v[2 * j % V]) | (unsigned)bf16_bits(v[(2 * j + 1) % V]) << 16 : __float_as_uint(v[j]);
-      __builtin_memcpy(static_cast<char *>(a.out) + (n * a.K + k) * (BF16 ? 2 : 4), &o, 16);
+      __builtin_memcpy(static_cast<char *>(a.out) + (n[i] * a.K + k[i]) * (BF16 ? 2 : 4), &o, 16);
     } else {
 #pragma unroll
       for (uint32_t j = 0; j < V; ++j)
-        if (k + j < a.K) store_value<BF16>(a.out, n * a.K + k + j, v[j]);
+        if (k[i] + j < a.K) store_value<BF16>(a.out, n[i] * a.K + k[i] + j, v[j]);
     }
   }
 }

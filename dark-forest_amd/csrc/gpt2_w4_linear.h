@@ -809,7 +809,7 @@ void launch_linear_format(const LinearArgs &a, bool bf16, uint32_t group, float 
     constexpr bool B = decltype(b)::value;
     constexpr int G = decltype(g)::value;
     // Wide layers have workgroups enough for matrix_kernel without sharing out the inputs (16 rows of 768 x 50257 in fp32
-    // 13.4 us, in bf16 10.8; stream_kernel 21 and 12.6. Of 4096 x 16384 in bf16 24 and 15).
+    // 13.4 us, in bf16 10.8; stream_kernel 21 and 12.6. Of 4096 x 16384 in bf16 16.3, in four splits, and 15.2).
     if (a.M > kStreamRows)
       launch_matrix<F, B, G>(a, workspace, stream);
     else if (a.N >= 32768)
