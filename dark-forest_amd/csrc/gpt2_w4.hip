@@ -395,13 +395,14 @@ int dfgpt2_w4_linear(const void *x, const void *codes, const uint16_t *scales, c
   if (st == DFATTN_OK && bias != nullptr) st = need(fn, {bias}, 4);
   if (st == DFATTN_OK && residual != nullptr) st = need(fn, {residual}, item);
   if (st != DFATTN_OK) return st;
-  const Span to{out, (size_t)rows * out_features * item};
-  if (overlap(to, {x, ((size_t)(rows - 1) * row_stride + in_features) * item}) ||
-      overlap(to, {codes, (size_t)out_features * dwords_of(in_features) * 4}) ||
-      overlap(to, {scales, 2 * groups * out_features}) ||
-      (format == DFGPT2_W4_U4 && overlap(to, {zeros, groups * out_features})) || overlap(to, {bias, 4 * (size_t)out_features}) ||
-      (residual != out && overlap(to, {residual, to.bytes})) || overlap(to, {need_bytes > 0 ? workspace : nullptr, need_bytes}))
-    return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": out must not overlap what is read, or be the residual itself");
+  const Span to{out, (size_t)rows * out_features * item}, sums_to{need_bytes > 0 ? workspace : nullptr, need_bytes};
+  const Span read[] = {{x, ((size_t)(rows - 1) * row_stride + in_features) * item}, {codes, (size_t)out_features * dwords_of(in_features) * 4},
+                       {scales, 2 * groups * out_features}, {format == DFGPT2_W4_U4 ? zeros : nullptr, groups * out_features},
+                       {bias, 4 * (size_t)out_features}, {residual, to.bytes}};
+  bool clash = overlap(to, sums_to);
+  for (const Span &r : read) clash |= overlap(sums_to, r) || (overlap(to, r) && !(r.p == residual && residual == out));
+  if (clash)
+    return record_error(DFATTN_ERR_SHAPE, std::string(fn) + ": out must not overlap what is read, or be the residual itself; the workspace neither");
   LinearArgs a{x, static_cast<const unsigned char *>(codes), scales,
                static_cast<const unsigned char *>(zeros), bias, residual, out, nullptr, row_stride,
                rows, out_features, in_features, 4 * dwords_of(in_features), (uint32_t)groups, log2_of(group), 1, 1, (int)gelu};

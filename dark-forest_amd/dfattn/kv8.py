@@ -275,7 +275,7 @@ class PagePools:
 
 def page_pools(pools):
     """PagePools of a list of tensors [n_pages, ...] (any type, contiguous) and of KV8Caches, to be kept by a program that
-    copies in the same ones each step."""
+    copies in the same ones each step (the tensors must keep the memory they have now: no resize_, no new .data)."""
     if KV8Cache in map(type, pools):
         tensors = [t for p in pools for t in (p if type(p) is KV8Cache else (p,))]
     else:

@@ -5,7 +5,8 @@ tensors:
     y = w4.linear(x, w, bias=b, gelu=True)              # x [rows, inputs], one token or many
     x = w4.linear(y, w2, bias=b2, residual=x, out=x)
 
-Weights made elsewhere are a Weight of their codes and scales. Tensors live on the current device; what a call
+Weights made elsewhere are a Weight of their codes and scales. The products have no gradient: where one would be wanted of x
+or the residual the call is refused (torch.no_grad() around it, or ops.linear). Tensors live on the current device; what a call
 allocates belongs to the stream it runs on.
 """
 from __future__ import annotations
@@ -89,6 +90,8 @@ def linear(x, w, bias=None, residual=None, gelu=False, out=None, workspace="auto
     dev = names[6]
     *ptrs, fmt, group, n, k = _weight(w, names)
     px, stride, dtype = _rows(x, "x", k, names)
+    if names[0].is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+        raise ValueError("linear has no gradient: call it under torch.no_grad(), or ops.linear")
     shape = (x.shape[0], n)
     if bias is not None and bias.shape != (n,):
         raise ValueError(f"bias must be [{n}]")

@@ -136,7 +136,8 @@ def linear(ptrs=None, dtype=0, fmt=1, group=64, rows=3, k=100, n=10, stride=None
     (dict(rows=1 << 20, n=1 << 24), OVER), (dict(rows=40, k=4096, n=256, ws=at(7), ws_bytes=64), WORK),
     (dict(rows=40, k=4096, n=256, ws=at(7, 2), ws_bytes=1 << 30), MIS), (dict(rows=40, k=4096, n=256, ws=at(6, 4), ws_bytes=1 << 30), SHAPE),
     (dict(ptrs={6: at(0, 1196)}), SHAPE), (dict(ptrs={6: at(1, 620)}), SHAPE), (dict(ptrs={6: at(4, 36)}), SHAPE),
-    (dict(ptrs={6: at(5, 4)}), SHAPE), (dict(ptrs={6: at(3, 16)}), SHAPE)])
+    (dict(ptrs={6: at(5, 4)}), SHAPE), (dict(ptrs={6: at(3, 16)}), SHAPE),
+    *[(dict(rows=40, k=4096, n=256, ws=at(i, 4), ws_bytes=1 << 30), SHAPE) for i in range(6)]])   # sums over what is read
 def test_linear(kw, status):
     expect(status, "dfgpt2_w4_linear", linear(**kw))
 
@@ -229,6 +230,15 @@ def a_weight(**kw):
 def test_linear_wrapper(here, w, x, kw):
     with pytest.raises(ValueError):
         w4.linear(meta(3, 100, dtype=torch.float32) if x is None else x, w, **kw)
+
+
+@pytest.mark.parametrize("wants", ["x", "residual"])
+def test_linear_has_no_gradient(here, wants):
+    x, r = (torch.empty(3, n, device="meta", requires_grad=wants == name) for name, n in (("x", 100), ("residual", 10)))
+    with pytest.raises(ValueError, match="gradient"):
+        w4.linear(x, a_weight(), residual=r)
+    with torch.no_grad(), pytest.raises(AssertionError, match="was called"):
+        w4.linear(x, a_weight(), residual=r)
 
 
 @pytest.mark.parametrize("w,group,fmt", [(meta(3, 4, dtype=torch.float32), 64, "i8"), (meta(3, 4, dtype=torch.float32), 48, "i4"),
