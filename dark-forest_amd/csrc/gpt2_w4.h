@@ -70,6 +70,18 @@ struct LinearArgs {
 // kMatrixRows x kMatrixOutputs results.
 constexpr uint32_t kVectorRows = 2, kStreamRows = 16, kMatrixRows = 32, kMatrixOutputs = 128;
 
+// 2 to 16 rows that matrix_kernel takes too (us, the kernel of few rows and matrix_kernel): layers wide enough for its workgroups
+// (16 rows of 768 x 50257 in fp32 21 and 13, in bf16 12.6 and 10.8; 2 rows 16 and 12, 14.7 and 10.6); and with the inputs
+// shared out large ones (fp32: 4 rows of 4096 x 16384 19 to 22 and 18, 16 rows 25 and 19, but of 4096 x 4096 10 and 11; bf16: 16 rows of
+// 8192 x 28672 48 and 40, of 4096 x 16384 15 and 16) and in fp32 many inputs of more than 8 rows, which every workgroup of
+// stream_kernel reads (16 rows of 8192 x 1024 20 and 15, 8 rows 15 and 15).
+inline bool few_in_matrix(uint32_t M, uint32_t N, uint32_t K, bool bf16) {
+  const uint64_t weights = (uint64_t)N * K;
+  if (M < 2 || N >= 32768) return M >= 2;
+  if (bf16) return M > kVectorRows && weights >= 1u << 27;
+  return weights >= 1u << 25 || (M > 8 && K >= 8192);
+}
+
 // Splits of the inputs for matrix_kernel: up to 8, for no more than some 512 workgroups, or two where there are
 // up to 512 and many inputs (4096 x 4096 in bf16: 500 rows 42 us whole, 40 in two, 48 in four; 64 rows 23 us whole, 15 in four
 // and in eight).

@@ -44,6 +44,7 @@ struct Eight<true> {
   u32x4 r;
   static constexpr int kTerms = 1;
   __device__ __forceinline__ void load(const char *p) { __builtin_memcpy(&r, p, 16); }
+  __device__ __forceinline__ float value(int j) const { return __uint_as_float(j & 1 ? r[j / 2] & 0xffff0000u : r[j / 2] << 16); }
   __device__ __forceinline__ void load_some(const char *p, int n) {  // the first n
     unsigned x[8];
 #pragma unroll
@@ -64,6 +65,7 @@ struct Eight<false> {
   float r[8];
   static constexpr int kTerms = 3;
   __device__ __forceinline__ void load(const char *p) { __builtin_memcpy(r, p, 32); }
+  __device__ __forceinline__ float value(int j) const { return r[j]; }
   __device__ __forceinline__ void load_some(const char *p, int n) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) r[j] = j < n ? reinterpret_cast<const float *>(p)[j] : 0.f;
@@ -366,7 +368,10 @@ __global__ __launch_bounds__(512) void vector_kernel(LinearArgs a) {
 #pragma unroll
     for (int m = 0; m < ROWS; ++m) {
       const char *at = static_cast<const char *>(a.x) + ((size_t)m * a.stride + unit * 32) * kItem;
-      if (mine && unit * 32 + 32 <= a.K) {
+      if (!mine) {  // (apart from a row's end, whose single loads the wave would else take for these lanes)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[m][j] = 0.f;
+      } else if (unit * 32 + 32 <= a.K) {
         if constexpr (BF16) {
           unsigned r[16];
           __builtin_memcpy(r, at, 64);
@@ -377,7 +382,24 @@ __global__ __launch_bounds__(512) void vector_kernel(LinearArgs a) {
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) x[m][j] = mine && unit * 32 + j < a.K ? load_value<BF16>(at, j) : 0.f;
+        for (int e = 0; e < 4; ++e) {
+          const char *from = at + 8 * e * kItem;
+          const uint32_t k = unit * 32 + 8 * e;
+          if (k + 8 <= a.K) {
+            Eight<BF16> v;
+            v.load(from);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[m][8 * e + j] = v.value(j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[m][8 * e + j] = 0.f;
+            if (k < a.K) {
+#pragma unroll
+              for (int j = 0; j < 7; ++j)
+                if (k + j < a.K) x[m][8 * e + j] = load_value<BF16>(from, j);
+            }
+          }
+        }
       }
     }
     unsigned short scale[kLoads];
@@ -805,20 +827,18 @@ void launch_matrix(const LinearArgs &args, float *workspace, hipStream_t stream)
 // The products in one format (a source file each).
 template <Format F>
 void launch_linear_format(const LinearArgs &a, bool bf16, uint32_t group, float *workspace, hipStream_t stream) {
+  // (Without a workspace the inputs are not shared out.)
+  const bool matrix = few_in_matrix(a.M, a.N, a.K, bf16) && (workspace != nullptr || a.N >= 32768 || splits_of(a.M, a.N, a.K) == 1);
   auto with_group = [&](auto b, auto g) {
     constexpr bool B = decltype(b)::value;
     constexpr int G = decltype(g)::value;
-    // Wide layers have workgroups enough for matrix_kernel without sharing out the inputs (16 rows of 768 x 50257 in fp32
-    // 13.4 us, in bf16 10.8; stream_kernel 21 and 12.6. Of 4096 x 16384 in bf16 16.3, in four splits, and 15.2).
-    if (a.M > kStreamRows)
+    if (a.M > kStreamRows || matrix)
       launch_matrix<F, B, G>(a, workspace, stream);
-    else if (a.N >= 32768)
-      launch_matrix<F, B, G>(a, nullptr, stream);
     else
       launch_stream<F, B, G>(a, stream);
   };
   auto with = [&](auto b) {
-    if (a.M <= kVectorRows) return launch_vector<F, decltype(b)::value>(a, stream);
+    if (a.M <= kVectorRows && !matrix) return launch_vector<F, decltype(b)::value>(a, stream);
     if (group == 32)
       with_group(b, std::integral_constant<int, 32>{});
     else if (group == 64)

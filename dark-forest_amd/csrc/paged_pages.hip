@@ -66,6 +66,10 @@ __device__ __forceinline__ uint32_t scan_block(uint32_t x, uint32_t *lds, uint32
   return before + s - x;
 }
 
+// Tables and page lists in four launches (five with moves), one dependent step each: 3 to 5 us of latency a launch
+// for up to some 10^5 pages. Every sum is over fixed blocks in fixed order, and the atomics are integer ones,
+// so results do not depend on the order of the work.
+
 // 1: no references yet.
 template <Mode M>
 __global__ __launch_bounds__(kThreads) void clear_kernel(PagesArgs a) {
@@ -83,7 +87,8 @@ __global__ __launch_bounds__(kThreads) void clear_kernel(PagesArgs a) {
   }
 }
 
-// 2: the references, and the new rows. A wave takes one of `parts` parts of a row.
+// 2: the references, and the new rows. A wave takes one of `parts` parts of a row. Bound by the rate of atomics on
+// scattered words (2000 rows of 140 pages each 14.4 us, 20 a ns; counting in LDS would need all pages in one workgroup).
 template <Mode M>
 __global__ __launch_bounds__(kThreads) void count_kernel(PagesArgs a) {
   const uint32_t item = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -229,9 +234,12 @@ __global__ __launch_bounds__(kThreads) void rename_kernel(PagesArgs a) {
 
 // ---------------------------------------------------------------- small batches: one workgroup, one launch
 constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / 64;
-constexpr uint32_t kSmallPages = 8192, kSmallRows = 2048, kSmallEntries = 32768, kStrips = kSmallPages / kSmallThreads;
+constexpr uint32_t kSmallPages = 8192, kSmallRows = 128, kStrips = kSmallPages / kSmallThreads;  // (kSmallRows: of up to 64 pages)
 
-// The five steps above with everything in LDS between barriers.
+// The five steps above with everything in LDS between barriers: bound by the latency of one workgroup's steps, where the launches
+// above have theirs five times. Replayed from a graph, fork / free / compact, here and above: 8 rows of up to 64 pages of 1500
+// 4.4, 3.5, 4.4 us and 10.7, 8.8, 12.1; 128 rows of 8192 pages 8.5, 7.7, 11.9 and 11.0, 9.1, 13.3; 256 rows 15, 13, 24 and
+// 11.5, 9.1, 13.
 template <Mode M>
 __global__ __launch_bounds__(kSmallThreads) void small_kernel(PagesArgs a) {
   // first, last: fork: the lowest row that writes in a page and how many do; compact: the pages that move, and where to.
@@ -259,15 +267,19 @@ __global__ __launch_bounds__(kSmallThreads) void small_kernel(PagesArgs a) {
     if (M == kFree && a.ended != nullptr && a.ended[i] != 0) a.new_lens[i] = 0;
   }
   __syncthreads();
-  // A wave takes 64 entries of a row at a time.
-  const uint32_t parts = (a.W + 63) / 64;
-  for (uint32_t item = wave; item < a.N * parts; item += kSmallWaves) {
-    const uint32_t i = item / parts, j = item % parts * 64 + lane;
-    if (j >= pages[i]) continue;
-    const uint32_t p = a.table[(size_t)(M == kFork ? from[i] : i) * a.W + j];
+  // Every entry of every row: 1 to 16 waves side by side on a row, 64 entries each at a time.
+  uint32_t side = 1;
+  while (side < kSmallWaves && side * 64 < a.W) side *= 2;
+  auto entries = [&](auto row, auto use) {
+    for (uint32_t i = wave / side; i < a.N; i += kSmallWaves / side) {
+      const uint32_t *at = a.table + (size_t)row(i) * a.W;
+      for (uint32_t j = wave % side * 64 + lane; j < pages[i]; j += side * 64) use(i, j, at[j]);
+    }
+  };
+  entries([&](uint32_t i) { return M == kFork ? from[i] : i; }, [&](uint32_t i, uint32_t j, uint32_t p) {
     if constexpr (M == kFork) a.new_table[(size_t)i * a.W + j] = p;
     if (p < a.n_pages) atomicAdd(refs + p, 1u);
-  }
+  });
   if constexpr (M == kFork)
     for (uint32_t i = tid; i < a.N; i += kSmallThreads)
       if (opened[i] != kNone) {
@@ -348,12 +360,9 @@ __global__ __launch_bounds__(kSmallThreads) void small_kernel(PagesArgs a) {
       a.counts[0] = moves;
     }
     __syncthreads();
-    for (uint32_t item = wave; item < a.N * parts; item += kSmallWaves) {
-      const uint32_t i = item / parts, j = item % parts * 64 + lane;
-      if (j >= pages[i]) continue;
-      const uint32_t p = a.table[(size_t)i * a.W + j];
+    entries([](uint32_t i) { return i; }, [&](uint32_t i, uint32_t j, uint32_t p) {
       a.new_table[(size_t)i * a.W + j] = p >= used && p < a.n_pages ? first[p] : p;
-    }
+    });
     return;
   }
   const uint32_t pairs = M == kFork ? min(need, n_free) : 0;
@@ -497,8 +506,7 @@ int run_pages(const char *fn, PagesArgs &a, void *workspace, size_t workspace_by
   if (workspace == nullptr || workspace_bytes < workspace_bytes_for(a.N, a.n_pages))
     return record_error(DFATTN_ERR_WORKSPACE, std::string(fn) + ": the workspace is too small");
   if (!aligned_to(workspace, 4)) return record_error(DFATTN_ERR_MISALIGNED, std::string(fn) + ": misaligned pointer");
-  // One workgroup as long as it is about as fast as the others' five launches.
-  if (a.n_pages <= kSmallPages && a.N <= kSmallRows && (uint64_t)a.N * a.W <= kSmallEntries) {
+  if (a.n_pages <= kSmallPages && (uint64_t)a.N * ((a.W + 63) / 64) <= kSmallRows) {
     hipLaunchKernelGGL(small_kernel<M>, dim3(1), dim3(kSmallThreads), 0, stream, a);
     return launched(fn);
   }

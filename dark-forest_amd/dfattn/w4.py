@@ -100,7 +100,7 @@ def linear(x, w, bias=None, residual=None, gelu=False, out=None, workspace="auto
     with _on(stream, dev):
         out, po = _out(out, "out", shape, x.dtype, x.device, names)
         if isinstance(workspace, str):
-            need = linear_workspace_bytes(shape[0], k, n) if shape[0] > 16 else 0
+            need = linear_workspace_bytes(shape[0], k, n) if shape[0] > 1 else 0
             workspace = names[0].empty((need // 4,), dtype=names[2], device=x.device) if need else None
     ws, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace, "workspace", names[2], dev), workspace.numel() * 4)
     _check(ops_lib().dfgpt2_w4_linear(

@@ -171,6 +171,24 @@ def test_linear_many_inputs(device, fmt, group, dtype, rows, n, k):
 
 @pytest.mark.parametrize("fmt,group", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n,k", [(2, 33000, 300), (2, 8200, 4100), (5, 8210, 4100), (9, 40, 8200), (16, 70, 8300)])
+def test_linear_few_rows(device, fmt, group, dtype, rows, n, k):
+    """Wide layers, large ones and many inputs, where few rows share out the inputs; and without a workspace."""
+    x = torch.randn(rows, k, generator=generator(k + n), device="cuda").to(dtype)
+    w = weight(5, n, k, group, fmt)
+    check(x, w)
+    check(x, w, workspace=None)
+
+
+@pytest.mark.parametrize("fmt,group", [("i4", 128), ("u4", 64), ("e2m1", 32)])
+@pytest.mark.parametrize("rows", [2, 3])
+def test_linear_few_rows_bf16(device, fmt, group, rows):
+    n, k = 16400, 8200
+    check(torch.randn(rows, k, generator=generator(k + n), device="cuda").bfloat16(), weight(6, n, k, group, fmt))
+
+
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,n,k", [(1, 16389, 300), (2, 16389, 300), (1, 16399, 1000), (2, 16399, 1000), (1, 16390, 1100), (2, 9000, 2200),
                                       (3, 16401, 300), (16, 16401, 300), (5, 8300, 900), (9, 33000, 300), (34, 16401, 300)])
 def test_linear_many_outputs(device, fmt, group, dtype, rows, n, k):

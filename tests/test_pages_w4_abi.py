@@ -161,6 +161,9 @@ def here(monkeypatch):
         def dfattn_paged_workspace_bytes(self, *_):
             return 64
 
+        def dfgpt2_w4_linear_workspace_bytes(self, *_):
+            return 0
+
         def __getattr__(self, name):
             def called(*_):
                 raise AssertionError(f"{name} was called")
