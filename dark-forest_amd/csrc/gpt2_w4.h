@@ -66,20 +66,27 @@ struct LinearArgs {
   int gelu;
 };
 
-// Up to kVectorRows rows take vector_kernel, up to kStreamRows stream_kernel, more matrix_kernel, whose workgroups take
-// kMatrixRows x kMatrixOutputs results.
+// matrix_kernel's workgroups take kMatrixRows x kMatrixOutputs results, stream_kernel's kStreamRows rows.
 constexpr uint32_t kVectorRows = 2, kStreamRows = 16, kMatrixRows = 32, kMatrixOutputs = 128;
 
-// 2 to 16 rows that matrix_kernel takes too (us, the kernel of few rows and matrix_kernel): layers wide enough for its workgroups
-// (16 rows of 768 x 50257 in fp32 21 and 13, in bf16 12.6 and 10.8; 2 rows 16 and 12, 14.7 and 10.6); and with the inputs
-// shared out large ones (fp32: 4 rows of 4096 x 16384 19 to 22 and 18, 16 rows 25 and 19, but of 4096 x 4096 10 and 11; bf16: 16 rows of
-// 8192 x 28672 48 and 40, of 4096 x 16384 15 and 16) and in fp32 many inputs of more than 8 rows, which every workgroup of
-// stream_kernel reads (16 rows of 8192 x 1024 20 and 15, 8 rows 15 and 15).
-inline bool few_in_matrix(uint32_t M, uint32_t N, uint32_t K, bool bf16) {
+// Which kernel takes M rows of N outputs and K inputs. One or two rows: vector_kernel (two of 4096 x 4096 in bf16 6.0 us,
+// stream_kernel 7). More: stream_kernel, which reads all codes for every 16 rows but is one launch, up to a number of
+// weights' uses, then matrix_kernel, with the inputs shared out. (us, stream_kernel and matrix_kernel:)
+//   fp32: 64 rows of 768 x 2304 8.6 and 10.5, 128 13.1 and 12.4; 32 of 2048 x 2048 8.3 and 9.5, 48 12.5 and 9.7;
+//   bf16: 192 rows of 768 x 2304 9.7 and 12.6; 64 of 2048 x 2048 8.3 and 8.7, 96 10.7 and 9.9;
+//   1000 rows of 64 x 64 4.4 and 6.8, of 768 x 128 7.6 and 9.6.
+// matrix_kernel also takes 2 to 16 rows of layers wide enough for its workgroups (16 rows of 768 x 50257 in fp32 21 and 13, in bf16
+// 12.6 and 10.8; 2 rows, vector_kernel's 16 and 12, 14.7 and 10.6), of large ones (fp32: 4 rows of 4096 x 16384 19 to 22 and 18, 16
+// rows 25 and 19, but of 4096 x 4096 10 and 11; bf16: 16 rows of 8192 x 28672 48 and 40, of 4096 x 16384 15 and 16) and in
+// fp32 of many inputs for more than 8 rows (16 rows of 8192 x 1024 20 and 15, 8 rows 15 and 15).
+enum Path { kVector, kStream, kMatrix };
+inline Path path_of(uint32_t M, uint32_t N, uint32_t K, bool bf16) {
   const uint64_t weights = (uint64_t)N * K;
-  if (M < 2 || N >= 32768) return M >= 2;
-  if (bf16) return M > kVectorRows && weights >= 1u << 27;
-  return weights >= 1u << 25 || (M > 8 && K >= 8192);
+  if (M == 1) return kVector;
+  if (N >= 32768) return kMatrix;
+  if (M > kStreamRows) return M <= 1024 && (M + 15) / 16 * weights <= (bf16 ? 22u << 20 : 10u << 20) ? kStream : kMatrix;
+  if (bf16 ? M > kVectorRows && weights >= 1u << 27 : weights >= 1u << 25 || (M > 8 && K >= 8192)) return kMatrix;
+  return M <= kVectorRows ? kVector : kStream;
 }
 
 // Splits of the inputs for matrix_kernel: up to 8, for no more than some 512 workgroups, or two where there are

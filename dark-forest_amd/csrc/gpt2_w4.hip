@@ -367,10 +367,10 @@ int dfgpt2_w4_dequantize(const void *codes, const uint16_t *scales, const void *
 }
 
 size_t dfgpt2_w4_linear_workspace_bytes(uint32_t rows, uint32_t in_features, uint32_t out_features) {
-  if (rows > (1u << 20) || in_features == 0 || in_features > kMaxFeatures || out_features == 0 || out_features > kMaxFeatures)
+  if (rows == 0 || rows > (1u << 20) || in_features == 0 || in_features > kMaxFeatures || out_features == 0 ||
+      out_features > kMaxFeatures)
     return 0;
-  // (what either type needs)
-  if (rows <= kStreamRows && !few_in_matrix(rows, out_features, in_features, false)) return 0;
+  if (path_of(rows, out_features, in_features, false) != kMatrix) return 0;  // (then nor is it with bf16)
   const uint32_t splits = splits_of(rows, out_features, in_features);
   return splits == 1 ? 0 : 4 * (size_t)splits * rows * out_features;
 }

@@ -791,15 +791,16 @@ void launch_stream(const LinearArgs &args, hipStream_t stream) {
   const uint32_t n_tiles = (a.N + 15) / 16, tiles = (a.K + 127) / 128;
   uint32_t T = n_tiles >= 1024 ? kMost : n_tiles >= 512 && BF16 ? 2 : 1;
   // (of at least three tiles each where there are waves enough)
+  const uint32_t row_blocks = (a.M + kStreamRows - 1) / kStreamRows, blocks = n_tiles / T * row_blocks;
   while (a.k_waves < 8 && a.k_waves * 2 <= tiles &&
-         (n_tiles / T * a.k_waves < 512 || (n_tiles / T * a.k_waves < 2048 && a.k_waves * 6 <= tiles)))
+         (blocks * a.k_waves < 512 || (blocks * a.k_waves < 2048 && a.k_waves * 6 <= tiles)))
     a.k_waves *= 2;
   uint32_t n_waves = 1;
   while (a.k_waves * n_waves < 4 && n_tiles / T / (2 * n_waves) >= 256) n_waves *= 2;
   const uint32_t outputs = 16 * T * n_waves, waves = a.k_waves * n_waves;
   auto go = [&](auto t) {
-    hipLaunchKernelGGL((stream_kernel<F, BF16, GROUP, decltype(t)::value>), dim3((a.N + outputs - 1) / outputs), dim3(64 * waves),
-                       a.k_waves == 1 ? 0 : waves * T * 1024, stream, a);
+    hipLaunchKernelGGL((stream_kernel<F, BF16, GROUP, decltype(t)::value>), dim3((a.N + outputs - 1) / outputs, row_blocks),
+                       dim3(64 * waves), a.k_waves == 1 ? 0 : waves * T * 1024, stream, a);
   };
   if (T == 1)
     go(std::integral_constant<int, 1>{});
@@ -827,18 +828,20 @@ void launch_matrix(const LinearArgs &args, float *workspace, hipStream_t stream)
 // The products in one format (a source file each).
 template <Format F>
 void launch_linear_format(const LinearArgs &a, bool bf16, uint32_t group, float *workspace, hipStream_t stream) {
+  Path path = path_of(a.M, a.N, a.K, bf16);
   // (Without a workspace the inputs are not shared out.)
-  const bool matrix = few_in_matrix(a.M, a.N, a.K, bf16) && (workspace != nullptr || a.N >= 32768 || splits_of(a.M, a.N, a.K) == 1);
+  if (path == kMatrix && a.M <= kStreamRows && workspace == nullptr && a.N < 32768 && splits_of(a.M, a.N, a.K) > 1)
+    path = a.M <= kVectorRows ? kVector : kStream;
   auto with_group = [&](auto b, auto g) {
     constexpr bool B = decltype(b)::value;
     constexpr int G = decltype(g)::value;
-    if (a.M > kStreamRows || matrix)
+    if (path == kMatrix)
       launch_matrix<F, B, G>(a, workspace, stream);
     else
       launch_stream<F, B, G>(a, stream);
   };
   auto with = [&](auto b) {
-    if (a.M <= kVectorRows && !matrix) return launch_vector<F, decltype(b)::value>(a, stream);
+    if (path == kVector) return launch_vector<F, decltype(b)::value>(a, stream);
     if (group == 32)
       with_group(b, std::integral_constant<int, 32>{});
     else if (group == 64)

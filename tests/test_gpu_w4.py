@@ -141,7 +141,7 @@ def test_quantize_far(device):
 
 @pytest.mark.parametrize("fmt,group", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows", [1, 2, 7, 16, 17, 33, 64, 65, 130])
+@pytest.mark.parametrize("rows", [1, 2, 7, 16, 17, 33, 64, 65, 130, 1025, 1060])
 def test_linear(device, fmt, group, dtype, rows):
     n, k = 72, 392
     x = torch.randn(rows, k, generator=generator(rows), device="cuda").to(dtype)
@@ -151,7 +151,8 @@ def test_linear(device, fmt, group, dtype, rows):
 @pytest.mark.parametrize("fmt,group", [("i4", 32), ("u4", 128), ("e2m1", 64)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (3, 15, 7), (2, 16, 31), (5, 17, 33), (1, 2304, 768), (1, 100, 4097), (20, 31, 127), (40, 300, 1111),
-                                      (1, 6000, 40), (16, 5001, 768), (200, 130, 260), (1, 40, 20000), (9, 2000, 2000), (300, 260, 1000)])
+                                      (1, 6000, 40), (16, 5001, 768), (200, 130, 260), (1, 40, 20000), (9, 2000, 2000), (300, 260, 1000),
+                                      (1100, 31, 127), (1030, 300, 1111), (1024, 130, 260), (2000, 33, 300)])
 def test_linear_sizes(device, fmt, group, dtype, rows, n, k):
     x = torch.randn(rows, k, generator=generator(k), device="cuda").to(dtype)
     bias = torch.randn(n, generator=generator(n), device="cuda") if k % 2 else None
@@ -160,7 +161,8 @@ def test_linear_sizes(device, fmt, group, dtype, rows, n, k):
 
 @pytest.mark.parametrize("fmt,group", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,n,k", [(1, 70, 4500), (2, 70, 2100), (4, 70, 5000), (16, 40, 9000), (33, 140, 4321), (200, 1100, 2048)])
+@pytest.mark.parametrize("rows,n,k", [(1, 70, 4500), (2, 70, 2100), (4, 70, 5000), (16, 40, 9000), (33, 140, 4321), (200, 1100, 2048),
+                                      (1030, 140, 4321), (100, 1000, 2300), (20, 700, 9000)])
 def test_linear_many_inputs(device, fmt, group, dtype, rows, n, k):
     """Many tiles of inputs, whole and shared out, and without a workspace."""
     x = torch.randn(rows, k, generator=generator(k), device="cuda").to(dtype)
@@ -190,7 +192,7 @@ def test_linear_few_rows_bf16(device, fmt, group, rows):
 @pytest.mark.parametrize("fmt,group", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,n,k", [(1, 16389, 300), (2, 16389, 300), (1, 16399, 1000), (2, 16399, 1000), (1, 16390, 1100), (2, 9000, 2200),
-                                      (3, 16401, 300), (16, 16401, 300), (5, 8300, 900), (9, 33000, 300), (34, 16401, 300)])
+                                      (3, 16401, 300), (16, 16401, 300), (5, 8300, 900), (9, 33000, 300), (34, 16401, 300), (70, 4100, 300), (20, 8300, 60), (33, 33000, 60)])
 def test_linear_many_outputs(device, fmt, group, dtype, rows, n, k):
     """Layers wide enough for the forms that give a wave more outputs."""
     x = torch.randn(rows, k, generator=generator(k + rows), device="cuda").to(dtype)
@@ -198,7 +200,7 @@ def test_linear_many_outputs(device, fmt, group, dtype, rows, n, k):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,n,k", [(1, 768, 768), (4, 1000, 640), (50, 77, 300), (150, 200, 512)])
+@pytest.mark.parametrize("rows,n,k", [(1, 768, 768), (4, 1000, 640), (50, 77, 300), (150, 200, 512), (1100, 200, 512)])
 def test_epilogue(device, dtype, rows, n, k):
     g = generator(7)
     x = torch.randn(rows, k, generator=g, device="cuda").to(dtype)
@@ -213,7 +215,7 @@ def test_epilogue(device, dtype, rows, n, k):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,k", [(1, 200), (5, 200), (20, 201), (70, 768)])
+@pytest.mark.parametrize("rows,k", [(1, 200), (5, 200), (20, 201), (70, 768), (1040, 520)])
 def test_rows_of_a_wider_tensor(device, dtype, rows, k):
     wide = torch.randn(rows, 3 * k + 9, generator=generator(3), device="cuda").to(dtype)
     w = weight(4, 50, k, 32, "u4")
@@ -223,10 +225,11 @@ def test_rows_of_a_wider_tensor(device, dtype, rows, k):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_rows_alone(device, dtype):
+@pytest.mark.parametrize("rows", [19, 1029])
+def test_rows_alone(device, dtype, rows):
     """A row's result does not depend on what the other rows hold, not-numbers among them, nor on what
     stands behind the inputs' codes."""
-    rows, n, k = 19, 90, 300
+    n, k = 90, 300
     x = torch.randn(rows, k, generator=generator(3), device="cuda").to(dtype)
     for fmt in ("i4", "u4", "e2m1"):
         w = weight(5, n, k, 64, fmt)
@@ -263,7 +266,7 @@ def test_far_values(device, dtype):
 
 
 @pytest.mark.parametrize("fmt,group", FORMATS)
-@pytest.mark.parametrize("rows,n", [(1, 40), (2, 16400), (16, 40), (16, 16400), (16, 32800), (1024, 40), (1024, 150)])
+@pytest.mark.parametrize("rows,n", [(1, 40), (2, 16400), (16, 40), (16, 16400), (16, 32800), (1024, 40), (1024, 150), (1056, 40), (1056, 150)])
 def test_exact_products(device, fmt, group, rows, n):
     """fp32 activations of 24 bits, one at a time in each of 1024 places: nothing of them is lost, wherever it stands.
 

@@ -133,11 +133,11 @@ def linear(ptrs=None, dtype=0, fmt=1, group=64, rows=3, k=100, n=10, stride=None
     *[(dict(ptrs={i: None}), NULL) for i in (0, 1, 2, 3, 6)], (dict(ptrs={0: at(0, 2)}), MIS), (dict(ptrs={1: at(1, 4)}), MIS),
     (dict(ptrs={4: at(4, 2)}), MIS), (dict(ptrs={5: at(5, 2)}), MIS), (dict(ptrs={6: at(6, 2)}), MIS), (dict(stride=99), SHAPE),
     (dict(ptrs={6: at(6, 1)}, dtype=1), MIS), (dict(rows=(1 << 20) + 1), OVER), (dict(stride=(1 << 28) + 1), OVER), (dict(rows=0), 0),
-    (dict(rows=1 << 20, n=1 << 24), OVER), (dict(rows=40, k=4096, n=256, ws=at(7), ws_bytes=64), WORK),
-    (dict(rows=40, k=4096, n=256, ws=at(7, 2), ws_bytes=1 << 30), MIS), (dict(rows=40, k=4096, n=256, ws=at(6, 4), ws_bytes=1 << 30), SHAPE),
+    (dict(rows=1 << 20, n=1 << 24), OVER), (dict(rows=1030, k=250, n=64, ws=at(7), ws_bytes=64), WORK),
+    (dict(rows=1030, k=250, n=64, ws=at(7, 2), ws_bytes=1 << 30), MIS), (dict(rows=1030, k=250, n=64, ws=at(6, 4), ws_bytes=1 << 30), SHAPE),
     (dict(ptrs={6: at(0, 1196)}), SHAPE), (dict(ptrs={6: at(1, 620)}), SHAPE), (dict(ptrs={6: at(4, 36)}), SHAPE),
     (dict(ptrs={6: at(5, 4)}), SHAPE), (dict(ptrs={6: at(3, 16)}), SHAPE),
-    *[(dict(rows=40, k=4096, n=256, ws=at(i, 4), ws_bytes=1 << 30), SHAPE) for i in range(6)]])   # sums over what is read
+    *[(dict(rows=1030, k=250, n=64, ws=at(i, 4), ws_bytes=1 << 30), SHAPE) for i in range(6)]])   # sums over what is read
 def test_linear(kw, status):
     expect(status, "dfgpt2_w4_linear", linear(**kw))
 
