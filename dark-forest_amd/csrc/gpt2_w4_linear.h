@@ -494,19 +494,24 @@ __global__ __launch_bounds__(512) void vector_kernel(LinearArgs a) {
 // the zero points take off, sum over the groups of (sum x)(zero s), is a product itself: four groups at a time on the fp32
 // matrix instruction, with the groups' sums of x by products with ones, 16 rows each by two of the waves.
 // Where rows and outputs give too few workgroups, `splits` share out the inputs and leave fp32 sums, which join_kernel adds.
-template <Format F, bool BF16, int GROUP, int R>
-__global__ __launch_bounds__(kThreads, 2) void matrix_kernel(LinearArgs a) {  // (2: no sums in accumulation registers)
+// With HALVES = 2 eight waves do, four for each half of the inputs, and the halves' sums meet in LDS.
+template <Format F, bool BF16, int GROUP, int R, int HALVES>
+__global__ __launch_bounds__(kThreads * HALVES, 2) void matrix_kernel(LinearArgs a) {  // (2: no sums in accumulation registers)
   constexpr bool E2M1 = F == kE2M1;
   constexpr int T = kMatrixOutputs / 64;
   constexpr int kGroups = 128 / GROUP, kSteps = GROUP / 32;
   constexpr int kTerms = Eight<BF16>::kTerms, kItem = BF16 ? 2 : 4;
-  __shared__ f32x4 operands[2][kTerms][4][R][64];
-  __shared__ f32x4 x_sums[2][4][R * 4];  // of four groups
-  const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ f32x4 operands_of_half[HALVES][2][kTerms][4][R][64];
+  __shared__ f32x4 x_sums_of_half[HALVES][2][4][R * 4];  // of four groups
+  const uint32_t lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4, thread = threadIdx.x % kThreads;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(thread >> 6), half = HALVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+  auto &operands = operands_of_half[half];
+  auto &x_sums = x_sums_of_half[half];
   const uint32_t n0 = (xcd_block(blockIdx.x, gridDim.x) * 4 + wave) * (16 * T), m0 = blockIdx.y * (16 * R);
   const uint32_t tiles = (a.K + 127) / 128;
-  const uint32_t t0 = (uint32_t)((uint64_t)tiles * blockIdx.z / gridDim.z), t1 = (uint32_t)((uint64_t)tiles * (blockIdx.z + 1) / gridDim.z);
+  const uint32_t parts = gridDim.z * HALVES, my_part = blockIdx.z * HALVES + half;
+  const uint32_t t0 = (uint32_t)((uint64_t)tiles * my_part / parts), t1 = (uint32_t)((uint64_t)tiles * (my_part + 1) / parts);
+  const uint32_t steps = HALVES == 1 ? t1 - t0 : (tiles + parts - 1) / parts;  // (the same for both halves: they meet at barriers)
   const uint32_t g1 = min(t1 * kGroups, a.groups);
   const unsigned char *codes[T];
   uint32_t n[T];
@@ -535,7 +540,7 @@ __global__ __launch_bounds__(kThreads, 2) void matrix_kernel(LinearArgs a) {  //
     }
   };
   // Staging: a thread has 8 inputs of R rows.
-  const uint32_t octet = threadIdx.x & 15, row = threadIdx.x >> 4;
+  const uint32_t octet = thread & 15, row = thread >> 4;
   const uint32_t step = GROUP == 128 ? octet & 3 : octet >> 2, part = GROUP == 128 ? octet >> 2 : octet & 3;
   struct Inputs {
     Eight<BF16> x[R];
@@ -677,35 +682,64 @@ __global__ __launch_bounds__(kThreads, 2) void matrix_kernel(LinearArgs a) {  //
     load_codes(t0, d[0]);
     load_scales(t0 * kGroups, sc);
     stage(0, in);
-    __syncthreads();
-    for (uint32_t tile = t0; tile < t1; tile += 4) {
+  }
+  __syncthreads();
+  for (uint32_t first = 0; first < steps; first += 4) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (tile + i >= t1) break;
-        const bool more = tile + i + 1 < t1;
-        const uint32_t group = (tile + i) * kGroups;
+    for (int i = 0; i < 4; ++i) {
+      if (first + i >= steps) break;
+      const uint32_t tile = t0 + first + i;
+      if (HALVES == 1 || tile < t1) {
+        const bool more = tile + 1 < t1;
+        const uint32_t group = tile * kGroups;
         if (more) {
-          load_x(tile + i + 1, in);  // (loads come back in order: what is waited for first, first)
-          load_codes(tile + i + 1, d[(i + 1) % 2]);
+          load_x(tile + 1, in);  // (loads come back in order: what is waited for first, first)
+          load_codes(tile + 1, d[(i + 1) % 2]);
         }
         // (The sums of x of the four groups before were written before the last barrier.)
-        const int fours = kGroups == 1 ? (int)((tile - t0) / 4 % 2) : i * kGroups / 4 % 2;
+        const int fours = kGroups == 1 ? (int)(first / 4 % 2) : i * kGroups / 4 % 2;
         if (i * kGroups % 4 == 0) {
-          if (tile + i > t0) take_off(group - 4, fours ^ 1);
+          if (tile > t0) take_off(group - 4, fours ^ 1);
           next_four(group, sc, taken);
           load_scales(group + 4, sc);
         }
         use(i % 2, d[i % 2], i * kGroups % 4, fours);
         if (more) stage((i + 1) % 2, in);
-        __syncthreads();
       }
+      __syncthreads();
     }
+  }
+  if (t0 < t1) {
     const uint32_t last = (t1 - t0 - 1) * kGroups / 4;  // the last four groups
     take_off(t0 * kGroups + 4 * last, (int)(last % 2));
   }
+  // With two halves each ends every other 16 outputs.
+  constexpr int kEnds = HALVES == 2 ? 1 : T;
+  f32x4 end[kEnds][R];
+  if constexpr (HALVES == 2) {
+    static_assert(T == 2 && sizeof(operands) >= 4 * R * 64 * sizeof(f32x4), "a half's sums take its operands' place");
+    f32x4 *mine = &operands_of_half[half][0][0][0][0][0], *other = &operands_of_half[half ^ 1][0][0][0][0][0];
+    const bool second = half != 0;
+    auto pick = [&](const f32x4 &x, const f32x4 &y) {  // (number by number: the arrays stay in registers)
+      f32x4 z;
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const uint32_t at = n0 + 16 * t + col;
+      for (int e = 0; e < 4; ++e) z[e] = second ? y[e] : x[e];
+      return z;
+    };
+#pragma unroll
+    for (int r = 0; r < R; ++r) mine[(wave * R + r) * 64 + lane] = pick(sum[1][r], sum[0][r]);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) end[0][r] = pick(sum[0][r], sum[1][r]) + other[(wave * R + r) * 64 + lane];
+  } else {
+#pragma unroll
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int r = 0; r < R; ++r) end[t][r] = sum[t][r];
+  }
+#pragma unroll
+  for (int t = 0; t < kEnds; ++t) {
+    const uint32_t at = n0 + 16 * (HALVES == 2 ? half : t) + col;
     if (at >= a.N) continue;
     const float bias = a.bias != nullptr ? a.bias[at] : 0.f;
 #pragma unroll
@@ -716,10 +750,10 @@ __global__ __launch_bounds__(kThreads, 2) void matrix_kernel(LinearArgs a) {  //
         if (m >= a.M) continue;
         const size_t o = (size_t)m * a.N + at;
         if (a.partial != nullptr) {
-          a.partial[(size_t)blockIdx.z * a.M * a.N + o] = sum[t][r][e];
+          a.partial[(size_t)blockIdx.z * a.M * a.N + o] = end[t][r][e];
           continue;
         }
-        float y = sum[t][r][e] + bias;
+        float y = end[t][r][e] + bias;
         if (a.gelu) y = gelu_f(y);
         if (a.residual != nullptr) y += load_value<BF16>(a.residual, o);
         store_value<BF16>(a.out, o, y);
@@ -814,12 +848,22 @@ template <Format F, bool BF16, int GROUP>
 void launch_matrix(const LinearArgs &args, float *workspace, hipStream_t stream) {
   LinearArgs a = args;
   uint32_t splits = workspace == nullptr ? 1 : splits_of(a.M, a.N, a.K);
+  // bf16: two of the splits in one workgroup, which saves their sums' way through memory (500 rows of 4096 x 4096 36 us for 31),
+  // where two such workgroups fit on every CU or each has few steps: with one a CU eight waves wait for each other at every
+  // step (128 rows of 4096 x 4096, 8 steps, 18.7 us and 16.3; 256 rows, 16 steps and no join_kernel, 25.1 and 20.7, in
+  // groups of 32 26.6 and 26.4; 128 rows of 16384 x 4096, 32 steps, 44 and 49).
+  const size_t blocks = (size_t)((a.N + kMatrixOutputs - 1) / kMatrixOutputs) * ((a.M + kMatrixRows - 1) / kMatrixRows);
+  const bool halves = BF16 && a.M > 16 && splits > 1 && (blocks * splits >= 1024 || (a.K + 127) / 128 <= (GROUP > 32 && splits == 2 ? 16 : 8) * splits);
+  if (halves) splits /= 2;
   if (splits > 1) a.partial = workspace;
   const dim3 grid((a.N + kMatrixOutputs - 1) / kMatrixOutputs, (a.M + kMatrixRows - 1) / kMatrixRows, splits);
-  if (a.M <= 16)
-    hipLaunchKernelGGL((matrix_kernel<F, BF16, GROUP, 1>), grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((matrix_kernel<F, BF16, GROUP, kMatrixRows / 16>), grid, dim3(kThreads), 0, stream, a);
+  if (a.M <= 16) {
+    hipLaunchKernelGGL((matrix_kernel<F, BF16, GROUP, 1, 1>), grid, dim3(kThreads), 0, stream, a);
+  } else if (halves) {
+    if constexpr (BF16) hipLaunchKernelGGL((matrix_kernel<F, BF16, GROUP, kMatrixRows / 16, 2>), grid, dim3(2 * kThreads), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((matrix_kernel<F, BF16, GROUP, kMatrixRows / 16, 1>), grid, dim3(kThreads), 0, stream, a);
+  }
   if (splits == 1) return;
   const size_t groups = ((size_t)a.M * a.N + kThreads - 1) / kThreads;
   hipLaunchKernelGGL((join_kernel<BF16>), dim3((uint32_t)std::min<size_t>(2048, groups)), dim3(kThreads), 0, stream, a, splits);
