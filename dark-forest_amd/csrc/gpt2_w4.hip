@@ -77,6 +77,8 @@ struct Divider {
 // A workgroup takes 32 outputs and 256 inputs: a lane 8 inputs of four outputs, 4 to 16 neighbours a
 // group. Each of four neighbours divides for one of the four outputs. The scales go through LDS, so that neighbouring
 // outputs' are written together.
+// Bound: VALU and memory nearly alike (16384 x 4096 from bf16 60 us, 2.8 TB/s: extremes, one double division a group and four
+// neighbours, the product, its check and clamp for each value); 768 x 768 4.2 us, a launch's latency.
 constexpr int kQuantRows = 32, kQuantCols = 256;
 template <Format F, bool BF16>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
 
 // ---------------------------------------------------------------- values
 // A lane writes 16 bytes at a time, neighbours next to each other: 4 fp32 or 8 bf16 values of a row; kValueSteps
-// times 256 lanes a workgroup.
+// times 256 lanes a workgroup. Bound: the stores (16384 x 4096 to fp32 47 us, 6.4 TB/s; 768 x 768 4.2 us).
 constexpr uint32_t kValueSteps = 8;
 template <Format F, bool BF16>
 __global__ __launch_bounds__(kThreads) void dequantize_kernel(QuantArgs a) {

@@ -152,7 +152,8 @@ def test_linear(device, fmt, group, dtype, rows):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,n,k", [(1, 1, 1), (3, 15, 7), (2, 16, 31), (5, 17, 33), (1, 2304, 768), (1, 100, 4097), (20, 31, 127), (40, 300, 1111),
                                       (1, 6000, 40), (16, 5001, 768), (200, 130, 260), (1, 40, 20000), (9, 2000, 2000), (300, 260, 1000),
-                                      (1100, 31, 127), (1030, 300, 1111), (1024, 130, 260), (2000, 33, 300)])
+                                      (1100, 31, 127), (1030, 300, 1111), (1024, 130, 260), (2000, 33, 300), (1100, 600, 700),
+                                      (1100, 600, 300)])
 def test_linear_sizes(device, fmt, group, dtype, rows, n, k):
     x = torch.randn(rows, k, generator=generator(k), device="cuda").to(dtype)
     bias = torch.randn(n, generator=generator(n), device="cuda") if k % 2 else None
@@ -200,7 +201,7 @@ def test_linear_many_outputs(device, fmt, group, dtype, rows, n, k):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,n,k", [(1, 768, 768), (4, 1000, 640), (50, 77, 300), (150, 200, 512), (1100, 200, 512)])
+@pytest.mark.parametrize("rows,n,k", [(1, 768, 768), (4, 1000, 640), (50, 77, 300), (150, 200, 512), (1100, 200, 512), (1100, 600, 512)])
 def test_epilogue(device, dtype, rows, n, k):
     g = generator(7)
     x = torch.randn(rows, k, generator=g, device="cuda").to(dtype)
