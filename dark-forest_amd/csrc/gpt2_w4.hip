@@ -77,8 +77,9 @@ struct Divider {
 // A workgroup takes 32 outputs and 256 inputs: a lane 8 inputs of four outputs, 4 to 16 neighbours a
 // group. Each of four neighbours divides for one of the four outputs. The scales go through LDS, so that neighbouring
 // outputs' are written together.
-// Bound: VALU and memory nearly alike (16384 x 4096 from bf16 60 us, 2.8 TB/s: extremes, one double division a group and four
-// neighbours, the product, its check and clamp for each value); 768 x 768 4.2 us, a launch's latency.
+// Bound: from fp32 memory (16384 x 4096 to u4 55 us, 5.5 TB/s), from bf16 VALU too (49 us, 3.4 TB/s, to i4 41): extremes, one
+// double division a group and four neighbours, the product, its check and clamp for each value; 768 x 768 4 us, a launch's
+// latency. Workgroups of several blocks with the next one's loads ahead were slower (63 us, then 54 without).
 constexpr int kQuantRows = 32, kQuantCols = 256;
 template <Format F, bool BF16>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
@@ -110,8 +111,8 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
       for (int j = 0; j < 8; ++j)
         x[r][j] = n0 + 8 * r + (threadIdx.x >> 5) < a.N && d * 8 + j < a.K ? load_value<BF16>(w + r * rows8, j) : 0.f;
   }
-  // The groups' extremes: the largest magnitude by its bits (an infinity or NaN is above all numbers), and with zero
-  // points the lowest and highest, over 4, 8 or 16 neighbouring lanes.
+  // The groups' extremes over 4, 8 or 16 neighbouring lanes: with zero points the lowest and highest, where a NaN goes on, else
+  // the largest magnitude by its bits (an infinity or NaN is above all numbers).
   auto among = [&](auto v, auto better) {
     v = better(v, dpp<0xb1>(v));
     v = better(v, dpp<0x4e>(v));
@@ -119,6 +120,8 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
     if (lanes > 8) v = better(v, dpp<0x140>(v));
     return v;
   };
+  auto lower = [](float x, float y) { return __builtin_elementwise_minimum(x, y); };
+  auto higher = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };
   float lo[4], hi[4];
   unsigned most[4];
 #pragma unroll
@@ -128,16 +131,19 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       if (F == kU4) {
-        lo[r] = fminf(lo[r], x[r][j]);
-        hi[r] = fmaxf(hi[r], x[r][j]);
+        lo[r] = lower(lo[r], x[r][j]);
+        hi[r] = higher(hi[r], x[r][j]);
+      } else {
+        most[r] = max(most[r], __float_as_uint(x[r][j]) & 0x7fffffffu);
       }
-      most[r] = max(most[r], __float_as_uint(x[r][j]) & 0x7fffffffu);
     }
     if (F == kU4) {
-      lo[r] = among(lo[r], [](float a, float b) { return fminf(a, b); });
-      hi[r] = among(hi[r], [](float a, float b) { return fmaxf(a, b); });
+      lo[r] = among(lo[r], lower);
+      hi[r] = among(hi[r], higher);
+      most[r] = max(__float_as_uint(lo[r]) & 0x7fffffffu, __float_as_uint(hi[r]) & 0x7fffffffu);
+    } else {
+      most[r] = among(most[r], [](unsigned a, unsigned b) { return max(a, b); });
     }
-    most[r] = among(most[r], [](unsigned a, unsigned b) { return max(a, b); });
   }
   const uint32_t which = lane & 3;
   float low = lo[0], high = F == kU4 ? hi[0] : __uint_as_float(most[0]);
@@ -147,21 +153,23 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
     high = which == r ? F == kU4 ? hi[r] : __uint_as_float(most[r]) : high;
   }
   const double top = F == kU4 ? ((double)high - (double)low) / 15.0 : (double)high / (F == kI4 ? 7.0 : 6.0);
-  const unsigned near = nearest_bf16(top);
+  unsigned near = nearest_bf16(top);
+  if (F == kU4 && near != 0) near |= (unsigned)fminf(fmaxf(Divider(bf16_value((unsigned short)near)).nearest(-low), 0.f), 15.f) << 16;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const uint32_t row = 8 * r + (threadIdx.x >> 5), n = n0 + row;
-    const unsigned short bits = most[r] >= 0x7f800000u ? 0x7fc0u : (unsigned short)__shfl((int)near, (int)((threadIdx.x & 63 & ~3u) + r), 64);
+    const unsigned theirs = (unsigned)__shfl((int)near, (int)((threadIdx.x & 63 & ~3u) + r), 64);  // scale, and zero point above
+    const unsigned short bits = most[r] >= 0x7f800000u ? 0x7fc0u : (unsigned short)theirs;
     const float s = bf16_value(bits);
     const bool some = s > 0.f;  // (neither 0 nor NaN)
     const Divider by(some ? s : 1.f);
     float zero = F == kI4 ? 8.f : 0.f;
-    if (F == kU4 && some) zero = fminf(fmaxf(by.nearest(-lo[r]), 0.f), 15.f);
+    if (F == kU4 && some) zero = (float)(theirs >> 16);
     float v[8], far = 0.f;
     if constexpr (F != kE2M1) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = by.first(x[r][j], &far);
-      // (Few values are next to a border: 16384 x 4096 weights with the correction always 70 us, like this 67.)
+      // (Few values are next to a border: with the correction always 3 of 70 us more.)
       if (__any(some && !(far < by.near()))) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = by.nearest(x[r][j]);
