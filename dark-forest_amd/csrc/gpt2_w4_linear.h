@@ -528,15 +528,15 @@ __global__ __launch_bounds__(kThreads * HALVES, 2) void matrix_kernel(LinearArgs
 #pragma unroll
   for (int t = 0; t < T; ++t) {
     n[t] = min(n0 + 16 * t + col, a.N - 1);
-    codes[t] = a.codes + (size_t)n[t] * a.row_bytes + 16 * quarter;
+    codes[t] = a.codes + (size_t)n[t] * a.row_bytes;
   }
   struct Codes {
     u32x4 c[T];
   };
   auto load_codes = [&](uint32_t tile, Codes &d) {
-    const bool there = tile * 64 + 16 * quarter < a.row_bytes;
+    const uint32_t mine = tile * 64 + 16 * quarter, at = mine < a.row_bytes ? mine : 0;  // (x is 0 behind the inputs; a row may be 16 bytes)
 #pragma unroll
-    for (int t = 0; t < T; ++t) d.c[t] = *reinterpret_cast<const u32x4 *>(codes[t] + (there ? tile * 64 : 0));  // (x is 0 behind the inputs)
+    for (int t = 0; t < T; ++t) d.c[t] = *reinterpret_cast<const u32x4 *>(codes[t] + at);
   };
   struct Scales {
     unsigned scale[T], zero[F == kU4 ? T : 1];  // of group first + quarter

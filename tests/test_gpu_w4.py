@@ -253,6 +253,19 @@ def test_rows_alone(device, dtype, rows):
     assert torch.isnan(got[:, 20]).all() and torch.equal(got[:, 21:], want[:, 21:])
 
 
+@pytest.mark.parametrize("fmt,group", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n,k", [(1030, 96, 5), (1030, 32, 33), (1100, 160, 70), (2, 32800, 31), (40, 32768, 96), (3, 64, 20), (1, 32, 8)])
+def test_short_rows_of_codes(device, fmt, group, dtype, rows, n, k):
+    """Rows of 16, 32 and 48 bytes of codes, in the middle of a tensor whose other bytes are no part of them."""
+    x = torch.randn(rows, k, generator=generator(k), device="cuda").to(dtype)
+    w = weight(9, n, k, group, fmt)
+    want = check(x, w)
+    whole = torch.full((n * w4.row_bytes(k) + 128,), 0xff, dtype=torch.uint8, device="cuda")
+    codes = whole[64:-64].view(n, -1).copy_(w.codes)
+    assert torch.equal(w4.linear(x, w._replace(codes=codes)), want)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_far_values(device, dtype):
     """Large and small activations, and fp32 ones whose last bits matter."""
