@@ -281,3 +281,61 @@ def test_plan_goes_on(device):
             assert len(set(open_)) == len(open_) and not set(open_) & {p for row in rows for p in row}
             assert sum(held) >= len({p for row in rows for p in row})
     stream.synchronize()
+
+
+@pytest.mark.parametrize("requests,width,n_pages", [(20, 40, 900), (300, 9, 4000)])
+def test_compact_captured(device, requests, width, n_pages):
+    """Both forms of the tables' kernels, replayed on other lengths, in place and with the copies."""
+    page = 16
+    table, _ = batch(11, requests, width, page, n_pages)
+    table = [[p if 0 <= p < n_pages else j % n_pages for j, p in enumerate(row)] for row in table]
+    t, n = i32(table), torch.zeros(requests, dtype=torch.int32, device="cuda")
+    pools = pools_of(6, n_pages, (16, 64, torch.bfloat16))
+    first = pools[0].clone()
+    stream = torch.cuda.Stream()
+
+    def step():
+        c = dfattn.paged_compact(t, n, page, n_pages)
+        dfattn.paged_copy(pools, c.copy_src, c.copy_dst, c.counts)
+        return c
+
+    with torch.cuda.stream(stream):
+        step()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        c = step()
+    for seed in range(4):
+        rng = random.Random(seed)
+        lens = [rng.choice((0, rng.randint(0, width * page))) for _ in range(requests)]
+        t.copy_(i32(table))
+        n.copy_(i32(lens))
+        pools[0].copy_(first)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want = ref.compact(table, lens, page, n_pages)
+        same_lists(c, want, n_pages)
+        assert [row[:len(w)] for row, w in zip(t.tolist(), want["rows"])] == want["rows"]
+        moved = first.clone()
+        if want["copies"]:
+            src, dst = zip(*want["copies"])
+            moved[list(dst)] = first[list(src)]
+        assert torch.equal(pools[0], moved)
+
+
+def test_two_streams(device):
+    """Calls on two streams at once, of both forms, by the stream argument: each has its own lists."""
+    sides = []
+    for seed, (requests, width, n_pages) in enumerate([(20, 40, 900), (300, 9, 4000)]):
+        table, lens = batch(seed, requests, width, 16, n_pages)
+        parents = [random.Random(seed + i).randrange(requests) for i in range(requests)]
+        sides.append((torch.cuda.Stream(), table, lens, parents, i32(table), i32(lens), i32(parents), n_pages))
+    torch.cuda.synchronize()
+    got = [[dfattn.paged_fork(t, n, p, 16, pages, stream=s) for s, _, _, _, t, n, p, pages in sides] for _ in range(20)]
+    torch.cuda.synchronize()
+    for each in got:
+        for f, (_, table, lens, parents, _, _, _, pages) in zip(each, sides):
+            want = ref.fork(table, lens, parents, 16, pages)
+            assert f.seq_lens.tolist() == want["lens"]
+            same_lists(f, want, pages)

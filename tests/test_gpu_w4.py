@@ -347,3 +347,40 @@ def test_large_offsets(device):
     wide[:, :300] = rows
     w = weight(3, 40, 300, 32, "i4")
     assert torch.equal(w4.linear(wide[:, :300], w), w4.linear(rows, w))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_two_streams(device, dtype):
+    """Products that share out their inputs, on two streams at once: each call has its own sums."""
+    w = weight(1, 300, 2300, 64, "u4")
+    xs = [torch.randn(1100, 2300, generator=generator(seed), device="cuda").to(dtype) for seed in range(2)]
+    assert w4.linear_workspace_bytes(1100, 2300, 300) > 0
+    want = [w4.linear(x, w) for x in xs]
+    streams = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = [[w4.linear(x, w, stream=s) for x, s in zip(xs, streams)] for _ in range(10)]
+    torch.cuda.synchronize()
+    for each in got:
+        for y, z in zip(each, want):
+            assert torch.equal(y, z)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n,k", [(1, 700, 520), (1100, 300, 2300), (40, 700, 520), (2, 33000, 300)])
+def test_captured_forms(device, dtype, rows, n, k):
+    """Every product's kernels as a graph, replayed on other inputs between eager calls."""
+    w = weight(2, n, k, 128, "i4")
+    x, bias = torch.randn(rows, k, generator=generator(1), device="cuda").to(dtype), torch.randn(n, generator=generator(2), device="cuda")
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        w4.linear(x, w, bias, gelu=True)
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        y = w4.linear(x, w, bias, gelu=True)
+    for seed in range(4):
+        x.copy_(torch.randn(rows, k, generator=generator(30 + seed), device="cuda"))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, w4.linear(x, w, bias, gelu=True))
