@@ -14,7 +14,7 @@ from __future__ import annotations
 import collections
 
 from . import _check, _stream_ptr
-from .kv8 import _names, _on, _out, _ptr, _rows
+from .kv8 import _names, _on, _out, _ptr, _rows, _sizes, _u32
 from .ops import ops_lib
 
 FORMATS = {"i4": 0, "u4": 1, "e2m1": 2}  # DFGPT2_W4_I4, DFGPT2_W4_U4, DFGPT2_W4_E2M1
@@ -39,6 +39,7 @@ def _weight(w, n):
     if k < 1 or codes.dim() != 2 or codes.shape[1] != row_bytes(k):
         raise ValueError(f"codes must be [outputs, {row_bytes(k)}] for {k} inputs")
     shape = (-(-k // group), codes.shape[0])
+    _sizes("codes", shape[1], k)
     if scales.shape != shape or (fmt == "u4" and (zeros is None or zeros.shape != shape)):
         raise ValueError(f"scales (and the zeros of u4) must be {list(shape)}")
     return (_ptr(codes, "codes", torch.uint8, dev), _ptr(scales, "scales", n[3], dev),
@@ -54,6 +55,7 @@ def quantize(w, group=64, format="i4", stream=None):
     if w.dim() != 2 or not w.numel():
         raise ValueError("w must be [outputs, inputs] and not empty")
     n, k = w.shape
+    _sizes("w", n, k)
     p, stride, dtype = _rows(w, "w", k, names)
     with _on(stream, dev):
         codes = torch.empty((n, row_bytes(k)), dtype=torch.uint8, device=w.device)
@@ -79,6 +81,7 @@ def dequantize(w, dtype=None, out=None, stream=None):
 
 
 def linear_workspace_bytes(rows, in_features, out_features):
+    _u32(rows, "rows"), _u32(in_features, "in_features"), _u32(out_features, "out_features")
     return ops_lib().dfgpt2_w4_linear_workspace_bytes(rows, in_features, out_features)
 
 
@@ -93,6 +96,7 @@ def linear(x, w, bias=None, residual=None, gelu=False, out=None, workspace="auto
     if names[0].is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
         raise ValueError("linear has no gradient: call it under torch.no_grad(), or ops.linear")
     shape = (x.shape[0], n)
+    _sizes("x", shape[0])
     if bias is not None and bias.shape != (n,):
         raise ValueError(f"bias must be [{n}]")
     if residual is not None and residual.shape != shape:
@@ -100,7 +104,7 @@ def linear(x, w, bias=None, residual=None, gelu=False, out=None, workspace="auto
     with _on(stream, dev):
         out, po = _out(out, "out", shape, x.dtype, x.device, names)
         if isinstance(workspace, str):
-            need = linear_workspace_bytes(shape[0], k, n) if shape[0] > 1 else 0
+            need = ops_lib().dfgpt2_w4_linear_workspace_bytes(shape[0], k, n) if shape[0] > 1 else 0
             workspace = names[0].empty((need // 4,), dtype=names[2], device=x.device) if need else None
     ws, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace, "workspace", names[2], dev), workspace.numel() * 4)
     _check(ops_lib().dfgpt2_w4_linear(

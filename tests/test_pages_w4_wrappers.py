@@ -1,0 +1,83 @@
+"""The wrappers of the page calls and the 4-bit linear layers, on tensors without a device: what they refuse before the
+library is called."""
+import pytest
+import torch
+
+import dfattn
+from dfattn import kv8, w4
+
+BIG = 1 << 32
+
+
+@pytest.fixture
+def here(monkeypatch):
+    """Tensors without a device of their own count as being on the current one; nothing may reach the library but the
+    questions for a workspace's size."""
+    names = (torch, torch.int32, torch.float32, torch.bfloat16, torch.int8, torch.float8_e4m3fn, -1)
+    for module in (kv8, w4):
+        monkeypatch.setattr(module, "_names", lambda: names)
+        monkeypatch.setattr(module, "_stream_ptr", lambda s: None)
+
+    class Lib:
+        def dfattn_paged_workspace_bytes(self, *_):
+            return 64
+
+        def dfgpt2_w4_linear_workspace_bytes(self, *_):
+            return 0
+
+        def __getattr__(self, name):
+            def called(*_):
+                raise AssertionError(f"{name} was called")
+
+            return called
+
+    monkeypatch.setattr(kv8, "lib", Lib)
+    monkeypatch.setattr(w4, "ops_lib", Lib)
+
+
+def meta(*shape, dtype=torch.int32):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+def weight(n=10, k=100, group=64):
+    return w4.Weight(meta(n, w4.row_bytes(k), dtype=torch.uint8), meta(-(-k // group), n, dtype=torch.bfloat16), None, k, group, "i4")
+
+
+# ---------------------------------------------------------------- sizes: the entry points take 32 bits, ctypes takes the rest off
+@pytest.mark.parametrize("pools", [[meta(BIG + 4, 1, dtype=torch.int8)], [meta(BIG, 2, dtype=torch.bfloat16)] * 2])
+def test_pools_of_too_many_pages(here, pools):
+    with pytest.raises(ValueError):
+        dfattn.page_pools(pools)
+    with pytest.raises(ValueError):
+        dfattn.paged_copy(pools, meta(3), meta(3))
+
+
+def test_too_many_copies(here):
+    with pytest.raises(ValueError):
+        dfattn.paged_copy([meta(4, 2)], meta(BIG + 1), meta(BIG + 1))
+
+
+@pytest.mark.parametrize("r,width,n", [(BIG + 4, 1, 3), (4, BIG + 8, 3), (4, 8, BIG + 3)])
+def test_tables_too_large(here, r, width, n):
+    table, lens = meta(r, width), meta(r)
+    with pytest.raises(ValueError):
+        dfattn.paged_fork(table, lens, meta(n), 16, 100)
+    if n < BIG:
+        with pytest.raises(ValueError):
+            dfattn.paged_free(table, lens, 16, 100)
+        with pytest.raises(ValueError):
+            dfattn.paged_compact(table, lens, 16, 100)
+
+
+@pytest.mark.parametrize("rows,n,k", [(BIG + 5, 10, 1), (3, BIG + 10, 1), (3, 1, BIG + 100)])
+def test_layers_too_large(here, rows, n, k):
+    w = weight(n, k)
+    with pytest.raises(ValueError):
+        w4.linear(meta(rows, k, dtype=torch.bfloat16), w)
+    with pytest.raises(ValueError):
+        w4.linear_workspace_bytes(rows, k, n)
+    if rows < BIG:
+        with pytest.raises(ValueError):
+            w4.dequantize(w)
+        with pytest.raises(ValueError):
+            w4.quantize(meta(n, k, dtype=torch.bfloat16))
