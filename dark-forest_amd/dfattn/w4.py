@@ -5,9 +5,10 @@ tensors:
     y = w4.linear(x, w, bias=b, gelu=True)              # x [rows, inputs], one token or many
     x = w4.linear(y, w2, bias=b2, residual=x, out=x)
 
-Weights made elsewhere are a Weight of their codes and scales. The products have no gradient: where one would be wanted of x
-or the residual the call is refused (torch.no_grad() around it, or ops.linear). Tensors live on the current device; what a call
-allocates belongs to the stream it runs on.
+Weights made elsewhere are a Weight of their codes and scales. Nothing here has a gradient: where one would be wanted of an
+argument of linear or dequantize (x, the scales, the bias, the residual, out) the call is refused, as it is where one has a
+tangent of forward mode; a product that has one is torch's, with dequantize's values. Quantising rounds, and what it
+returns is apart from the weight's graph. Tensors live on the current device; what a call allocates belongs to the stream it runs on.
 """
 from __future__ import annotations
 
@@ -46,6 +47,18 @@ def _weight(w, n):
             _ptr(zeros, "zeros", torch.uint8, dev) if fmt == "u4" else None, FORMATS[fmt], group, shape[1], k)
 
 
+def _no_gradient(torch, name, *tensors):
+    """Refuses a call that a gradient of `tensors`, or a tangent of forward mode (which torch.no_grad() leaves on), would be
+    lost in."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
+    forward_ad = torch.autograd.forward_ad
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{name} has no gradient of forward mode: give it the primals")
+
+
 def quantize(w, group=64, format="i4", stream=None):
     """dfgpt2_w4_quantize: the Weight of w [outputs, inputs] (float32 or bfloat16, rows may be a column block)."""
     names = _names()
@@ -74,6 +87,7 @@ def dequantize(w, dtype=None, out=None, stream=None):
         dtype = names[2] if out is None else out.dtype
     if dtype is not names[2] and dtype is not names[3]:
         raise ValueError("values are read as float32 or bfloat16")
+    _no_gradient(names[0], "dequantize", w.scales, out)
     with _on(stream, names[6]):
         out, p = _out(out, "out", (n, k), dtype, w.codes.device, names)
     _check(ops_lib().dfgpt2_w4_dequantize(*ptrs, p, 0 if dtype is names[2] else 1, fmt, group, n, k, _stream_ptr(stream)))
@@ -93,8 +107,7 @@ def linear(x, w, bias=None, residual=None, gelu=False, out=None, workspace="auto
     dev = names[6]
     *ptrs, fmt, group, n, k = _weight(w, names)
     px, stride, dtype = _rows(x, "x", k, names)
-    if names[0].is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        raise ValueError("linear has no gradient: call it under torch.no_grad(), or ops.linear")
+    _no_gradient(names[0], "linear", x, w.scales, bias, residual, out)
     shape = (x.shape[0], n)
     _sizes("x", shape[0])
     if bias is not None and bias.shape != (n,):

@@ -81,3 +81,45 @@ def test_layers_too_large(here, rows, n, k):
             w4.dequantize(w)
         with pytest.raises(ValueError):
             w4.quantize(meta(n, k, dtype=torch.bfloat16))
+
+
+# ---------------------------------------------------------------- gradients: none is lost without a word
+def activations(n, wants):
+    t = torch.empty(3, n, device="meta")
+    return t.requires_grad_() if wants else t
+
+
+@pytest.mark.parametrize("wants", ["bias", "scales", "out"])
+def test_linear_refuses_gradients(here, wants):
+    bias = torch.empty(10, device="meta").requires_grad_(wants == "bias")
+    w = weight()
+    w.scales.requires_grad_(wants == "scales")
+    out = activations(10, wants == "out")
+    with pytest.raises(ValueError, match="gradient"):
+        w4.linear(activations(100, False), w, bias, out=out)
+    with torch.no_grad(), pytest.raises(AssertionError, match="was called"):
+        w4.linear(activations(100, False), w, bias, out=out)
+
+
+def test_dequantize_refuses_gradients(here):
+    w = weight()
+    w.scales.requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        w4.dequantize(w)
+    with torch.no_grad(), pytest.raises(AssertionError, match="was called"):
+        w4.dequantize(w)
+
+
+@pytest.mark.parametrize("wants", ["x", "residual", "bias"])
+@pytest.mark.parametrize("grad", [True, False])
+def test_linear_refuses_tangents(here, wants, grad):
+    """Forward mode goes on under torch.no_grad()."""
+    from torch.autograd import forward_ad
+
+    t = dict(x=activations(100, False), residual=activations(10, False), bias=torch.empty(10, device="meta"))
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        with pytest.raises(AssertionError, match="was called"):
+            w4.linear(t["x"], weight(), t["bias"], t["residual"])
+        t[wants] = forward_ad.make_dual(t[wants], torch.empty_like(t[wants]))
+        with pytest.raises(ValueError, match="gradient"):
+            w4.linear(t["x"], weight(), t["bias"], t["residual"])
