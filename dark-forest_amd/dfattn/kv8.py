@@ -209,10 +209,19 @@ def _table(block_table, seq_lens, names):
     return (_ptr(block_table, "block_table", i32, dev), _ptr(seq_lens, "seq_lens", i32, dev)) + tuple(block_table.shape)
 
 
+# A workspace of more words than this (some 7500 pages) is an allocation of its own, so that a program that keeps the free list does not
+# keep the scratch; up to there it stands behind the outputs, which saves a small call 1.3 of its 12 us on the host.
+_SCRATCH_WORDS = 16384
+
+
 def _parts(names, on, *sizes):
-    """int32 tensors of these sizes in one allocation, and the pointer of the workspace of the last size behind them."""
-    parts = names[0].empty_strided((sum(sizes),), (1,), dtype=names[1], device=on).split_with_sizes(sizes)
-    return parts[:-1], [t.data_ptr() for t in parts]
+    """int32 tensors of these sizes but the last, the workspace's; the pointers of all; what must live until the call is made."""
+    apart = sizes[-1] > _SCRATCH_WORDS
+    new = lambda n: names[0].empty_strided((n,), (1,), dtype=names[1], device=on)
+    scratch = new(sizes[-1]) if apart else None
+    parts = new(sum(sizes[:-1]) if apart else sum(sizes)).split_with_sizes(sizes[:-1] if apart else sizes)
+    ptrs = [t.data_ptr() for t in parts]
+    return (parts, ptrs + [scratch.data_ptr()], scratch) if apart else (parts[:-1], ptrs, None)
 
 
 def paged_fork(block_table, seq_lens, parents, page_size, n_pages, keep_lens=None, new_table=None, stream=None):
@@ -234,7 +243,7 @@ def paged_fork(block_table, seq_lens, parents, page_size, n_pages, keep_lens=Non
             new_table = names[0].empty_strided((n, width), (width, 1), dtype=i32, device=on)
         _same(new_table, "new_table", (n, width))
         pages = n_pages if ws else 0  # (0: the call refuses the sizes)
-        parts, ptrs = _parts(names, on, n, pages, pages, 1, n, n, 2, ws // 4)
+        parts, ptrs, scratch = _parts(names, on, n, pages, pages, 1, n, n, 2, ws // 4)
     _check(lib().dfattn_paged_fork(
         pt, pl, _ptr(parents, "parents", i32, dev), None if keep_lens is None else _ptr(keep_lens, "keep_lens", i32, dev),
         _ptr(new_table, "new_table", i32, dev), *ptrs[:7], r, n, width, page_size, n_pages, ptrs[7], ws, _stream_ptr(stream)))
@@ -252,7 +261,7 @@ def paged_free(block_table, seq_lens, page_size, n_pages, ended=None, stream=Non
     ws = lib().dfattn_paged_workspace_bytes(r, n_pages)
     with _on(stream, names[6]):
         pages = n_pages if ws else 0
-        parts, ptrs = _parts(names, block_table.device, pages, pages, 1, ws // 4)
+        parts, ptrs, scratch = _parts(names, block_table.device, pages, pages, 1, ws // 4)
     _check(lib().dfattn_paged_free(pt, pl, None if ended is None else _ptr(ended, "ended", names[1], names[6]), *ptrs[:3],
                                    r, width, page_size, n_pages, ptrs[3], ws, _stream_ptr(stream)))
     return tuple(parts)
@@ -269,7 +278,7 @@ def paged_compact(block_table, seq_lens, page_size, n_pages, new_table=None, str
     ws = lib().dfattn_paged_workspace_bytes(r, n_pages)
     with _on(stream, names[6]):
         pages = n_pages if ws else 0
-        parts, ptrs = _parts(names, block_table.device, pages, pages, 1, pages // 2, pages // 2, 1, ws // 4)
+        parts, ptrs, scratch = _parts(names, block_table.device, pages, pages, 1, pages // 2, pages // 2, 1, ws // 4)
     _check(lib().dfattn_paged_compact(pt, pl, _ptr(new_table, "new_table", names[1], names[6]), *ptrs[:6], r, width,
                                       page_size, n_pages, ptrs[6], ws, _stream_ptr(stream)))
     return PagedCompact(new_table, *parts)

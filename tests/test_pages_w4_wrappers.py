@@ -123,3 +123,19 @@ def test_linear_refuses_tangents(here, wants, grad):
         t[wants] = forward_ad.make_dual(t[wants], torch.empty_like(t[wants]))
         with pytest.raises(ValueError, match="gradient"):
             w4.linear(t["x"], weight(), t["bias"], t["residual"])
+
+
+# ---------------------------------------------------------------- memory
+@pytest.mark.parametrize("n_pages", [8193, 500000])
+def test_scratch_goes_with_the_call(here, monkeypatch, n_pages):
+    """What a program keeps of a call from step to step keeps none of its workspace (8 bytes a page)."""
+    class Lib:
+        dfattn_paged_workspace_bytes = lambda self, rows, pages: 4 * (2 * pages + 1025 + rows)
+        dfattn_paged_fork = dfattn_paged_free = dfattn_paged_compact = lambda self, *_: 0
+
+    monkeypatch.setattr(kv8, "lib", Lib)
+    table, lens = meta(4, 8), meta(4)
+    for tensors in (dfattn.paged_fork(table, lens, meta(6), 16, n_pages)[1:], dfattn.paged_free(table, lens, 16, n_pages),
+                    dfattn.paged_compact(table, lens, 16, n_pages)[1:]):
+        held = {t.untyped_storage()._cdata: t.untyped_storage().nbytes() for t in tensors}
+        assert sum(held.values()) == 4 * sum(t.numel() for t in tensors)
