@@ -194,8 +194,8 @@ def paged_plan(cached_lens, new_lens, block_table, free_pages, free_start, page_
     return seq_lens, query_start, slot_map, counts
 
 
-# A batch's rows after a fork: the new table and lengths, how often each page is held, the page ids (held ones, then free
-# ones), the first free one's place, the pairs of pages to copy and counts [2] = pairs, rows cut for want of a page.
+# A batch's rows after a fork: the new table and lengths, how often each page is held, the page ids (those held of the parents, the
+# new ones, the free ones, each rising), the first free one's place, the pairs of pages to copy and counts [2] = pairs, rows cut for want of a page.
 PagedFork = collections.namedtuple("PagedFork", "block_table seq_lens refs free_pages free_start copy_src copy_dst counts")
 PagedCompact = collections.namedtuple("PagedCompact", "block_table refs free_pages free_start copy_src copy_dst counts")
 

@@ -376,7 +376,7 @@ int dfattn_paged_plan(const uint32_t *cached_lens, const uint32_t *new_lens,
  * page, and a page that no row holds is free. These calls find that out from
  * the tables each time: refs [n_pages] receives how often each page is held,
  * free_pages [n_pages] all ids, first those held and then the free ones, each
- * in rising order, and free_start [1] the place of the first free one:
+ * in rising order (fork: see there), and free_start [1] the place of the first free one:
  * what dfattn_paged_plan takes (n_free = n_pages). Rows of a request that has ended
  * have the length 0.
  *
@@ -391,8 +391,9 @@ int dfattn_paged_plan(const uint32_t *cached_lens, const uint32_t *new_lens,
  * copy_src and copy_dst [n_children] (DFATTN_NO_SLOT behind the last). Where
  * no page is left, new_lens[i] falls to the last whole page. counts [2]: pairs,
  * and children cut like that. refs, free_pages and free_start are of the new
- * rows (with the new pages held). The free pages' contents are kept until they
- * are given out, so the copies may follow the call.
+ * rows; free_pages has first the pages that these hold of their parents, then the
+ * new ones (as copy_dst), then the free ones, each part in rising order. The free
+ * pages' contents are kept until they are given out, so the copies may follow the call.
  *
  * free: seq_lens[r] becomes 0 where ended[r] != 0 (ended may be NULL), and refs,
  * free_pages and free_start are of the rest.
