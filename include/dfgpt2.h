@@ -189,7 +189,8 @@ int dfgpt2_token_logprobs_backward(const void *logits, const uint32_t *tokens, c
  * quantize: w [out_features, in_features] (dtype DFATTN_KV_F32 or DFATTN_KV_BF16, rows row_stride elements
  * apart). The scale of a group is the bf16 number nearest to its largest magnitude / 7 (I4) or / 6 (E2M1), or to
  * (high - low) / 15 with low and high its extremes and 0 (U4; zero is -low / scale, rounded, at most 15); a code is
- * the nearest one, ties to even, at the border where that is past it. All roundings are exact ones of the quotients. A group of
+ * the value's quotient by the scale, rounded, plus 8 (I4) or zero (U4), or that of the nearest number (E2M1; ties to the even code), and
+ * the nearest of 0..15 where that is past them. Roundings are exact ones of the quotients, to the nearest, ties to even. A group of
  * zeros, or whose scale is below bf16's range, has the scale 0 and values 0; one with an infinity or NaN the scale NaN.
  * dequantize: the values, [out_features, in_features] contiguous, in dtype (exact in fp32, rounded to bf16).
  * linear: out [rows, out_features] = x W^T + bias, then GELU where gelu is not 0, then + residual, in dtype (x's
