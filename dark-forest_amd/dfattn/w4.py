@@ -15,7 +15,7 @@ from __future__ import annotations
 import collections
 
 from . import _check, _stream_ptr
-from .kv8 import _names, _on, _out, _ptr, _rows, _sizes, _u32
+from .kv8 import _names, _on, _out, _ptr, _rows, _too_large, _u32
 from .ops import ops_lib
 
 FORMATS = {"i4": 0, "u4": 1, "e2m1": 2}  # DFGPT2_W4_I4, DFGPT2_W4_U4, DFGPT2_W4_E2M1
@@ -40,22 +40,28 @@ def _weight(w, n):
     if k < 1 or codes.dim() != 2 or codes.shape[1] != row_bytes(k):
         raise ValueError(f"codes must be [outputs, {row_bytes(k)}] for {k} inputs")
     shape = (-(-k // group), codes.shape[0])
-    _sizes("codes", shape[1], k)
+    if (shape[1] | k) >> 32:
+        _too_large("codes")
     if scales.shape != shape or (fmt == "u4" and (zeros is None or zeros.shape != shape)):
         raise ValueError(f"scales (and the zeros of u4) must be {list(shape)}")
     return (_ptr(codes, "codes", torch.uint8, dev), _ptr(scales, "scales", n[3], dev),
             _ptr(zeros, "zeros", torch.uint8, dev) if fmt == "u4" else None, FORMATS[fmt], group, shape[1], k)
 
 
-def _no_gradient(torch, name, *tensors):
-    """Refuses a call that a gradient of `tensors`, or a tangent of forward mode (which torch.no_grad() leaves on), would be
-    lost in."""
+_forward_ad = None
+
+
+def _no_gradient(torch, name, tensors):
+    """Refuses a call that a gradient of one of `tensors`, or a tangent of forward mode (which torch.no_grad() leaves on),
+    would be lost in."""
+    global _forward_ad
+    if _forward_ad is None:
+        _forward_ad = torch.autograd.forward_ad
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
-    forward_ad = torch.autograd.forward_ad
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise ValueError(f"{name} has no gradient of forward mode: give it the primals")
 
 
@@ -68,7 +74,8 @@ def quantize(w, group=64, format="i4", stream=None):
     if w.dim() != 2 or not w.numel():
         raise ValueError("w must be [outputs, inputs] and not empty")
     n, k = w.shape
-    _sizes("w", n, k)
+    if (n | k) >> 32:
+        _too_large("w")
     p, stride, dtype = _rows(w, "w", k, names)
     with _on(stream, dev):
         codes = torch.empty((n, row_bytes(k)), dtype=torch.uint8, device=w.device)
@@ -87,7 +94,7 @@ def dequantize(w, dtype=None, out=None, stream=None):
         dtype = names[2] if out is None else out.dtype
     if dtype is not names[2] and dtype is not names[3]:
         raise ValueError("values are read as float32 or bfloat16")
-    _no_gradient(names[0], "dequantize", w.scales, out)
+    _no_gradient(names[0], "dequantize", (w[1], out))
     with _on(stream, names[6]):
         out, p = _out(out, "out", (n, k), dtype, w.codes.device, names)
     _check(ops_lib().dfgpt2_w4_dequantize(*ptrs, p, 0 if dtype is names[2] else 1, fmt, group, n, k, _stream_ptr(stream)))
@@ -107,9 +114,10 @@ def linear(x, w, bias=None, residual=None, gelu=False, out=None, workspace="auto
     dev = names[6]
     *ptrs, fmt, group, n, k = _weight(w, names)
     px, stride, dtype = _rows(x, "x", k, names)
-    _no_gradient(names[0], "linear", x, w.scales, bias, residual, out)
+    _no_gradient(names[0], "linear", (x, w[1], bias, residual, out))
     shape = (x.shape[0], n)
-    _sizes("x", shape[0])
+    if shape[0] >> 32:
+        _too_large("x")
     if bias is not None and bias.shape != (n,):
         raise ValueError(f"bias must be [{n}]")
     if residual is not None and residual.shape != shape:

@@ -126,7 +126,7 @@ def test_linear_refuses_tangents(here, wants, grad):
 
 
 # ---------------------------------------------------------------- memory
-@pytest.mark.parametrize("n_pages", [8193, 500000])
+@pytest.mark.parametrize("n_pages", [131073, 500000])
 def test_scratch_goes_with_the_call(here, monkeypatch, n_pages):
     """What a program keeps of a call from step to step keeps none of its workspace (8 bytes a page)."""
     class Lib:
