@@ -79,6 +79,10 @@ constexpr uint32_t kVectorRows = 2, kStreamRows = 16, kMatrixRows = 32, kMatrixO
 // 12.6 and 10.8; 2 rows, vector_kernel's 16 and 12, 14.7 and 10.6), of large ones (fp32: 4 rows of 4096 x 16384 19 to 22 and 18, 16
 // rows 25 and 19, but of 4096 x 4096 10 and 11; bf16: 16 rows of 8192 x 28672 48 and 40, of 4096 x 16384 15 and 16) and in
 // fp32 of many inputs for more than 8 rows (16 rows of 8192 x 1024 20 and 15, 8 rows 15 and 15).
+// Wide is the same number of outputs whatever the inputs. At that border (2 to 16 rows of 32752 and of 32768 outputs, i4; the
+// second is matrix_kernel) in fp32 64 inputs 5.0 to 7.5 and 4.5 to 5.3, 256 6.4 to 8.7 and 7.3 to 9.4, 768 9.5 to 13.1 and 10.5 to
+// 12.7; in bf16 256 inputs 5.5 to 6.9 and 6.8 to 8.9, 768 8.6 to 9.9 and 9.1 to 11.2, 2048 14.3 to 15.9 and 14.8 to 16.2, 3968
+// 25.2 to 28.5 and 23.3 to 24.5: with 256 to 768 inputs and bf16 the other kernels would still be up to a quarter faster there.
 enum Path { kVector, kStream, kMatrix };
 inline Path path_of(uint32_t M, uint32_t N, uint32_t K, bool bf16) {
   const uint64_t weights = (uint64_t)N * K;
@@ -91,7 +95,8 @@ inline Path path_of(uint32_t M, uint32_t N, uint32_t K, bool bf16) {
 
 // Splits of the inputs for matrix_kernel: up to 8, for no more than some 512 workgroups, or two where there are
 // up to 512 and many inputs (4096 x 4096 in bf16: 500 rows 42 us whole, 40 in two, 48 in four; 64 rows 23 us whole, 15 in four
-// and in eight).
+// and in eight). In fp32, where no two of the splits are one workgroup's, the sums' way through memory costs more than it
+// brings from some 400 rows on (500 rows of 4096 x 4096 70 us in two and 68 whole, 400 of 768 x 2304 17 and 14).
 inline uint32_t splits_of(uint32_t M, uint32_t N, uint32_t K) {
   const uint64_t groups = (uint64_t)((M + kMatrixRows - 1) / kMatrixRows) * ((N + kMatrixOutputs - 1) / kMatrixOutputs);
   const uint32_t tiles = (K + 127) / 128;

@@ -77,9 +77,10 @@ struct Divider {
 // A workgroup takes 32 outputs and 256 inputs: a lane 8 inputs of four outputs, 4 to 16 neighbours a
 // group. Each of four neighbours divides for one of the four outputs. The scales go through LDS, so that neighbouring
 // outputs' are written together.
-// Bound: from fp32 memory (16384 x 4096 to u4 55 us, 5.5 TB/s), from bf16 VALU too (49 us, 3.4 TB/s, to i4 41): extremes, one
-// double division a group and four neighbours, the product, its check and clamp for each value; 768 x 768 4 us, a launch's
-// latency. Workgroups of several blocks with the next one's loads ahead were slower (63 us, then 54 without).
+// Bound: from fp32 memory (16384 x 4096 to u4 55 us, 5.5 TB/s, VALU busy 53 % of the time), from bf16 VALU (u4 46 to 54 us, 3.1 to 3.7
+// TB/s, i4 41; busy 95 % of the time in both): extremes, one double division a group and four neighbours, the product, its
+// check and clamp for each value, and the correction, which three of five rows of a wave take where values have bf16's 8 bits (0.2 % of
+// them are half way; from fp32 hardly any). 768 x 768 4 to 6 us, a launch's latency. Workgroups of several blocks with the next one's loads ahead were slower (63 us, then 54 without).
 constexpr int kQuantRows = 32, kQuantCols = 256;
 template <Format F, bool BF16>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
@@ -169,7 +170,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
     if constexpr (F != kE2M1) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = by.first(x[r][j], &far);
-      // (Few values are next to a border: with the correction always 3 of 70 us more.)
+      // (Few fp32 values are next to a border: with the correction always 3 of 70 us more.)
       if (__any(some && !(far < by.near()))) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = by.nearest(x[r][j]);
@@ -208,7 +209,9 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(QuantArgs a) {
 
 // ---------------------------------------------------------------- values
 // A lane writes 16 bytes at a time, neighbours next to each other: 4 fp32 or 8 bf16 values of a row; kValueSteps
-// times 256 lanes a workgroup. Bound: the stores (16384 x 4096 to fp32 47 us, 6.4 TB/s; 768 x 768 4.2 us).
+// times 256 lanes a workgroup. Bound: to fp32 the stores (16384 x 4096 47 us into the same memory each time, part of which stays in the
+// Infinity Cache, 70 us into four in turn, 4.3 TB/s); to bf16 neither memory nor VALU (46 us, 3.7 TB/s, 56 %): each wave loads,
+// computes and stores in turn. 768 x 768 to fp32 3.8 us, to bf16, with half the workgroups, 5.7.
 constexpr uint32_t kValueSteps = 8;
 template <Format F, bool BF16>
 __global__ __launch_bounds__(kThreads) void dequantize_kernel(QuantArgs a) {

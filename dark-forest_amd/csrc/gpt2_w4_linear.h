@@ -109,9 +109,9 @@ __device__ __forceinline__ uint32_t xcd_block(uint32_t b, uint32_t n) {
 // rounds of swaps between the quarters of the wave make four operands of 32 consecutive inputs, so that a product stays
 // within a group. Each group's sum is scaled once, in fp32: out += s (sum q x - zero sum x), sum x by a product with ones.
 // The waves' sums meet in LDS in the order of the inputs.
-// Bound: with few weights latency (4 rows of 768 x 2304 in fp32 4.7 us, in bf16 4.0); with many the vector unit, which makes
-// operands of the codes and, in fp32, three terms of each activation in every wave (4 rows of 4096 x 16384 in bf16 13.4 us,
-// 2.6 TB/s of codes, in fp32 19). The activations straight from L2: through LDS was no faster.
+// Bound: with few weights latency (4 rows of 768 x 2304 in fp32 4.7 us, in bf16 4.0); with many what each wave has in flight (4 rows of
+// 4096 x 16384 in bf16 13.7 us, 2.5 TB/s of codes: the vector unit is busy 29 % of the time, the matrix pipe 7 %, and the
+// waves wait for half of theirs). The activations straight from L2: through LDS was no faster.
 template <Format F, bool BF16, int GROUP, int T>
 __global__ __launch_bounds__(512) void stream_kernel(LinearArgs a) {
   constexpr bool E2M1 = F == kE2M1;
@@ -324,9 +324,9 @@ __global__ __launch_bounds__(512) void stream_kernel(LinearArgs a) {
 // rows of codes together); the products are fp32 multiply-adds of exact code values. A lane's 32 inputs are in one
 // group: its sum is scaled once. At the end kLoads sums of L lanes are added by swaps that halve
 // their number with the lanes', then along 16 lanes.
-// Bound: with few weights latency (one row of 768 x 2304 3.3 us in fp32, a launch that does nothing 1.6); with many half
-// memory and half the vector unit, one multiply-add a code and row besides the conversions (4096 x 16384 in bf16 10.5 us,
-// 3.3 TB/s, stream_kernel 13; 8192 x 28672 28 us, 4.3). More codes in flight, or waves that stay for more outputs, no faster.
+// Bound: with few weights latency (one row of 768 x 2304 3.3 us in fp32, a launch that does nothing 1.6); with many
+// memory and the vector unit in turn, since all waves run in step: one multiply-add a code and row besides the conversions, 50 % of
+// the time (4096 x 16384 in bf16 10.5 us, 3.3 TB/s, stream_kernel 13; 8192 x 28672 28 us, 4.3). More codes in flight, or waves that stay for more outputs, no faster.
 __device__ __forceinline__ float row_sum(float v) {  // of 16 neighbouring lanes, in all of them
   v += dpp<0x128>(v);
   v += dpp<0x124>(v);
@@ -502,8 +502,11 @@ __global__ __launch_bounds__(512) void vector_kernel(LinearArgs a) {
 // Where rows and outputs give too few workgroups, `splits` share out the inputs and leave fp32 sums, which join_kernel adds.
 // Bound: the vector unit, which turns codes into operands once for every 32 rows, and the matrix pipe behind it (2000 rows of 4096 x
 // 4096 in bf16, groups of 128: 108 us, 620 TFLOP/s; VALU busy 47 %, matrix pipe 28 % of the time, hardly at once; without any loads or conversions
-// of codes the products alone take 70). More rows a workgroup, which would convert less often, need registers that the sums of a
-// group and of the layer take already: 64 rows and 256 outputs were both slower.
+// of codes the products alone take 70). More rows a wave, which would convert less often, need registers that the sums of a group and
+// of the layer take already: 64 rows and 256 outputs were both slower. Operands of codes made once for four waves, in LDS, were not tried.
+// With few rows of wide layers what is in flight: 16 rows of 768 x 50257, e2m1, are 393 workgroups of six steps for 256 CUs, a
+// barrier in each and one tile of codes ahead (fp32 12 us, vector unit 26 %, matrix pipe 11 %; bf16 10.8, 25 % and 5 %; the waves
+// wait for half of their time in both).
 // With HALVES = 2 eight waves do, four for each half of the inputs, and the halves' sums meet in LDS.
 template <Format F, bool BF16, int GROUP, int R, int HALVES>
 __global__ __launch_bounds__(kThreads * HALVES, 2) void matrix_kernel(LinearArgs a) {  // (2: no sums in accumulation registers)

@@ -199,9 +199,10 @@ int dfgpt2_token_logprobs_backward(const void *logits, const uint32_t *tokens, c
  * as the sum of three bf16 terms, exactly from 2^-100 on) and summed in fp32; a group's sum is scaled once. An infinity
  * or NaN in a row of x makes that row's results infinite or NaN; 32 times the sum of a row's magnitudes in a group,
  * and that times the group's scale, must stay below fp32's range. rows <= 2^20; features <= 2^24; outputs and workspace
- * must not overlap what is read. Workspace: dfgpt2_w4_linear_workspace_bytes (0: none needed; 4-byte aligned), one for
- * each call that may overlap; NULL: the inputs are not shared out, slower for some 17 to 200 rows, and for fewer of
- * large layers. Results are reproducible bit for bit. */
+ * must not overlap what is read. Workspace: dfgpt2_w4_linear_workspace_bytes (0: none needed; 4-byte aligned; enough for
+ * both types, of which bf16 may use half or none), one for each call that may overlap; NULL: the inputs are not shared out,
+ * slower for some 17 to 250 rows in fp32 and 17 to 500 in bf16 (4096 x 4096: 64 rows 50 us for 20 and 30 for 14, 500 bf16 rows 40 for
+ * 36), and in fp32 for fewer of large layers (16 rows of 4096 x 16384 25 for 19). Results are reproducible bit for bit. */
 #define DFGPT2_W4_I4 0u
 #define DFGPT2_W4_U4 1u
 #define DFGPT2_W4_E2M1 2u
