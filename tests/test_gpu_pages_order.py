@@ -77,3 +77,23 @@ def test_large_pools_captured(device):
             assert list(zip(c.copy_src.tolist(), c.copy_dst.tolist()))[:len(dense["copies"])] == dense["copies"]
             last = ref.free(rows, want["lens"], page, n_pages, gone)
             assert after.tolist() == last["lens"] and [x.tolist() for x in freed] == [last["refs"], last["free_pages"], [last["free_start"]]]
+
+
+@pytest.mark.parametrize("n_pages,page_bytes", [(70000, 65536), ((1 << 24) - 5, 272), ((1 << 24) - 5, 260), ((1 << 24) - 5, 257)])
+def test_copies_past_32_bits(device, n_pages, page_bytes):
+    """Pools of more than 2^32 bytes, in pieces of 16 (long and short pages), 4 and 1 bytes: what is copied, and what stays."""
+    pool = torch.zeros(n_pages, page_bytes, dtype=torch.int8, device="cuda")
+    assert pool.nbytes > 1 << 32
+    far = n_pages - 1
+    border = (1 << 32) // page_bytes  # the page across 2^32 bytes
+    src, dst = [far, 3, border, 7], [0, border + 1, 5, far - 1]
+    g = torch.Generator(device="cuda").manual_seed(page_bytes)
+    for p in src:
+        pool[p] = torch.randint(-128, 128, (page_bytes,), generator=g, device="cuda", dtype=torch.int8)
+    want = {p: pool[p].clone() for p in src}
+    want.update({d: pool[s].clone() for s, d in zip(src, dst)})
+    dfattn.paged_copy([pool], i32(src), i32(dst))
+    for p, w in want.items():
+        assert torch.equal(pool[p], w), p
+        pool[p] = 0
+    assert not pool.view(torch.int8).any()

@@ -87,3 +87,24 @@ def test_u4(device, group, dtype):
     assert max(map(len, rows)) <= 32
     got, scales, z = codes_of(rows, group, "u4", dtype)
     assert scales == steps and z == zeros and got == want
+
+
+def test_past_32_bits(device):
+    """A matrix of more than 2^32 weights: rows of it against the same rows by themselves, quantised and read back."""
+    n, k, rows = 70000, 65536, 6
+    pick = [0, 1, 32768, 65535, 65536, n - 1]
+    g = torch.Generator(device="cuda").manual_seed(2)
+    few = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+    w = torch.zeros(n, k, dtype=torch.bfloat16, device="cuda")
+    assert w.numel() > 1 << 32
+    w[pick] = few
+    for fmt in ("i4", "u4", "e2m1"):
+        q, small = w4.quantize(w, 128, fmt), w4.quantize(few, 128, fmt)
+        assert torch.equal(q.codes[pick], small.codes) and torch.equal(q.scales[:, pick], small.scales)
+        assert q.zeros is None or torch.equal(q.zeros[:, pick], small.zeros)
+        for dtype in (torch.bfloat16, torch.float32):
+            values = w4.dequantize(q, dtype)
+            assert torch.equal(values[pick], w4.dequantize(small, dtype))
+            values[pick] = 0
+            assert not values.any()
+            del values
